@@ -41,6 +41,7 @@ extern "C" {
 #define QVL_DTYPE_FP16 2
 #define QVL_DTYPE_INT8 3
 #define QVL_DTYPE_INT4 4
+#define QVL_DTYPE_BF16 5         /* not in the reference's enum */
 
 /* Floating-point summation semantics of the INT8 products.
  * The integer group sums are exact in all modes; the modes differ only in how
@@ -427,6 +428,94 @@ int *qvl_text_decode_abort_flag(void *workspace);
  * global-timer stamps (ns) of the last call -- [0] kernel start, [1 + i] the
  * opening of grid barrier i (5 per layer + 1 barriers per token). */
 const uint64_t *qvl_text_decode_trace(const void *workspace);
+
+/* ---- drafted and multimodal tokens over the paged cache -----------------
+ * No counterpart in the reference (it decodes one token of one request at a
+ * time, at text positions).  One step of a batch of requests whose draft is a
+ * tree: plan the pages and slots of its tokens, per layer write their keys
+ * and values to the slots (qvl_qknorm_mrope_kv_append) and attend
+ * (qvl_tree_attention), score them (qvl_token_logprobs), and plan once more
+ * with the lengths that were accepted.  The floating types are
+ * QVL_DTYPE_FP32, _FP16 and _BF16. */
+
+/* Page tables and slot maps from request lengths, on the device.
+ * Request s holds ceil(old_lengths[s] / page_size) pages, the first entries
+ * of its row of page_table [n_seqs, max_pages_per_seq], and is to hold
+ * ceil(new_lengths[s] / page_size) of them (at most max_pages_per_seq; a
+ * negative length counts as 0).  free_pages[0, free_count) is a stack of free
+ * pages, of `capacity` entries in all.  Requests that shrink push the pages they
+ * no longer need, in request order, lowest page first; requests that grow
+ * then pop theirs in request order, and find -1 where the stack is empty.
+ * Tokens new_lengths - old_lengths > 0 are packed in request order:
+ *   starts [n_seqs + 1]  first token of each request (prefix sums)
+ *   seq_ids, positions, slots [max_tokens]  each token's request, its position
+ *       and its slot page * page_size + offset (-1: no page); entries past the
+ *       last token are -1, tokens past max_tokens are left out
+ *   missing [1]  tokens that no page was left for
+ * The step's state is written so that it can be dropped: page_table changes
+ * at or past the old pages of growing requests, free_pages at or past
+ * *free_count, and free_count_out is a word of its own.  A caller that finds
+ * missing > 0 plans again from the same lengths and the same free_count with
+ * smaller new_lengths.  n_seqs <= 16384; fewer than 2^31 tokens in all. */
+int qvl_plan_pages(const int32_t *old_lengths, const int32_t *new_lengths, size_t n_seqs, int32_t *page_table,
+                   int page_size, int max_pages_per_seq, int32_t *free_pages, const int32_t *free_count,
+                   size_t capacity, int32_t *free_count_out, int32_t *missing, int32_t *starts, int32_t *seq_ids,
+                   int32_t *positions, int32_t *slots, size_t max_tokens, void *stream);
+
+/* RMS norm of every query and key head, rotary positions with several axes
+ * (time, height, width of image and video tokens), and the write of keys and
+ * values to their cache slots, in one pass.  q [n_tokens, NH, D], k and v
+ * [n_tokens, NKV, D] of `dtype` with *_stride elements between tokens (rows
+ * of one fused projection will do); q_out [n_tokens, NH, D] of the same type,
+ * contiguous, may be q itself.  Pair (i, i + D/2) of token t is turned by row
+ * positions[axes[i] * pos_stride + t], column i of rope_cos / rope_sin [max_pos,
+ * D/2]; axes [D/2] in [0, n_axes).  Keys and values are rounded to kv_dtype
+ * (FP16 or BF16) and written at slots[t] of pages [num_pages, NKV, page_size,
+ * D]; a token whose slot is outside the cache (-1: padding) writes nothing.  A
+ * token with a position outside the table gets zeros in q_out and writes
+ * nothing.  Slots must differ.  Norm weights [D]: INT8 with fp32 scales
+ * [D / norm_group], or a float type (scales NULL); both NULL: no norm.
+ * D 64, 128 or 256; rows 16-byte aligned. */
+int qvl_qknorm_mrope_kv_append(const void *q, const void *k, const void *v, int dtype, size_t q_stride, size_t k_stride,
+                               size_t v_stride, void *q_out, void *k_pages, void *v_pages, int kv_dtype,
+                               size_t num_pages, const int32_t *slots, const int32_t *positions, size_t pos_stride,
+                               int n_axes, const int32_t *axes, size_t n_tokens, const float *rope_cos,
+                               const float *rope_sin, const void *q_norm_w, const float *q_norm_s,
+                               const void *k_norm_w, const float *k_norm_s, int norm_dtype, size_t norm_group,
+                               float eps, const qvl_attn_dims *dims, void *stream);
+
+/* Attention of a tree of drafted tokens over the paged cache.  Node i of
+ * request s is row starts[s] + i of q [n_rows, NH, D] (q_stride elements between
+ * rows); its key and value are in the cache at position ctx_lens[s] + i of row
+ * s of page_table.  It sees positions [0, ctx_lens[s]) and, of the nodes, itself and
+ * its ancestors: parents[row] is the parent's index in its request, less than i; any
+ * other value marks a root.  out [n_rows, NH, D] of q's type = softmax(scale
+ * q k^T) v; masked keys and values have no influence whatever they hold, and
+ * positions past the page table's width, or on pages outside [0, num_pages), do not
+ * exist.  A row that sees nothing, a row of q outside [starts[0], starts[n_seqs]) and a
+ * node past max_nodes get zeros.  max_ctx, a bound of ctx_lens + nodes, only
+ * shapes the launch.  Types (q, cache): fp32 or fp16 over fp16, bf16 over
+ * bf16.  D 64 or 128, max_nodes <= 256, page_size a multiple of 16. */
+size_t qvl_tree_attention_workspace_bytes(size_t n_seqs, size_t n_rows, int max_ctx, int max_nodes,
+                                          const qvl_attn_dims *dims);
+int qvl_tree_attention(const void *q, int dtype, size_t q_stride, const void *k_pages, const void *v_pages,
+                       int kv_dtype, size_t num_pages, const int32_t *page_table, const int32_t *ctx_lens,
+                       const int32_t *starts, const int32_t *parents, size_t n_seqs, size_t n_rows, int max_ctx,
+                       int max_nodes, float scale, void *out, const qvl_attn_dims *dims, void *workspace,
+                       size_t workspace_bytes, void *stream);
+
+/* Log-probabilities of given tokens: logprobs[r] = logits[r, tokens[r]] -
+ * log sum exp(logits[r, :]) (0 for a token outside [0, vocab): nothing was asked),
+ * entropy[r] (nullable) of the row's distribution in nats, and its top_k
+ * largest entries (top_k <= 64, 0 for none): top_ids and top_logprobs [n_rows,
+ * top_k], largest first, equal logits by lower index.  -inf logits (masked
+ * tokens) have no weight; in a row of nothing else every log-probability is
+ * -inf and the entropy 0.  NaN is never among the top entries; what they leave
+ * empty has id -1.  logits of `dtype`, `stride` elements between rows, any
+ * alignment. */
+int qvl_token_logprobs(const void *logits, int dtype, size_t stride, const int32_t *tokens, size_t n_rows, size_t vocab,
+                       int top_k, float *logprobs, float *entropy, int32_t *top_ids, float *top_logprobs,
+                       void *stream);
 
 /* ---- vision tower (FP16 weights; forward_img, model/src/forward.cpp:3-456)
  * fp16 tensors are passed as uint16_t.  Token-major layouts throughout:

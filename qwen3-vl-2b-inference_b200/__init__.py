@@ -19,6 +19,10 @@ this module            reference
 ``greedy_decode``      ``greedy_decode``, tokenizer/src/utils.cpp:34-44
 =====================  ==========================================================
 
+and, with no counterpart there, the operators that serve drafted (speculative)
+and multimodal tokens over the paged cache: ``plan_pages``,
+``qknorm_mrope_kv_append``, ``tree_attention``, ``token_logprobs``.
+
 Tensors are torch CUDA tensors (torch supplies device memory and streams
 only).  There is no CPU fallback: if the library is missing, importing this
 module raises.  An unsupported combination raises ``QvlError`` (the
@@ -36,7 +40,7 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG_DIR, "lib", "libqvl_b200.so")
 
 SEM_REFERENCE, SEM_LANE8, SEM_TILED = 0, 1, 2
-DTYPE_FP32, DTYPE_INT32, DTYPE_FP16, DTYPE_INT8, DTYPE_INT4 = 0, 1, 2, 3, 4
+DTYPE_FP32, DTYPE_INT32, DTYPE_FP16, DTYPE_INT8, DTYPE_INT4, DTYPE_BF16 = 0, 1, 2, 3, 4, 5
 
 EXPORTED = (
     "qvl_status_string", "qvl_last_cuda_error", "qvl_version", "qvl_quantize_rows",
@@ -51,6 +55,8 @@ EXPORTED = (
     "qvl_text_decode_abort_flag", "qvl_text_decode_trace", "qvl_tc_timeout_status",
     "qvl_attention_decode_static", "qvl_attention_ordered_workspace_bytes", "qvl_attention_decode_ordered",
     "qvl_rope_table", "qvl_quantize_rows_planes", "qvl_qknorm_rope_attention_decode_ordered", "qvl_rms_norm_i8_planes", "qvl_linear_planes_i8_batched",
+    "qvl_plan_pages", "qvl_qknorm_mrope_kv_append", "qvl_tree_attention_workspace_bytes", "qvl_tree_attention",
+    "qvl_token_logprobs",
 )
 SEM_ACCUMULATE = 0x100
 
@@ -145,6 +151,14 @@ def load_library(path: str = LIB_PATH):
     L.qvl_rms_norm_i8_planes.argtypes = [_P] * 8 + [_Z, _Z, _Z, ctypes.c_float, _I, _P]
     L.qvl_linear_planes_i8_batched.argtypes = [_P, _P, _P, _Z, _P, _P, _P, _P, _Z, _Z, _I, _P]
     L.qvl_internal_set_tc_timeout.argtypes = [_P]
+    L.qvl_plan_pages.argtypes = [_P, _P, _Z, _P, _I, _I, _P, _P, _Z] + [_P] * 6 + [_Z, _P]
+    L.qvl_qknorm_mrope_kv_append.argtypes = ([_P] * 3 + [_I, _Z, _Z, _Z] + [_P] * 3 + [_I, _Z, _P, _P, _Z, _I, _P, _Z] +
+                                             [_P] * 6 + [_I, _Z, ctypes.c_float, ctypes.POINTER(AttnDims), _P])
+    L.qvl_tree_attention_workspace_bytes.restype = _Z
+    L.qvl_tree_attention_workspace_bytes.argtypes = [_Z, _Z, _I, _I, ctypes.POINTER(AttnDims)]
+    L.qvl_tree_attention.argtypes = ([_P, _I, _Z, _P, _P, _I, _Z] + [_P] * 4 + [_Z, _Z, _I, _I, ctypes.c_float, _P,
+                                     ctypes.POINTER(AttnDims), _P, _Z, _P])
+    L.qvl_token_logprobs.argtypes = [_P, _I, _Z, _P, _Z, _Z, _I] + [_P] * 5
     _lib = L
     return L
 
@@ -566,4 +580,207 @@ def attention_q16(q, kv: PagedKV, seq_ids, positions, max_ctx, out, q_out, q_out
                                       _ptr(seq_ids), _ptr(positions), nq, max_ctx, _ptr(out), _ptr(q_out),
                                       _ptr(q_out_scales), _ptr(counter), ctypes.byref(kv.dims), _ptr(ws),
                                       ws.numel(), _stream(stream)), "attention_q16")
+    return out
+
+
+# ------------------------------------------------- drafted and multimodal tokens
+_FLOAT_DTYPES = {torch.float32: DTYPE_FP32, torch.float16: DTYPE_FP16, torch.bfloat16: DTYPE_BF16}
+
+
+def _dtype(t: torch.Tensor) -> int:
+    d = _FLOAT_DTYPES.get(t.dtype)
+    if d is None:
+        raise QvlError(f"expected a tensor of fp32, fp16 or bf16, got {t.dtype}")
+    return d
+
+
+def _i32(t: torch.Tensor, n: int | None = None, what: str = "index") -> int:
+    """Pointer of a contiguous int32 tensor of n values."""
+    if t.dtype != torch.int32 or (n is not None and t.numel() != n):
+        raise QvlError(f"{what}: expected int32{'' if n is None else f' [{n}]'}, got {t.dtype} {tuple(t.shape)}")
+    return _ptr(t)
+
+
+def _rows(t: torch.Tensor, shape, what: str) -> int:
+    """Pointer of a tensor of `shape` whose rows (all but the first dimension)
+    are contiguous; rows may lie apart."""
+    if not t.is_cuda:
+        raise QvlError(f"{what}: expected a CUDA tensor")
+    if tuple(t.shape) != tuple(shape):
+        raise QvlError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    st, want = t.stride(), 1
+    for i in range(t.dim() - 1, 0, -1):
+        if t.shape[i] != 1 and st[i] != want:
+            raise QvlError(f"{what}: each token's values must be contiguous")
+        want *= t.shape[i]
+    return t.data_ptr()
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Elements between rows (of one row: its width, whatever the stride says)."""
+    return t.stride(0) if t.shape[0] > 1 else t[0].numel() if t.shape[0] else t.stride(0)
+
+
+class PagePlan:
+    """What plan_pages writes: one int32 buffer with views of it."""
+
+    def __init__(self, n_seqs: int, max_tokens: int, device):
+        self.n_seqs, self.max_tokens = n_seqs, max_tokens
+        buf = self.buf = torch.empty(n_seqs + 3 + 3 * max_tokens, dtype=torch.int32, device=device)
+        self.free_count, self.missing, self.starts = buf[0:1], buf[1:2], buf[2:n_seqs + 3]
+        self.seq_ids, self.positions, self.slots = buf[n_seqs + 3:].view(3, max_tokens)
+
+
+def plan_pages(old_lengths, new_lengths, page_table, free_pages, free_count, page_size, max_tokens,
+               plan: PagePlan | None = None, stream=None) -> PagePlan:
+    """Page tables and slot maps from request lengths (int32 [S] each), on the GPU.
+
+    Requests that shrink push the pages they no longer need onto the stack
+    free_pages[:free_count], requests that grow pop theirs off it; page_table
+    [S, max_pages] and free_pages are updated in place, the stack's new size is
+    plan.free_count.  plan.starts [S + 1], .seq_ids, .positions and .slots
+    [max_tokens] describe the new tokens, packed in request order (-1: padding,
+    or no page left: plan.missing counts these tokens).  A plan that is not
+    wanted is dropped by keeping the old lengths and the old free_count."""
+    S = old_lengths.numel()
+    if page_table.dim() != 2 or page_table.shape[0] != S:
+        raise QvlError(f"page_table: expected {S} rows, got {tuple(page_table.shape)}")
+    if plan is None:
+        plan = PagePlan(S, max_tokens, old_lengths.device)
+    elif plan.n_seqs != S or plan.max_tokens != max_tokens:
+        raise QvlError("plan was made for another number of requests or tokens")
+    p = plan.buf.data_ptr()
+    tok = p + 4 * (S + 3)
+    _check(load_library().qvl_plan_pages(
+        _i32(old_lengths, S, "old_lengths"), _i32(new_lengths, S, "new_lengths"), S, _i32(page_table, None, "page_table"),
+        page_size, page_table.shape[1], _i32(free_pages, None, "free_pages"), _i32(free_count, 1, "free_count"),
+        free_pages.numel(), p, p + 4, p + 8, tok, tok + 4 * max_tokens, tok + 8 * max_tokens, max_tokens,
+        _stream(stream)), "plan_pages")
+    return plan
+
+
+def mrope_axes(sections, interleaved: bool = True, device="cuda") -> torch.Tensor:
+    """int32 [sum(sections)]: the position axis of each rotary frequency.
+    Contiguous sections, or interleaved: axes 1, 2, ... take every n-th frequency from
+    their own index on, as often as their section says, and axis 0 the rest."""
+    n, A = sum(sections), len(sections)
+    if interleaved:
+        a = np.zeros(n, np.int32)
+        for axis in range(1, A):
+            a[axis:A * sections[axis]:A] = axis
+        if [int((a == i).sum()) for i in range(A)] != list(sections):
+            raise QvlError(f"sections {tuple(sections)} do not interleave")
+    else:
+        a = np.repeat(np.arange(A, dtype=np.int32), sections)
+    return torch.from_numpy(a).to(device)
+
+
+def _norm_weight(w, D, what):
+    """(pointer, scales, dtype, group) of a norm weight: None, a float tensor [D]
+    or (int8 [D], fp32 scales [D / group], group)."""
+    if w is None:
+        return None, None, DTYPE_FP32, 0
+    if isinstance(w, tuple):
+        w, s, group = w
+        if w.dtype != torch.int8 or s.dtype != torch.float32 or w.numel() != D or s.numel() * group != D:
+            raise QvlError(f"{what}: expected int8 [{D}] with fp32 scales [{D} / group]")
+        return _ptr(w), _ptr(s), DTYPE_INT8, group
+    if w.numel() != D:
+        raise QvlError(f"{what}: expected {D} weights")
+    return _ptr(w), None, _dtype(w), 0
+
+
+def qknorm_mrope_kv_append(q, k, v, kv: PagedKV, slots, positions, axes, rope_cos, rope_sin, q_norm=None, k_norm=None,
+                           eps=1e-6, out=None, stream=None):
+    """Norms of the query and key heads, rotary positions with several axes
+    and the write of keys and values to their cache slots, in one pass.
+
+    q [T, NH, D], k, v [T, NKV, D] (fp32, fp16 or bf16; a token's values
+    contiguous, tokens may lie apart); slots int32 [T] (-1: nothing is written);
+    positions int32 [n_axes, T]; axes int32 [D/2] (mrope_axes); q_norm, k_norm:
+    None, a float weight [D] or (int8 weight, fp32 scales, group).  Returns the
+    normed, rotated queries (out, or a new tensor; out may be q)."""
+    T, NH, D = q.shape
+    d = kv.dims
+    if (NH, D) != (d.num_heads, d.head_dim):
+        raise QvlError(f"q: expected {d.num_heads} heads of {d.head_dim}, got {NH} of {D}")
+    dt, kdt = _dtype(q), _dtype(kv.k)
+    if k.dtype != q.dtype or v.dtype != q.dtype or kv.v.dtype != kv.k.dtype:
+        raise QvlError("q, k and v must have one type, and so must the cache's two halves")
+    if out is None:
+        out = torch.empty((T, NH, D), dtype=q.dtype, device=q.device)
+    elif out.dtype != q.dtype or out.shape != q.shape:
+        raise QvlError("out must have q's shape and type")
+    if positions.dim() != 2 or positions.shape[1] != T or axes.numel() != D // 2:
+        raise QvlError(f"positions: expected [axes, {T}], axes: [{D // 2}]")
+    if rope_cos.shape != rope_sin.shape or rope_cos.shape != (d.max_pos, D // 2) or rope_cos.dtype != torch.float32 or \
+            rope_sin.dtype != torch.float32:
+        raise QvlError(f"rope tables: expected fp32 [{d.max_pos}, {D // 2}]")
+    qw, qs, wd, g = _norm_weight(q_norm, D, "q_norm")
+    kw, ks, wd2, g2 = _norm_weight(k_norm, D, "k_norm")
+    if (wd, g) != (wd2, g2):
+        raise QvlError("q_norm and k_norm must be of one kind")
+    shape = (T, d.num_kv_heads, D)
+    _check(load_library().qvl_qknorm_mrope_kv_append(
+        _rows(q, (T, NH, D), "q"), _rows(k, shape, "k"), _rows(v, shape, "v"), dt, _row_stride(q), _row_stride(k),
+        _row_stride(v), _ptr(out), _ptr(kv.k), _ptr(kv.v), kdt, kv.k.shape[0], _i32(slots, T, "slots"),
+        _i32(positions, None, "positions"), T, positions.shape[0], _i32(axes, None, "axes"), T, _ptr(rope_cos),
+        _ptr(rope_sin), qw, qs, kw, ks, wd, g, eps, ctypes.byref(d), _stream(stream)), "qknorm_mrope_kv_append")
+    return out
+
+
+def tree_attention(q, kv: PagedKV, ctx_lens, starts, parents, max_ctx, max_nodes, scale=None, out=None, workspace=None,
+                   stream=None):
+    """Attention of trees of drafted tokens over the paged cache.
+
+    Row starts[s] + i of q [T, NH, D] is node i of request s (row s of kv's page
+    table); its key and value are in the cache at position ctx_lens[s] + i.  It
+    sees positions [0, ctx_lens[s]), itself and its ancestors: parents[row] is
+    its parent's index in the request (-1: a root).  max_ctx bounds ctx_lens +
+    nodes, max_nodes the nodes of a request (<= 256).  fp32 or fp16 queries
+    over an fp16 cache, bf16 over bf16; rows that see nothing get zeros."""
+    T, NH, D = q.shape
+    d = kv.dims
+    if (NH, D) != (d.num_heads, d.head_dim):
+        raise QvlError(f"q: expected {d.num_heads} heads of {d.head_dim}, got {NH} of {D}")
+    S = ctx_lens.numel()
+    if kv.page_table.shape[0] < S or kv.v.dtype != kv.k.dtype:
+        raise QvlError("the page table has fewer rows than there are requests, or the cache has two types")
+    if out is None:
+        out = torch.empty((T, NH, D), dtype=q.dtype, device=q.device)
+    elif out.dtype != q.dtype or out.shape != q.shape:
+        raise QvlError("out must have q's shape and type")
+    L = load_library()
+    dims = ctypes.byref(d)
+    ws = _ws(workspace, q.device).get(L.qvl_tree_attention_workspace_bytes(S, T, max_ctx, max_nodes, dims))
+    _check(L.qvl_tree_attention(
+        _rows(q, (T, NH, D), "q"), _dtype(q), _row_stride(q), _ptr(kv.k), _ptr(kv.v), _dtype(kv.k), kv.k.shape[0],
+        _i32(kv.page_table, None, "page_table"), _i32(ctx_lens, S, "ctx_lens"), _i32(starts, S + 1, "starts"),
+        _i32(parents, T, "parents"), S, T, max_ctx, max_nodes, D ** -0.5 if scale is None else scale, _ptr(out), dims,
+        _ptr(ws), ws.numel(), _stream(stream)), "tree_attention")
+    return out
+
+
+class TokenLogprobs:
+    """What token_logprobs writes: logprobs, entropy [T], top_ids, top_logprobs [T, k]."""
+
+    def __init__(self, rows: int, top_k: int, device):
+        self.logprobs, self.entropy = torch.empty((2, rows), dtype=torch.float32, device=device)
+        self.top_ids = torch.empty((rows, top_k), dtype=torch.int32, device=device)
+        self.top_logprobs = torch.empty((rows, top_k), dtype=torch.float32, device=device)
+
+
+def token_logprobs(logits, tokens, top_k=0, out: TokenLogprobs | None = None, stream=None) -> TokenLogprobs:
+    """Log-probability of tokens[r] (int32 [T]; outside the vocabulary: 0) under
+    each row of logits [T, V] (fp32, fp16, bf16; rows may lie apart), the row's
+    entropy in nats and its top_k alternatives (<= 64), ties to the lowest id."""
+    T, V = logits.shape
+    if out is None:
+        out = TokenLogprobs(T, top_k, logits.device)
+    elif tuple(out.top_ids.shape) != (T, top_k):
+        raise QvlError("out was made for another number of rows or alternatives")
+    _check(load_library().qvl_token_logprobs(
+        _rows(logits, (T, V), "logits"), _dtype(logits), max(_row_stride(logits), V), _i32(tokens, T, "tokens"), T, V,
+        top_k, out.logprobs.data_ptr(), out.entropy.data_ptr(), out.top_ids.data_ptr(), out.top_logprobs.data_ptr(),
+        _stream(stream)), "token_logprobs")
     return out
