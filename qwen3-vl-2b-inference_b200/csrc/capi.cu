@@ -12,6 +12,7 @@
 #include "swiglu.cuh"
 #include "attention_ordered.cuh"
 #include "gemm_f16_tc.cuh"
+#include "serving.cuh"
 #include "attention.cuh"
 #include "argmax.cuh"
 #include "norm.cuh"
@@ -155,15 +156,15 @@ int qvl_rope_table(int theta, int head_dim, int rows, float *cos_out, float *sin
 
 int qvl_tc_timeout_status(int *timed_out, int clear, void *stream) {
     if (!timed_out) return QVL_ERR_INVALID;
-    int *words[2] = {qvl::gemm_tc_timeout_word(), qvl::gemm_f16_timeout_word()};
-    if (!words[0] || !words[1]) return QVL_ERR_CUDA;
+    int *words[3] = {qvl::gemm_tc_timeout_word(), qvl::gemm_f16_timeout_word(), qvl::tree_timeout_word()};
+    if (!words[0] || !words[1] || !words[2]) return QVL_ERR_CUDA;
     cudaStream_t st = (cudaStream_t)stream;
-    int v[2] = {0, 0};
-    for (int i = 0; i < 2; ++i) QVL_CUDA_TRY(cudaMemcpyAsync(&v[i], words[i], sizeof(int), cudaMemcpyDeviceToHost, st));
+    int v[3] = {0, 0, 0};
+    for (int i = 0; i < 3; ++i) QVL_CUDA_TRY(cudaMemcpyAsync(&v[i], words[i], sizeof(int), cudaMemcpyDeviceToHost, st));
     QVL_CUDA_TRY(cudaStreamSynchronize(st));
-    *timed_out = (v[0] | v[1]) != 0;
+    *timed_out = (v[0] | v[1] | v[2]) != 0;
     if (clear && *timed_out) {
-        for (int i = 0; i < 2; ++i) QVL_CUDA_TRY(cudaMemsetAsync(words[i], 0, sizeof(int), st));
+        for (int i = 0; i < 3; ++i) QVL_CUDA_TRY(cudaMemsetAsync(words[i], 0, sizeof(int), st));
         QVL_CUDA_TRY(cudaStreamSynchronize(st));
     }
     return QVL_OK;
