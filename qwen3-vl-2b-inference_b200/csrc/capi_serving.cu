@@ -103,8 +103,7 @@ size_t qvl_tree_attention_workspace_bytes(size_t n_seqs, size_t n_rows, int max_
     if (!dims_ok(dims) || n_seqs == 0 || n_seqs > 65535 || n_rows > (1u << 26) || max_ctx <= 0 || max_nodes <= 0 ||
         max_nodes > qvl::kTreeMaxNodes || (dims->head_dim != 64 && dims->head_dim != 128))
         return 0;
-    return qvl::tree_workspace_bytes((int)n_seqs, (int)n_rows, max_ctx, max_nodes, dims->num_heads, dims->num_kv_heads,
-                                     dims->head_dim);
+    return qvl::tree_workspace_bytes(dims->head_dim);
 }
 
 int qvl_tree_attention(const void *q, int dtype, size_t q_stride, const void *k_pages, const void *v_pages,
@@ -133,9 +132,8 @@ int qvl_tree_attention(const void *q, int dtype, size_t q_stride, const void *k_
     if (!al16(k_pages) || !al16(v_pages) || !al16(out) || !al4(page_table) || !al4(ctx_lens) || !al4(starts) ||
         !al4(parents))
         return QVL_ERR_INVALID;
-    const size_t need = qvl::tree_workspace_bytes((int)n_seqs, (int)n_rows, max_ctx, max_nodes, dims->num_heads,
-                                                  dims->num_kv_heads, D);
-    if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255))) return QVL_ERR_WORKSPACE;
+    if (!workspace || workspace_bytes < qvl::tree_workspace_bytes(D) || ((uintptr_t)workspace & 255))
+        return QVL_ERR_WORKSPACE;
     qvl::TreeArgs a{};
     a.q = q; a.q_stride = (long)q_stride; a.k_pages = k_pages; a.v_pages = v_pages; a.num_pages = (long)num_pages;
     a.table = page_table; a.ctx_lens = ctx_lens; a.starts = starts; a.parents = parents;

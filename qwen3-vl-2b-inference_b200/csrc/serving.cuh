@@ -72,7 +72,7 @@ struct TreeArgs {
     int dtype, kv_dtype;
     void *workspace;
 };
-size_t tree_workspace_bytes(int S, int T, int max_ctx, int max_nodes, int NH, int NKV, int D);
+size_t tree_workspace_bytes(int D);
 cudaError_t launch_tree_attention(const TreeArgs &a, cudaStream_t st);
 // device address (current device) of the kernel's timeout word, or nullptr
 int *tree_timeout_word();

@@ -7,35 +7,41 @@
 // that names no earlier node counts as a root.
 //
 // The query rows of one request that share a key head (nodes x heads per
-// key head) read the same keys and values: 512 bytes a position (D 128) for up to
-// NC rows.  Up to ~128 rows that is bound by memory, so the cache is to be
-// read once and everything else has to hide behind it.
+// key head) read the same keys and values, 512 bytes a position at D 128.  Up to 128
+// such rows are one tile of the tensor cores' long side, so that the cache is
+// read once; with 6.5 TB/s of memory a tile of 128 positions (64 KB) then has 1.5
+// us of one SM's time, and everything else has to hide behind it.
 //
-// Both products run on the tensor cores with the *cache* as the 128-row
-// operand and the query rows as its columns, so that any number of rows from 1
-// up fills the tile's long side:
-//   S^T [128 positions, NC rows] = K [128, D] . Q^T          (K as TMA wrote it)
-//   O^T [D, NC rows]            = V^T [D, 128] . P^T         (V as TMA wrote it, read
-//                                                            along its rows)
-// One CTA takes one request, key head, tile of NC rows and slice of the
-// context.  Warps: one softmax warpgroup (two for 64 rows: half the columns each;
-// thread = position), one warpgroup that sums the output (thread = value of
-// the head), a warp for the TMA loads and one for the MMAs.  Per tile of 128
-// positions:
-//   maxima of the columns over a warp's 32 positions (redux.f32), joined over
-//   the warps in shared memory, p = 2^(s - m) -> shared memory, PV into a fresh
-//   accumulator, and acc = acc * 2^(m_old - m) + PV in fp32 registers: the
-//   tensor cores' accumulation is not rounded to nearest, so no chain of it is
-//   longer than a tile.
+// Work: a unit is a tile of 128 positions of one (request, key head, 128 rows).
+// All units in a row are cut into one equal stretch per CTA, one CTA
+// per SM, whatever the requests' lengths are; a stretch is a few segments,
+// each a range of one pair's tiles.  A segment that is a whole pair writes its
+// rows; parts of a pair go to the workspace and meet in tree_join_kernel.
+//
+// Warps of a CTA:
+//   TMA      cuts the stretch into segments, finds the pages, fills a ring of slots for K
+//            and one for V (a slot: 128 positions, 128-byte swizzle)
+//   MMA      S = Q K^T [128 rows, 128 positions], O = P V [128 rows, D], one thread;
+//            S, P and O in tensor memory, two buffers each, P over S
+//   softmax  two warpgroups, half of a tile's positions each; thread = row, so that maximum
+//            and sum need one exchange with the partner warp.  The maximum is left as it is
+//            until a score passes it by 2^7, which p held times 2^8 in fp16 allows: almost
+//            no tile rescales anything
+//   sums     two warpgroups (half of D each) add each tile's O to fp32 registers: the
+//            tensor cores do not round their sums to nearest, so no chain of them is
+//            longer than a tile; and they bring the next segment's Q to shared memory
+//   fixer    the nodes' ancestors as bits, and values of the drafted tile that some
+//            row does not see: 0 * NaN
 // fp32 queries are split q = hi + lo (fp16 each, after a power of two per row
-// that keeps both in fp16's normal range), and the probabilities
-// p = hi + lo as well, 22 bits in all: the products of 16-bit values are exact in the
-// tensor core, so fp32 outputs keep fp32 accuracy, and the second products hide
-// behind the cache's loads.  16-bit queries are exact as they are.
-// The slices of a context meet in a second launch (tree_join_kernel).
+// that keeps both in fp16's normal range) and all probabilities p = hi + lo,
+// 22 bits in all (bf16: 16): the products of 16-bit values are exact in the tensor
+// cores, so fp32 outputs keep fp32 accuracy and 16-bit ones are rounded once.
+// 16-bit queries are exact as they are.
 //
 // Every wait is bounded (2 s); one that gives up sets this kernel's timeout word,
 // and while it is set the kernel computes nothing (qvl_tc_timeout_status).
+#include <algorithm>
+#include <type_traits>
 #include "serving.cuh"
 #include "tc_common.cuh"
 
@@ -44,32 +50,30 @@ namespace qvl {
 __device__ int g_tree_timeout = 0;
 
 namespace {
-constexpr int kTile = 128;              // positions per tile: the MMA's M
-constexpr int kMaxWords = kTreeMaxNodes / 32;
+constexpr int kTile = 128;              // positions per tile
+constexpr int kRows = 128;              // query rows per tile
+constexpr int kSMs = 148;
+constexpr int kThreads = 19 * 32;       // 96 registers each
+constexpr int kSumWarp = 8, kTmaWarp = 16, kMmaWarp = 17;           // the fixer is the last one
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kPBias = 8.0f;          // p is held times 2^8: its low half stays normal
 
 // ---- tensor core helpers ----
+// kind::f16, fp32 sums; B with the contraction index as its slow one if `b_mn`.
 template <typename C>
-__host__ __device__ constexpr uint32_t idesc_16(int n, bool mn_major) {
+__host__ __device__ constexpr uint32_t idesc_16(int n, bool b_mn) {
     const uint32_t t = std::is_same<C, __nv_bfloat16>::value ? 1u : 0u;
-    const uint32_t tr = mn_major ? (3u << 15) : 0u;
-    return (1u << 4) | (t << 7) | (t << 10) | tr | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+    return (1u << 4) | (t << 7) | (t << 10) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) |
+           ((uint32_t)(kRows >> 4) << 24);
 }
 // Operand whose contraction index is the slow one, as TMA wrote it with
 // 128-byte swizzle: rows of 64 values, 8-row atoms of 1024 bytes, `chunk`
-// bytes from one 64-value column block to the next.
+// bytes from one block of 64 values to the next.
 __device__ __forceinline__ uint64_t sdesc_mn_sw128(uint32_t addr, uint32_t chunk) {
     return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)(chunk >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
            (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
-// The same without swizzle: 8 x 8 blocks of 128 contiguous bytes, the next 8
-// contraction indices 128 bytes on, the next 8 rows `chunk` bytes on.
-__device__ __forceinline__ uint64_t sdesc_mn_plain(uint32_t addr, uint32_t chunk) {
-    return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)(128 >> 4) << 16 | (uint64_t)(chunk >> 4) << 32 |
-           (uint64_t)1 << 46;
-}
-__device__ __forceinline__ void mma_16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
@@ -77,6 +81,39 @@ __device__ __forceinline__ void mma_16(uint32_t d, uint64_t a, uint64_t b, uint3
         "l"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
+// A from tensor memory: row = lane, two 16-bit values a column.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+#define QVL_R8(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7])
+#define QVL_V8(r, o) "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7])
+__device__ __forceinline__ void tmem_ld32(uint32_t t, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : QVL_R8(r, 0), QVL_R8(r, 8), QVL_R8(r, 16), QVL_R8(r, 24)
+        : "r"(t));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t t, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::QVL_V8(r, 0), "r"(t) : "memory");
+}
+// Waits for this thread's loads; the values in r are not looked at before.
+#define QVL_RW8(r, o) "+r"(r[o]), "+r"(r[o + 1]), "+r"(r[o + 2]), "+r"(r[o + 3]), "+r"(r[o + 4]), "+r"(r[o + 5]), "+r"(r[o + 6]), "+r"(r[o + 7])
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : QVL_RW8(r, 0), QVL_RW8(r, 8)::"memory");
+}
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : QVL_RW8(r, 0), QVL_RW8(r, 8), QVL_RW8(r, 16), QVL_RW8(r, 24)::"memory");
+}
+#undef QVL_RW8
+#undef QVL_R8
+#undef QVL_V8
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ float redux_max(float v) {
     float r;
     asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
@@ -86,11 +123,14 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
+}
+// A whole warp's wait: false for all lanes where one gave up.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
+    return __all_sync(~0u, tc::mbar_wait(bar, parity, &g_tree_timeout));
 }
 
 // Two floats to packed 16-bit values (a low, b high) and what is left of them.
@@ -110,20 +150,29 @@ template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
 template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
     return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
 }
-// Some half of a packed pair is infinite or NaN.
-template <typename C> __device__ __forceinline__ bool nonfinite2(uint32_t v) {
+// Both halves of a packed pair are finite; the pair with those that are not set to 0.
+template <typename C> __device__ __forceinline__ bool finite2(uint32_t v) {
     constexpr uint32_t e = std::is_same<C, __half>::value ? 0x7c00u : 0x7f80u;
-    return (v & e) == e || ((v >> 16) & e) == e;
+    return (v & e) != e && ((v >> 16) & e) != e;
+}
+template <typename C> __device__ __forceinline__ uint32_t held2(uint32_t v) {
+    constexpr uint32_t e = std::is_same<C, __half>::value ? 0x7c00u : 0x7f80u;
+    return ((v & e) == e ? 0u : v & 0xffffu) | (((v >> 16) & e) == e ? 0u : v & 0xffff0000u);
+}
+// Eight outputs acc / l (`inv` = 1 / l), rounded once.
+template <typename T> __device__ __forceinline__ void store8(T *o, const float *acc, bool none, float inv) {
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = none ? 0.0f : acc[e] * inv;
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4 *>(o) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4 *>(o + 4) = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+        *reinterpret_cast<uint4 *>(o) = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+    }
 }
 
-// ---- what a CTA works on ----
-struct Plan {
-    int chunk;          // tiles per slice
-    int splits;         // slices of the longest context
-    int row_tiles;
-    int box;            // positions per TMA box
-};
-
+// ---- the work ----
 // Rows of q that a request's nodes own: [first, first + n).
 __device__ __forceinline__ int node_count(const TreeArgs &a, int s, int &first) {
     first = min(max(a.starts[s], 0), a.T);
@@ -136,570 +185,820 @@ __device__ __forceinline__ int context(const TreeArgs &a, int s, int n, int &ctx
     ctx = (int)min((long)max(a.ctx_lens[s], 0), cap);
     return (int)min((long)ctx + n, cap);
 }
-__device__ __forceinline__ int slices(int L, const Plan &p) {
-    return max(1, min(p.splits, (L + p.chunk * kTile - 1) / (p.chunk * kTile)));
+struct Request {
+    int first, n, ctx, L, tiles, row_tiles;
+    long units;
+};
+__device__ __forceinline__ Request request_of(const TreeArgs &a, int s) {
+    Request r;
+    r.n = node_count(a, s, r.first);
+    r.L = context(a, s, r.n, r.ctx);
+    r.tiles = (r.L + kTile - 1) / kTile;
+    r.row_tiles = (r.n * (a.NH / a.NKV) + kRows - 1) / kRows;
+    r.units = (long)r.tiles * r.row_tiles * a.NKV;
+    return r;
 }
+// A range of the tiles of one pair.  part: -1 whole pair; otherwise the place in
+// the CTA's half of the workspace.
+struct Segment {
+    int s, kvh, r0, rows, tile0, nt, ctx, L, first, n, part, pad;
+};
+// What the joining launch knows of a partial segment.
+struct Part {
+    int first, kvh, r0, rows;      // rows 0: nothing
+    int starts, ends;              // holds the pair's first / last tile
+};
 
-template <typename T, int D, int NC>
+template <typename T, int D>
 struct Conf {
     static constexpr bool kSplitQ = std::is_same<T, float>::value;
-    static constexpr int kSW = NC > 32 ? 2 : 1;                       // softmax warpgroups
-    static constexpr int kCols = NC / kSW;                            // columns of a softmax thread
-    static constexpr int kThreads = kSW * 128 + 128 + 64;
-    static constexpr int kPerSM = NC > 32 ? 1 : 2;
-    static constexpr int kQ = NC * D * 2;
-    static constexpr int kP = NC * kTile * 2;
+    static constexpr int kQHalves = kSplitQ ? 2 : 1;
     static constexpr int kSlot = kTile * D * 2;
-    static constexpr int kFixed = (kSplitQ ? 2 : 1) * kQ + 2 * kP;
-    static constexpr int kMiscMask = kTreeMaxNodes * (NC > 32 ? NC / 32 : 1) * 4;
-    static constexpr int kMisc = kMiscMask + 4 * NC * 4 + NC * 8 + kSW * 4 * kCols * 4 + 2048;
-    static constexpr int kRoom = (kPerSM == 2 ? 113 : 226) * 1024 - kFixed - kMisc - 1024;
-    static constexpr int kSlots = kRoom / kSlot > 8 ? 8 : kRoom / kSlot;
-    static constexpr int kSmem = 1024 + kSlots * kSlot + kFixed + kMisc;
-    static constexpr int kTmem = 4 * NC < 32 ? 32 : 4 * NC;
-    static_assert(kSlots >= 2, "keys and values take turns in the slots");
+    static constexpr int kMaxRing = 4;
 };
+// Shared memory of a launch: the rest of an SM's after Q goes to the rings.
+struct Layout {
+    int rows;           // of a tile that Q has room for
+    int q_bytes;        // of one half of Q
+    int nk, nv;         // slots for K and for V
+    int words;          // of a node's ancestors
+    int box;            // positions per TMA box
+    int smem;
+};
+// What does not depend on the launch, behind Q.
+struct Fixed {
+    float alpha[4][kRows];          // factors of the sums, by tile
+    float cs[2][kRows];             // score factors, by segment
+    float l[2][2][kRows];           // sums of p, by segment and warpgroup
+    float m[2][kRows];              // maxima, by segment
+    float px[2][2][kRows];          // maxima of a tile's halves, by tile and warpgroup
+    Segment seg[4];
+    uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], p_ready[2], o_full[2], o_empty[2], x_bar[2][8], q_full,
+        q_empty, anc_full[2], seg_full[4], seg_empty[4], l_bar[2], seg_done[2], fix_ask, fix_done;
+    uint32_t valid[8];              // boxes of a tile that exist, by tile
+    uint32_t bad[8][4];             // positions with values held back, by tile
+    uint32_t moved[4][4];           // some maximum moved, by tile and warp
+    long range[3];                  // the stretch's request, offset in it, length
+    long wsum[kThreads / 32];
+    uint32_t tmem;
+    int off;
+};
+// Tensor memory columns: S/P (128 each), O (128 each)
+constexpr uint32_t kTmO = 256, kTmCols = 512;
+
+__host__ __device__ constexpr size_t part_floats(int D) { return (size_t)kRows * D; }
+__host__ __device__ constexpr size_t part_bytes(int D) {
+    return (size_t)kSMs * 2 * (part_floats(D) * sizeof(float) + kRows * sizeof(float2) + sizeof(Part));
+}
+struct Workspace {
+    float *acc;         // [CTA][2][row][D]
+    float2 *ml;         // [CTA][2][row]: maximum, sum
+    Part *part;         // [CTA][2]
+};
+__device__ __forceinline__ Workspace workspace_of(void *p, int D) {
+    Workspace w;
+    w.acc = static_cast<float *>(p);
+    w.ml = reinterpret_cast<float2 *>(w.acc + (size_t)kSMs * 2 * part_floats(D));
+    w.part = reinterpret_cast<Part *>(w.ml + (size_t)kSMs * 2 * kRows);
+    return w;
+}
+
+// One row of Q into shared memory, K-major with 128-byte swizzle, by a warp
+// (lane: E consecutive values); rows past the last one are zero.
+template <typename T, typename C, int D>
+__device__ __forceinline__ void stage_row(float (&x)[D / 32], int r, float qmul, const Layout &ly, unsigned char *q_s,
+                                          float *cs_s, int lane) {
+    using F = Conf<T, D>;
+    constexpr int E = D / 32;
+    float cs = fabsf(qmul);
+    if constexpr (F::kSplitQ) {
+        float mx = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            x[e] *= qmul;
+            mx = fmaxf(mx, fabsf(x[e]));
+        }
+        mx = redux_max(mx);
+        // largest value into [2^9, 2^10)
+        int ex = (int)(__float_as_uint(mx) >> 23);
+        if (mx == 0.0f || ex == 255) ex = 127 + 9;
+        ex = max(ex, 10);
+        const float f = __uint_as_float((uint32_t)min(254, 263 - ex) << 23);
+        cs = __uint_as_float((uint32_t)(ex - 9) << 23);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] *= f;
+    } else if (qmul < 0.0f) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = -x[e];
+    }
+    const int half = (lane * E) >> 6, in = (lane * E) & 63;
+    unsigned char *dst = q_s + half * (ly.rows * 128) + r * 128 + ((((in * 2) >> 4) ^ (r & 7)) << 4) + ((in * 2) & 15);
+    uint32_t hi[E / 2], lo[E / 2];
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+        hi[e / 2] = pack2<C>(x[e], x[e + 1]);
+        if constexpr (F::kSplitQ) {
+            const float2 h = unpack2<C>(hi[e / 2]);
+            lo[e / 2] = pack2<C>(x[e] - h.x, x[e + 1] - h.y);
+        }
+    }
+    if constexpr (E == 4) {
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(hi[0], hi[1]);
+        if constexpr (F::kSplitQ) *reinterpret_cast<uint2 *>(dst + ly.q_bytes) = make_uint2(lo[0], lo[1]);
+    } else {
+        *reinterpret_cast<uint32_t *>(dst) = hi[0];
+        if constexpr (F::kSplitQ) *reinterpret_cast<uint32_t *>(dst + ly.q_bytes) = lo[0];
+    }
+    if (lane == 0) cs_s[r] = cs;
+}
+template <typename T, int E>
+__device__ __forceinline__ void load_e(const T *p, float (&x)[E]) {
+    if constexpr (sizeof(T) * E == 16) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(p);
+        const T *t = reinterpret_cast<const T *>(&v);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = to_f32(t[e]);
+    } else if constexpr (sizeof(T) * E == 8) {
+        const uint2 v = *reinterpret_cast<const uint2 *>(p);
+        const T *t = reinterpret_cast<const T *>(&v);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = to_f32(t[e]);
+    } else {
+        const uint32_t v = *reinterpret_cast<const uint32_t *>(p);
+        const T *t = reinterpret_cast<const T *>(&v);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = to_f32(t[e]);
+    }
+}
+// The segment's query rows, warp w of nw; several rows' loads in flight.
+template <typename T, typename C, int D>
+__device__ __forceinline__ void stage_queries(const TreeArgs &a, const Layout &ly, const Segment &g, unsigned char *q_s,
+                                              float *cs_s, int w, int nw, int lane) {
+    constexpr int E = D / 32, U = 4;
+    const int G = a.NH / a.NKV;
+    const float qmul = a.scale * kLog2e;
+    const int nr = (g.rows + 7) & ~7;           // rows past these are never looked at
+    for (int r = w; r < nr; r += nw * U) {
+        float x[U][E];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int rr = r + u * nw;
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[u][e] = 0.0f;
+            if (rr < g.rows) {
+                const int node = (g.r0 + rr) / G, h = (g.r0 + rr) - node * G;
+                load_e<T, E>(reinterpret_cast<const T *>(a.q) + (long)(g.first + node) * a.q_stride +
+                                 (long)(g.kvh * G + h) * D + lane * E, x[u]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (r + u * nw < nr) stage_row<T, C, D>(x[u], r + u * nw, qmul, ly, q_s, cs_s, lane);
+    }
+}
+// Ancestors of every node as bits, its own among them: a node's are its parent's and itself.  One warp.
+__device__ __forceinline__ void stage_ancestors(const TreeArgs &a, const Segment &g, uint32_t *anc, int words, int lane) {
+    for (int i0 = 0; i0 < g.n; i0 += 32) {
+        const int mine = i0 + lane < g.n ? a.parents[g.first + i0 + lane] : -1;
+        for (int i = i0; i < min(i0 + 32, g.n); ++i) {
+            const int p = __shfl_sync(~0u, mine, i - i0);
+            if (lane < words) {
+                uint32_t v = p >= 0 && p < i ? anc[p * words + lane] : 0u;
+                if (lane == (i >> 5)) v |= 1u << (i & 31);
+                anc[i * words + lane] = v;
+            }
+            __syncwarp();
+        }
+    }
+}
+// What a row sees of positions t0 .. t0 + 31, of its ancestors' bits.
+__device__ __forceinline__ uint32_t seen_word(const uint32_t *anc, int words, int t0, int ctx, int L) {
+    if (t0 >= L) return 0u;
+    uint32_t m;
+    const int off = t0 - ctx;                   // the node at t0
+    if (off <= -32) {
+        m = ~0u;
+    } else if (off < 0) {
+        m = ((1u << -off) - 1u) | (anc[0] << -off);
+    } else {
+        const int w = off >> 5, b = off & 31;
+        const uint32_t lo = w < words ? anc[w] : 0u, hi = w + 1 < words ? anc[w + 1] : 0u;
+        m = __funnelshift_r(lo, hi, b);
+    }
+    return L - t0 < 32 ? m & ((1u << (L - t0)) - 1u) : m;
+}
+// A place in a ring of n slots: the slot, and the parity of its turn.
+struct Turn {
+    int slot = 0;
+    uint32_t parity = 0;
+    __device__ __forceinline__ void step(int n) {
+        if (++slot == n) {
+            slot = 0;
+            parity ^= 1;
+        }
+    }
+};
+// TMA load whose lines leave L2 first: the cache is read once, and would push
+// everything else out.
+__device__ __forceinline__ void tma_load_once(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar, uint64_t pol) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3}], "
+        "[%4], %5;" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar), "l"(pol)
+        : "memory");
+}
 }  // namespace
 
-// grid (splits * row_tiles, NKV, S)
-template <typename T, typename C, int D, int NC>
-__global__ void __launch_bounds__(Conf<T, D, NC>::kThreads, Conf<T, D, NC>::kPerSM)
+template <typename T, typename C, int D>
+__global__ void __launch_bounds__(kThreads, 1)
 tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-               const __grid_constant__ TreeArgs a, const __grid_constant__ Plan pl) {
-    using F = Conf<T, D, NC>;
-    constexpr int kSW = F::kSW, kCols = F::kCols, NS = F::kSlots;
-    constexpr int kWordsC = NC > 32 ? NC / 32 : 1;
-    extern __shared__ __align__(1024) unsigned char smem_raw[];
-    unsigned char *smem =
-        reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    unsigned char *slots = smem;
-    unsigned char *q_s = slots + NS * F::kSlot;                        // hi, then lo
-    unsigned char *p_s = q_s + (F::kSplitQ ? 2 : 1) * F::kQ;           // hi, then lo
-    uint32_t *tmask = reinterpret_cast<uint32_t *>(p_s + 2 * F::kP);   // [node][kWordsC]: columns that see it
-    float *alpha_s = reinterpret_cast<float *>(tmask + kTreeMaxNodes * kWordsC);      // [4][NC]
-    float2 *cm_s = reinterpret_cast<float2 *>(alpha_s + 4 * NC);       // [NC]: {score factor, maximum}
-    float *wmax_s = reinterpret_cast<float *>(cm_s + NC);              // [kSW][4][kCols]
-    uint32_t *bad_s = reinterpret_cast<uint32_t *>(wmax_s + kSW * 4 * kCols);         // [4][4]: rows of V held back
-    uint64_t *bars = reinterpret_cast<uint64_t *>(bad_s + 16);
-    const uint32_t kv_full = tc::smem_u32(bars), kv_empty = kv_full + 8 * 8, s_full = kv_empty + 8 * 8,
-                   s_empty = s_full + 16, o_full = s_empty + 16, o_empty = o_full + 16, p_ready = o_empty + 16,
-                   p_empty = p_ready + 8;
-    uint32_t *valid_s = reinterpret_cast<uint32_t *>(bars + 26);       // [8], by tile: its boxes that exist
-    uint32_t *tmem_slot = valid_s + 8;
-    int *off_s = reinterpret_cast<int *>(tmem_slot + 1);
+               const __grid_constant__ TreeArgs a, const __grid_constant__ Layout ly) {
+    using F = Conf<T, D>;
+    // (addresses in it are constants, which keeps them out of the registers)
+    extern __shared__ __align__(1024) unsigned char smem[];
+    Fixed &fx = *reinterpret_cast<Fixed *>(smem);
+    constexpr int kHead = ((int)sizeof(Fixed) + 1023) & ~1023;
+    unsigned char *q_s = smem + kHead;                              // hi, then lo
+    unsigned char *k_s = q_s + F::kQHalves * ly.q_bytes;            // slots of K, of V
+    unsigned char *v_s = k_s + ly.nk * F::kSlot;
+    uint32_t *anc_s = reinterpret_cast<uint32_t *>(v_s + ly.nv * F::kSlot);     // [2][node][words], by segment
+    auto bar = [](uint64_t &b) { return tc::smem_u32(&b); };
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int s = blockIdx.z, kvh = blockIdx.y;
-    const int z = blockIdx.x % pl.splits, rt = blockIdx.x / pl.splits;
     const int G = a.NH / a.NKV;
 
-    pdl_wait();
-    int first, ctx;
-    const int n = node_count(a, s, first);
-    const int L = context(a, s, n, ctx);
-    const int r0 = rt * NC;
-    T *out = reinterpret_cast<T *>(a.out);
-    const int nsl = slices(L, pl);
-
-    // rows that no node owns
-    if (z == 0 && rt == 0) {
-        auto clear = [&](int from, int to) {
-            for (long e = (long)from * G * D + tid; e < (long)to * G * D; e += F::kThreads) {
-                const long row = e / (G * D), c = e - row * (G * D);
-                out[(row * a.NH + (long)kvh * G) * D + c] = from_f32<T>(0.0f);
-            }
-        };
-        if (s == 0) clear(0, min(max(a.starts[0], 0), a.T));
-        // past max_nodes, and behind the last request
-        clear(first + n, s + 1 < a.S ? min(max(a.starts[s + 1], first), a.T) : a.T);
-    }
-    if (n == 0 || r0 >= n * G || z >= nsl) return;
-    const int rows = min(NC, n * G - r0);
-    const int tile0 = z * pl.chunk;
-    const int tiles = (L + kTile - 1) / kTile;
-    const int nt = (z == nsl - 1 ? tiles : min(tiles, tile0 + pl.chunk)) - tile0;
-    const bool has_tree = (long)(tile0 + nt) * kTile > ctx;
-
     if (tid == 0) {
-        off_s[0] = *reinterpret_cast<volatile int *>(&g_tree_timeout);
-        for (int i = 0; i < NS; ++i) {
-            tc::mbar_init(kv_full + 8 * i, 1);
-            tc::mbar_init(kv_empty + 8 * i, 1);
+        for (int i = 0; i < 4; ++i) {
+            tc::mbar_init(bar(fx.k_full[i]), 1);
+            tc::mbar_init(bar(fx.k_empty[i]), 1);
+            tc::mbar_init(bar(fx.v_full[i]), 1);
+            tc::mbar_init(bar(fx.v_empty[i]), 1);
+            tc::mbar_init(bar(fx.seg_full[i]), 1);
+            tc::mbar_init(bar(fx.seg_empty[i]), 18);
         }
         for (int i = 0; i < 2; ++i) {
-            tc::mbar_init(s_full + 8 * i, 1);
-            tc::mbar_init(s_empty + 8 * i, kSW * 128);
-            tc::mbar_init(o_full + 8 * i, 1);
-            tc::mbar_init(o_empty + 8 * i, 128);
+            tc::mbar_init(bar(fx.s_full[i]), 1);
+            tc::mbar_init(bar(fx.p_ready[i]), 256);
+            tc::mbar_init(bar(fx.o_full[i]), 1);
+            tc::mbar_init(bar(fx.o_empty[i]), 256);
+            tc::mbar_init(bar(fx.anc_full[i]), 1);
+            tc::mbar_init(bar(fx.l_bar[i]), 256);
+            tc::mbar_init(bar(fx.seg_done[i]), 16);
+            for (int w = 0; w < 8; ++w) tc::mbar_init(bar(fx.x_bar[i][w]), 1);
         }
-        tc::mbar_init(p_ready, kSW * 128);
-        tc::mbar_init(p_empty, 1);
+        tc::mbar_init(bar(fx.q_full), 256);
+        tc::mbar_init(bar(fx.q_empty), 1);
+        tc::mbar_init(bar(fx.fix_ask), 1);
+        tc::mbar_init(bar(fx.fix_done), 32);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         tc::prefetch_tmap(&tm_k);
         tc::prefetch_tmap(&tm_v);
     }
-    constexpr int kMmaWarp = kSW * 4 + 4, kTmaWarp = kMmaWarp + 1;
     if (warp == kMmaWarp) {
-        tc::tmem_alloc(tc::smem_u32(tmem_slot), F::kTmem);
+        tc::tmem_alloc(tc::smem_u32(&fx.tmem), kTmCols);
         tc::tmem_relinquish();
     }
+    pdl_wait();
+    if (tid == 0) fx.off = *reinterpret_cast<volatile int *>(&g_tree_timeout);
 
-    // query rows into shared memory, K-major with 128-byte swizzle: one warp a
-    // row; rows past the last one are zero
-    const float qmul = a.scale * kLog2e;
-    for (int r = warp; r < NC; r += F::kThreads / 32) {
-        constexpr int E = D / 32;           // values of a lane
-        float x[E];
-        const int node = (r0 + r) / G, hq = (r0 + r) - node * G;
-        const T *src = reinterpret_cast<const T *>(a.q) + (long)(first + node) * a.q_stride + (long)(kvh * G + hq) * D + lane * E;
+    // this CTA's stretch of the units
+    {
+        const int per = (a.S + kThreads - 1) / kThreads;
+        const int s0 = min(tid * per, a.S), s1 = min(s0 + per, a.S);
+        long mine = 0;
+        for (int s = s0; s < s1; ++s) mine += request_of(a, s).units;
+        long inc = mine;
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = r < rows ? to_f32(src[e]) : 0.0f;
-        float cs = fabsf(qmul);
-        if constexpr (F::kSplitQ) {
-            float mx = 0.0f;
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                x[e] *= qmul;
-                mx = fmaxf(mx, fabsf(x[e]));
-            }
-            mx = redux_max(mx);
-            // largest value into [2^9, 2^10)
-            int ex = (int)(__float_as_uint(mx) >> 23);
-            if (mx == 0.0f || ex == 255) ex = 127 + 9;
-            ex = max(ex, 10);
-            const float f = __uint_as_float((uint32_t)min(254, 263 - ex) << 23);
-            cs = __uint_as_float((uint32_t)(ex - 9) << 23);
-#pragma unroll
-            for (int e = 0; e < E; ++e) x[e] *= f;
-        } else if (qmul < 0.0f) {
-#pragma unroll
-            for (int e = 0; e < E; ++e) x[e] = -x[e];
+        for (int o = 1; o < 32; o <<= 1) {
+            const long up = __shfl_up_sync(~0u, inc, o);
+            if (lane >= o) inc += up;
         }
-        const int half = lane * E >> 6, in = lane * E & 63;
-        unsigned char *dst = q_s + half * (NC * 128) + r * 128 + ((((in * 2) >> 4) ^ (r & 7)) << 4) + ((in * 2) & 15);
-#pragma unroll
-        for (int e = 0; e < E; e += 2) {
-            const uint32_t hi = pack2<C>(x[e], x[e + 1]);
-            *reinterpret_cast<uint32_t *>(dst + e * 2) = hi;
-            if constexpr (F::kSplitQ) {
-                const float2 h = unpack2<C>(hi);
-                *reinterpret_cast<uint32_t *>(dst + F::kQ + e * 2) = pack2<C>(x[e] - h.x, x[e + 1] - h.y);
-            }
-        }
-        if (lane == 0) cm_s[r] = make_float2(cs, -INFINITY);
-    }
-    if (tid < 16) bad_s[tid] = 0;
-
-    // columns that see each drafted position: ancestors by doubling (a node's
-    // set is its own bit, its parent's set, ...), turned to bits over columns
-    if (has_tree) {
-        uint32_t *anc = reinterpret_cast<uint32_t *>(slots);           // [2][256][words]; before the first load
-        int *up = reinterpret_cast<int *>(slots + 2 * kTreeMaxNodes * kMaxWords * 4);
-        const int words = (n + 31) / 32;
-        for (int i = tid; i < n; i += F::kThreads) {
-            const int p = a.parents[first + i];
-            up[i] = p >= 0 && p < i ? p : -1;
-            for (int w = 0; w < words; ++w) anc[i * kMaxWords + w] = w == (i >> 5) ? 1u << (i & 31) : 0u;
-        }
+        if (lane == 31) fx.wsum[warp] = inc;
+        if (tid == 0) fx.range[2] = 0;
         __syncthreads();
-        int cur = 0;
-        for (int d = 1; d < n; d *= 2) {
-            const uint32_t *src = anc + cur * kTreeMaxNodes * kMaxWords;
-            uint32_t *dst = anc + (cur ^ 1) * kTreeMaxNodes * kMaxWords;
-            const int *us = up + cur * kTreeMaxNodes;
-            int *ud = up + (cur ^ 1) * kTreeMaxNodes;
-            for (int i = tid; i < n; i += F::kThreads) {
-                const int p = us[i];
-                for (int w = 0; w < words; ++w)
-                    dst[i * kMaxWords + w] = src[i * kMaxWords + w] | (p >= 0 ? src[p * kMaxWords + w] : 0u);
-                ud[i] = p >= 0 ? us[p] : -1;
-            }
-            cur ^= 1;
-            __syncthreads();
+        long before = inc - mine, total = 0;
+#pragma unroll 1
+        for (int w = 0; w < kThreads / 32; ++w) {
+            const long v = fx.wsum[w];
+            if (w < warp) before += v;
+            total += v;
         }
-        const uint32_t *res = anc + cur * kTreeMaxNodes * kMaxWords;
-        for (int e = tid; e < n * kWordsC; e += F::kThreads) {
-            const int j = e / kWordsC, w = e - j * kWordsC;
-            uint32_t m = 0;
-            for (int c = 0; c < 32 && w * 32 + c < rows; ++c) {
-                const int node = (r0 + w * 32 + c) / G;
-                m |= ((res[node * kMaxWords + (j >> 5)] >> (j & 31)) & 1u) << c;
+        // (fewer units than CTAs: the last CTAs have none, so that a pair's parts
+        // are in consecutive CTAs)
+        const long ctas = min((long)gridDim.x, max(total, 1l)), me = min((long)blockIdx.x, ctas);
+        const long lo = total * me / ctas, hi = total * min(me + 1, ctas) / ctas;
+        if (lo < hi && before <= lo && lo < before + mine) {
+            int s = s0;
+            long u = request_of(a, s).units;
+            while (before + u <= lo) {
+                before += u;
+                u = request_of(a, ++s).units;
             }
-            tmask[e] = m;
+            fx.range[0] = s;
+            fx.range[1] = lo - before;
+            fx.range[2] = hi - lo;
         }
-        fence_async_smem();         // the loads overwrite what the generic proxy read and wrote here
     }
-    fence_async_smem();
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
     pdl_launch_dependents();
-    const uint32_t tmem = *tmem_slot;
-    const uint32_t tm_s = tmem, tm_o = tmem + 2 * NC;
-    bool ok = off_s[0] == 0;
-    int issued = 0;                      // slots that the TMA warp filled
+    const uint32_t tmem = fx.tmem;
+    bool ok = fx.off == 0 && (tc::smem_u32(smem) & 1023) == 0;
+    const Workspace ws = workspace_of(a.workspace, D);
+    int seg = 0, i = 0;                 // segments and tiles so far, in step in all roles
+    auto next = [&](const Segment *&g) {        // the segment, or false at the end
+        if (!(ok = warp_wait(bar(fx.seg_full[seg & 3]), (seg >> 2) & 1))) return false;
+        g = &fx.seg[seg & 3];
+        return g->nt > 0;
+    };
+    auto done = [&] {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(fx.seg_empty[seg & 3]));
+        ++seg;
+    };
+
+    if (warp < kTmaWarp) {
+        // the first segment's queries: the warps that have nothing to do yet
+        if (ok) ok = warp_wait(bar(fx.seg_full[0]), 0);
+        if (ok && fx.seg[0].nt > 0) {
+            stage_queries<T, C, D>(a, ly, fx.seg[0], q_s, fx.cs[0], warp, kTmaWarp, lane);
+            fence_async_smem();
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(kTmaWarp * 32) : "memory");
+    }
 
     if (warp == kTmaWarp) {
-        // lane l: box l / 2 of the tile's 64-value half l % 2
-        const int nb = kTile / pl.box, lanes = nb * (D / 64);
-        const int b = lane / (D / 64), half = lane % (D / 64);
+        // ---- segments, pages and loads ----
+        int s = (int)fx.range[0];
+        long off = fx.range[1], left = ok ? fx.range[2] : 0;
+        Request rq{};
+        if (left > 0) rq = request_of(a, s);
+        if (lane < 2) ws.part[blockIdx.x * 2 + lane].rows = 0;
+        __syncwarp();
+        // lane l: box l / (D / 64) of the tile's 64-value half l % (D / 64)
+        const int lanes = kTile / ly.box * (D / 64);
+        const int bx = lane / (D / 64), half = lane % (D / 64);
         const int oob = (int)(a.num_pages * a.NKV * a.P);          // past the last row: zeros
-        for (int i = 0; ok && i < nt; ++i) {
-            const int t = (tile0 + i) * kTile + b * pl.box;
-            int y = oob;
-            if (lane < lanes && t < L) {
-                const int c = t / a.P;
-                const int pg = a.table[(size_t)s * a.maxp + c];
-                if (pg >= 0 && pg < a.num_pages) y = (int)(((long)pg * a.NKV + kvh) * a.P + (t - c * a.P));
+        const int to = half * (kTile * 128) + bx * ly.box * 128;
+        Turn kt, vt;
+        int loads = 0;                                             // K slots filled; V slots are one behind at most
+        uint64_t once;
+        asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(once));
+        while (ok) {
+            Segment g{};
+            if (left > 0) {
+                while (off >= rq.units) {
+                    off -= rq.units;
+                    rq = request_of(a, ++s);
+                }
+                const int pair = (int)(off / rq.tiles);            // key head, then tile of rows
+                g.s = s;
+                g.kvh = pair / rq.row_tiles;
+                g.r0 = (pair - g.kvh * rq.row_tiles) * kRows;
+                g.rows = min(kRows, rq.n * G - g.r0);
+                g.tile0 = (int)(off - (long)pair * rq.tiles);
+                g.nt = (int)min(left, (long)(rq.tiles - g.tile0));
+                g.ctx = rq.ctx;
+                g.L = rq.L;
+                g.first = rq.first;
+                g.n = rq.n;
+                const bool starts = g.tile0 == 0, ends = g.tile0 + g.nt == rq.tiles;
+                g.part = starts && ends ? -1 : starts ? 1 : 0;
+                if (g.part >= 0 && lane == 0)
+                    ws.part[blockIdx.x * 2 + g.part] = {g.first, g.kvh, g.r0, g.rows, starts, ends};
+                off += g.nt;
+                left -= g.nt;
             }
-            const uint32_t there = __ballot_sync(~0u, y != oob);
-            for (int h = 0; h < 2 && ok; ++h) {
-                const int u = 2 * i + h, sl = u % NS, k = u / NS;
-                if (k > 0) ok = tc::mbar_wait(kv_empty + 8 * sl, (k - 1) & 1, &g_tree_timeout);
-                ok = __all_sync(~0u, ok);
-                if (!ok) break;
+            if (seg >= 4) ok = warp_wait(bar(fx.seg_empty[seg & 3]), ((seg >> 2) - 1) & 1);
+            if (!ok) break;
+            if (lane == 0) {
+                fx.seg[seg & 3] = g;
+                mbar_arrive(bar(fx.seg_full[seg & 3]));
+            }
+            ++seg;
+            if (g.nt == 0) break;
+            for (int k = 0; k < g.nt; ++k, ++i) {
+                const int t = (g.tile0 + k) * kTile + bx * ly.box;
+                int y = oob;
+                if (lane < lanes && t < g.L) {
+                    const int c = t / a.P;
+                    const int pg = a.table[(size_t)g.s * a.maxp + c];
+                    if (pg >= 0 && pg < a.num_pages) y = (int)(((long)pg * a.NKV + g.kvh) * a.P + (t - c * a.P));
+                }
+                const uint32_t there = __ballot_sync(~0u, y != oob);
+                if (i >= ly.nk && !(ok = warp_wait(bar(fx.k_empty[kt.slot]), kt.parity ^ 1))) break;
                 if (lane == 0) {
-                    // (the load of a tile's keys runs at most kSlots / 2 + 1 tiles
-                    // ahead of the softmax that reads this)
-                    if (h == 0) valid_s[i & 7] = there;
-                    tc::mbar_expect_tx(kv_full + 8 * sl, F::kSlot);
+                    // (keys are loaded at most nk + 2 tiles ahead of the softmax
+                    // that reads this)
+                    fx.valid[i & 7] = there;
+                    tc::mbar_expect_tx(bar(fx.k_full[kt.slot]), F::kSlot);
                 }
                 __syncwarp();
                 if (lane < lanes)
-                    tc::tma_load_2d(tc::smem_u32(slots + sl * F::kSlot + half * (kTile * 128) + b * pl.box * 128),
-                                    h ? &tm_v : &tm_k, half * 64, y, kv_full + 8 * sl);
+                    tma_load_once(tc::smem_u32(k_s + kt.slot * F::kSlot + to), &tm_k, half * 64, y, bar(fx.k_full[kt.slot]), once);
+                kt.step(ly.nk);
+                ++loads;
+                if (i >= ly.nv && !(ok = warp_wait(bar(fx.v_empty[vt.slot]), vt.parity ^ 1))) break;
+                if (lane == 0) tc::mbar_expect_tx(bar(fx.v_full[vt.slot]), F::kSlot);
                 __syncwarp();
-                issued = u + 1;
+                if (lane < lanes)
+                    tma_load_once(tc::smem_u32(v_s + vt.slot * F::kSlot + to), &tm_v, half * 64, y, bar(fx.v_full[vt.slot]), once);
+                vt.step(ly.nv);
             }
         }
-        // loads in flight land before the CTA ends
-        if (!ok)
-            for (int u = max(0, issued - NS); u < issued; ++u)
-                tc::mbar_wait(kv_full + 8 * (u % NS), (u / NS) & 1, nullptr);
+        // after a wait that gave up: loads in flight land before the CTA ends
+        // (each slot's last load; a slot never filled has nothing in flight)
+        if (!ok) {
+            for (int n = 0; n < min(loads, ly.nk); ++n) tc::mbar_wait(bar(fx.k_full[n]), (((loads - 1 - n) / ly.nk) & 1), nullptr);
+            for (int n = 0; n < min(i, ly.nv); ++n) tc::mbar_wait(bar(fx.v_full[n]), (((i - 1 - n) / ly.nv) & 1), nullptr);
+        }
     } else if (warp == kMmaWarp) {
+        // ---- products: the scores of the tile after next behind each O.  One thread,
+        // which an issue holds until the tensor cores take it: what stands between
+        // two products is kept short ----
         if (lane == 0) {
-            constexpr uint32_t id_s = idesc_16<C>(NC, false), id_o = idesc_16<C>(NC, true);
-            const uint32_t qa = tc::smem_u32(q_s), pa = tc::smem_u32(p_s), sa = tc::smem_u32(slots);
-            auto scores = [&](int i) {
-                const int u = 2 * i, sl = u % NS, b = i & 1;
-                ok = ok && tc::mbar_wait(kv_full + 8 * sl, (u / NS) & 1, &g_tree_timeout);
-                if (i >= 2) ok = ok && tc::mbar_wait(s_empty + 8 * b, ((i >> 1) - 1) & 1, &g_tree_timeout);
-                if (!ok) return;
+            constexpr uint32_t id_s = idesc_16<C>(kTile, false), id_o = idesc_16<C>(D, true);
+            // descriptors: the address is their low end, in units of 16 bytes
+            const uint64_t qd = tc::sdesc_k_sw128(tc::smem_u32(q_s)), kd = tc::sdesc_k_sw128(tc::smem_u32(k_s));
+            const uint64_t vd = sdesc_mn_sw128(tc::smem_u32(v_s), kTile * 128);
+            const uint32_t q_lo = ly.q_bytes >> 4, q_half = (ly.rows * 128) >> 4;
+            int qseg = 0, qk = 0, qnt = 0, qi = 0;        // scores: segment, tile in it, its tiles, tile in all
+            bool more = ok;
+            Turn kt, vt;
+            auto wait = [&](uint64_t &b, uint32_t parity) { return ok = tc::mbar_wait(bar(b), parity, &g_tree_timeout); };
+            // low halves first: what they add up to is small, and exact beside the
+            // roundings of the high halves' sums
+            auto scores = [&] {
+                if (!more) return;
+                if (qk == 0) {
+                    if (!wait(fx.seg_full[qseg & 3], (qseg >> 2) & 1)) return;
+                    qnt = *reinterpret_cast<volatile int *>(&fx.seg[qseg & 3].nt);
+                    if (qnt == 0) {
+                        more = false;
+                        return;
+                    }
+                    if (!wait(fx.q_full, qseg & 1)) return;
+                }
+                if (!wait(fx.k_full[kt.slot], kt.parity)) return;
                 tc::tc_fence_after();
-                const uint32_t ka = sa + sl * F::kSlot;
+                const uint64_t kb = kd + (uint32_t)(kt.slot * (F::kSlot >> 4));
+                const uint32_t d = tmem + (qi & 1) * kTile;
 #pragma unroll
-                for (int l = 0; l < (F::kSplitQ ? 2 : 1); ++l)
+                for (int l = F::kQHalves - 1; l >= 0; --l)
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k)
-                        mma_16(tm_s + b * NC, tc::sdesc_k_sw128(ka + (k >> 2) * (kTile * 128) + (k & 3) * 32),
-                               tc::sdesc_k_sw128(qa + l * F::kQ + (k >> 2) * (NC * 128) + (k & 3) * 32), id_s,
-                               (l | k) ? 1u : 0u);
-                tc::tc_commit(kv_empty + 8 * sl);
-                tc::tc_commit(s_full + 8 * b);
+                        mma_ss(d, qd + (l * q_lo + (k >> 2) * q_half + (k & 3) * 2), kb + ((k >> 2) * (kTile * 8) + (k & 3) * 2),
+                               id_s, l < F::kQHalves - 1 || k ? 1u : 0u);
+                tc::tc_commit(bar(fx.s_full[qi & 1]));
+                tc::tc_commit(bar(fx.k_empty[kt.slot]));
+                kt.step(ly.nk);
+                ++qi;
+                if (++qk == qnt) {
+                    tc::tc_commit(bar(fx.q_empty));
+                    qk = 0;
+                    ++qseg;
+                }
             };
-            scores(0);
-            for (int i = 0; ok && i < nt; ++i) {
-                if (i + 1 < nt) scores(i + 1);
-                const int u = 2 * i + 1, sl = u % NS, b = i & 1;
-                ok = ok && tc::mbar_wait(kv_full + 8 * sl, (u / NS) & 1, &g_tree_timeout);
-                ok = ok && tc::mbar_wait(p_ready, i & 1, &g_tree_timeout);
-                if (i >= 2) ok = ok && tc::mbar_wait(o_empty + 8 * b, ((i >> 1) - 1) & 1, &g_tree_timeout);
+            scores();
+            if (ok) scores();
+            int fixes = 0;
+            while (ok && wait(fx.seg_full[seg & 3], (seg >> 2) & 1)) {
+                const volatile Segment &sg = fx.seg[seg & 3];
+                const int nt = sg.nt, plain = max(0, sg.ctx / kTile - sg.tile0);      // tiles before the drafted ones
+                if (nt == 0) break;
+                for (int k = 0; k < nt; ++k, ++i) {
+                    const int b = i & 1;
+                    const bool tail = k >= plain;
+                    if (tail) {
+                        if (!wait(fx.v_full[vt.slot], vt.parity)) break;
+                        mbar_arrive(bar(fx.fix_ask));
+                    }
+                    if (i >= 2 && !wait(fx.o_empty[b], ((i >> 1) - 1) & 1)) break;
+                    if (!wait(fx.v_full[vt.slot], vt.parity)) break;
+                    if (tail && !wait(fx.fix_done, fixes++ & 1)) break;
+                    if (!wait(fx.p_ready[b], (i >> 1) & 1)) break;
+                    tc::tc_fence_after();
+                    const uint64_t vb = vd + (uint32_t)(vt.slot * (F::kSlot >> 4));
+                    const uint32_t pb = tmem + b * kTile, d = tmem + kTmO + b * 128;
+#pragma unroll
+                    for (int l = 1; l >= 0; --l)
+#pragma unroll
+                        for (int c = 0; c < kTile / 16; ++c)
+                            mma_ts(d, pb + (c >> 2) * 64 + l * 32 + (c & 3) * 8, vb + c * (2048 >> 4), id_o, l == 0 || c ? 1u : 0u);
+                    tc::tc_commit(bar(fx.o_full[b]));
+                    tc::tc_commit(bar(fx.v_empty[vt.slot]));
+                    vt.step(ly.nv);
+                    scores();
+                    if (!ok) break;
+                }
                 if (!ok) break;
-                tc::tc_fence_after();
-                const uint32_t va = sa + sl * F::kSlot;
-                // D 64: the second 64 rows of the product are not read; any
-                // part of shared memory will do for them
-                constexpr uint32_t kChunk = D == 128 ? kTile * 128 : 1024;
-#pragma unroll
-                for (int l = 0; l < 2; ++l)
-#pragma unroll
-                    for (int k = 0; k < kTile / 16; ++k)
-                        mma_16(tm_o + b * NC, sdesc_mn_sw128(va + k * 2048, kChunk),
-                               sdesc_mn_plain(pa + l * F::kP + k * 256, kTile * 16), id_o, (l | k) ? 1u : 0u);
-                tc::tc_commit(kv_empty + 8 * sl);
-                tc::tc_commit(p_empty);
-                tc::tc_commit(o_full + 8 * b);
+                mbar_arrive(bar(fx.seg_empty[seg & 3]));
+                ++seg;
             }
         }
-        __syncwarp();
-    } else if (warp < kSW * 4) {
-        // ---- softmax: thread = position, columns [c0, c0 + kCols) ----
-        const int wg = warp >> 2, w4 = warp & 3, c0 = wg * kCols;
-        const int jl = w4 * 32 + lane;
-        const uint32_t lane_off = (uint32_t)(w4 * 32) << 16;
-        float *wmax = wmax_s + wg * 4 * kCols;
-        const int own = tid & 127;                    // the column this thread keeps the maximum of
-        float m_own = -INFINITY;
-        const float cs_own = own < kCols ? cm_s[c0 + own].x : 0.0f;
-        float l[kCols];
+    } else if (warp < kSumWarp) {
+        // ---- softmax: thread = row, positions 64 wg .. 64 wg + 63 of each tile ----
+        const int wg = warp >> 2, w4 = warp & 3, row = tid & 127;
+        const uint32_t ts = tmem + ((uint32_t)(w4 * 32) << 16) + wg * 64;
+        const Segment *g;
+        while (ok && next(g)) {
+            // (what is seldom needed is read from shared memory where it is)
+            const volatile Segment &sg = fx.seg[seg & 3];
+            const int nt = sg.nt;
+            const bool active = w4 * 32 < sg.rows;
+            float m = -INFINITY, l = 0.0f;
+            for (int k = 0; k < nt; ++k, ++i) {
+                const int b = i & 1;
+                if (!(ok = warp_wait(bar(fx.s_full[b]), (i >> 1) & 1))) break;
+                tc::tc_fence_after();
+                const int t0 = (sg.tile0 + k) * kTile + wg * 64, ctx = sg.ctx;
+                const uint32_t there = *reinterpret_cast<volatile uint32_t *>(&fx.valid[i & 7]);
+                const bool plain = t0 + 64 <= ctx && there == (1u << (kTile / ly.box * (D / 64))) - 1u;
+                if (t0 + 64 > ctx && !(ok = warp_wait(bar(fx.anc_full[seg & 1]), (seg >> 1) & 1))) break;
+                uint32_t r[2][32];
+                float top = -INFINITY;
+                if (active) {
+                    tmem_ld32(ts + b * kTile, r[0]);
+                    tmem_ld32(ts + b * kTile + 32, r[1]);
+                    uint32_t see[2];
+                    if (!plain) {
+                        const uint32_t *anc = anc_s + ((seg & 1) * a.max_nodes + min((sg.r0 + row) / G, sg.n - 1)) * ly.words;
 #pragma unroll
-        for (int c = 0; c < kCols; ++c) l[c] = 0.0f;
-
-        // (after a wait that gave up, the loops run on without waiting: the
-        // barriers among a warpgroup's threads have to be met by all of them)
-        for (int i = 0; i < nt; ++i) {
-            const int b = i & 1;
-            const int t0 = (tile0 + i) * kTile, t = t0 + jl;
-            if (ok) ok = tc::mbar_wait(s_full + 8 * b, (i >> 1) & 1, &g_tree_timeout);
-            // what this position's columns see: all, or the bits of `see`
-            const int vu = 2 * i + 1;
-            const uint32_t there = *reinterpret_cast<volatile uint32_t *>(&valid_s[i & 7]);
-            const bool plain = t0 + kTile <= ctx && there == (1u << (kTile / pl.box * (D / 64))) - 1u;
-            uint32_t see[kWordsC];
-#pragma unroll
-            for (int w = 0; w < kWordsC; ++w) see[w] = ~0u;
-            if (!plain) {
-                const bool in = t < L && ((there >> ((jl / pl.box) * (D / 64))) & 1u);
-#pragma unroll
-                for (int w = 0; w < kWordsC; ++w)
-                    see[w] = !in ? 0u : t < ctx ? ~0u : tmask[(t - ctx) * kWordsC + w];
-                // V of positions that some row does not see: what is not finite
-                // would reach every row through 0 * v; it is taken out here and added
-                // to the rows that see it by the summing warps
-                if (ok) ok = tc::mbar_wait(kv_full + 8 * (vu % NS), (vu / NS) & 1, &g_tree_timeout);
-                if (t >= ctx || !in) {
-                    unsigned char *vr = slots + (vu % NS) * F::kSlot + jl * 128;
-                    bool bad = false;
-                    constexpr int kPieces = D / 8 / kSW;
-                    for (int e = 0; e < kPieces; ++e) {
-                        const int ch = wg * kPieces + e;
-                        uint4 *p = reinterpret_cast<uint4 *>(vr + (ch >> 3) * (kTile * 128) + (((ch & 7) ^ (jl & 7)) << 4));
-                        if (!in) {
-                            *p = make_uint4(0, 0, 0, 0);
-                        } else {
-                            uint4 v = *p;
-                            uint32_t *x = reinterpret_cast<uint32_t *>(&v);
-                            bool hit = false;
-#pragma unroll
-                            for (int y = 0; y < 4; ++y)
-                                if (nonfinite2<C>(x[y])) {
-                                    constexpr uint32_t ee = std::is_same<C, __half>::value ? 0x7c00u : 0x7f80u;
-                                    hit = true;
-                                    if ((x[y] & ee) == ee) x[y] &= 0xffff0000u;
-                                    if (((x[y] >> 16) & ee) == ee) x[y] &= 0x0000ffffu;
-                                }
-                            if (hit) {
-                                *p = v;
-                                bad = true;
-                            }
+                        for (int w = 0; w < 2; ++w) {
+                            const int at = wg * 64 + w * 32;
+                            const uint32_t lo = (there >> (at / ly.box * (D / 64))) & 1u;
+                            const uint32_t hi = (there >> ((at + 16) / ly.box * (D / 64))) & 1u;
+                            see[w] = seen_word(anc, ly.words, t0 + w * 32, ctx, sg.L) &
+                                     ((lo ? 0xffffu : 0u) | (hi ? 0xffff0000u : 0u));
                         }
                     }
-                    if (bad) atomicOr(&bad_s[(i & 3) * 4 + w4], 1u << lane);
-                }
-            }
-            tc::tc_fence_after();
-
-            // maxima of the columns over the tile
-            float sv[kCols];
-            {
-                uint32_t r[kCols];
-#pragma unroll
-                for (int c = 0; c < kCols; c += 16)
-                    tc::tmem_ld16(tm_s + b * NC + lane_off + c0 + c, *reinterpret_cast<uint32_t(*)[16]>(r + c));
-                tc::tmem_wait_ld();
-#pragma unroll
-                for (int c = 0; c < kCols; ++c) sv[c] = __uint_as_float(r[c]);
-            }
-            tc::tc_fence_before();
-            mbar_arrive(s_empty + 8 * b);
-            float keep = -INFINITY;
-            if (plain) {
-#pragma unroll
-                for (int c = 0; c < kCols; ++c) {
-                    const float v = redux_max(sv[c]);
-                    if (lane == c % 32) keep = v;
-                }
-            } else {
-#pragma unroll
-                for (int c = 0; c < kCols; ++c) {
-                    const bool on = (see[(c0 + c) / 32] >> ((c0 + c) % 32)) & 1u;
-                    const float v = redux_max(on ? sv[c] : -INFINITY);
-                    if (lane == c % 32) keep = v;
-                }
-            }
-            if (lane < kCols) wmax[w4 * kCols + lane] = keep;
-            bar_sync(1 + wg, 128);
-            if (own < kCols) {
-                float v = fmaxf(fmaxf(wmax[own], wmax[kCols + own]), fmaxf(wmax[2 * kCols + own], wmax[3 * kCols + own]));
-                v = v == -INFINITY ? v : v * cs_own;
-                const float m = fmaxf(m_own, v);
-                alpha_s[(i & 3) * NC + c0 + own] = m_own == m ? 1.0f : ex2(m_own - m);
-                m_own = m;
-                cm_s[c0 + own].y = m == -INFINITY ? 0.0f : m - kPBias;
-            }
-            bar_sync(1 + wg, 128);
-
-            // p, its sum, and p into shared memory as hi + lo
-            if (i > 0 && ok) ok = tc::mbar_wait(p_empty, (i - 1) & 1, &g_tree_timeout);
-            unsigned char *pd = p_s + (c0 / 8) * (kTile * 16) + jl * 16;
-#pragma unroll
-            for (int c8 = 0; c8 < kCols; c8 += 8) {
-                uint32_t hi[4], lo[4];
-#pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    const int c = c8 + e;
-                    const float4 cm = *reinterpret_cast<const float4 *>(&cm_s[c0 + c]);
-                    const float2 al = *reinterpret_cast<const float2 *>(&alpha_s[(i & 3) * NC + c0 + c]);
-                    float pa = ex2(fmaf(sv[c], cm.x, -cm.y)), pb = ex2(fmaf(sv[c + 1], cm.z, -cm.w));
+                    tmem_wait_ld(r[0]);
+                    tmem_wait_ld(r[1]);
                     if (!plain) {
-                        pa = ((see[(c0 + c) / 32] >> ((c0 + c) % 32)) & 1u) ? pa : 0.0f;
-                        pb = ((see[(c0 + c + 1) / 32] >> ((c0 + c + 1) % 32)) & 1u) ? pb : 0.0f;
+                        // (scores are finite or NaN times a factor >= 0: -inf stays -inf)
+#pragma unroll
+                        for (int e = 0; e < 64; ++e)
+                            if (!((see[e / 32] >> (e % 32)) & 1u)) r[e / 32][e % 32] = __float_as_uint(-INFINITY);
                     }
-                    l[c] = fmaf(l[c], al.x, pa);
-                    l[c + 1] = fmaf(l[c + 1], al.y, pb);
-                    hi[e / 2] = pack2<C>(pa, pb);
-                    const float2 h = unpack2<C>(hi[e / 2]);
-                    lo[e / 2] = pack2<C>(pa - h.x, pb - h.y);
+#pragma unroll
+                    for (int e = 0; e < 64; ++e) top = fmaxf(top, __uint_as_float(r[e / 32][e % 32]));
                 }
-                *reinterpret_cast<uint4 *>(pd + (c8 / 8) * (kTile * 16)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                *reinterpret_cast<uint4 *>(pd + F::kP + (c8 / 8) * (kTile * 16)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                // the tile's maximum: the partner warp has the other positions of these rows
+                fx.px[b][wg][row] = top;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(fx.x_bar[b][wg * 4 + w4]));
+                if (!(ok = warp_wait(bar(fx.x_bar[b][(wg ^ 1) * 4 + w4]), (i >> 1) & 1))) break;
+                top = fmaxf(top, fx.px[b][wg ^ 1][row]);
+                const float cs = fx.cs[seg & 1][row];
+                const float mt = top == -INFINITY ? top : top * cs;
+                const bool move = mt > m + 7.0f && row < sg.rows;
+                const bool moved = __any_sync(~0u, move);
+                if (moved) {
+                    const float f = move ? ex2(m - mt) : 1.0f;
+                    if (wg == 0) fx.alpha[i & 3][row] = f;
+                    l *= f;
+                    if (move) m = mt;
+                }
+                if (wg == 0 && lane == 0) fx.moved[i & 3][w4] = moved;
+                if (active) {
+                    const float mm = m == -INFINITY ? 0.0f : m - kPBias;
+                    // (a factor of 0 -- scale 0 -- keeps what is masked at -inf too)
+                    const float c1 = cs == 0.0f ? 1e-38f : cs;
+                    float la = 0.0f, lb = 0.0f;
+#pragma unroll
+                    for (int c = 0; c < 64; c += 16) {
+                        uint32_t hi[8], lo[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const int x = c + 2 * e;
+                            const float pa = ex2(fmaf(__uint_as_float(r[x / 32][x % 32]), c1, -mm));
+                            const float pb = ex2(fmaf(__uint_as_float(r[x / 32][x % 32 + 1]), c1, -mm));
+                            la += pa;
+                            lb += pb;
+                            hi[e] = pack2<C>(pa, pb);
+                            const float2 h = unpack2<C>(hi[e]);
+                            lo[e] = pack2<C>(pa - h.x, pb - h.y);
+                        }
+                        tmem_st8(ts + b * kTile + c / 2, hi);
+                        tmem_st8(ts + b * kTile + 32 + c / 2, lo);
+                    }
+                    l += la + lb;
+                    tmem_wait_st();
+                }
+                tc::tc_fence_before();
+                mbar_arrive(bar(fx.p_ready[b]));
             }
-            fence_async_smem();
-            mbar_arrive(p_ready);
+            if (!ok) break;
+            fx.l[seg & 1][wg][row] = l;
+            if (wg == 0) fx.m[seg & 1][row] = m;
+            mbar_arrive(bar(fx.l_bar[seg & 1]));
+            if (lane == 0) mbar_arrive(bar(fx.seg_done[seg & 1]));
+            done();
         }
-        // sums over the positions
-#pragma unroll
-        for (int c = 0; c < kCols; ++c) {
-            float v = l[c];
-#pragma unroll
-            for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-            if (lane == c % 32) wmax[w4 * kCols + c] = v;
+    } else if (warp < kTmaWarp) {
+        // ---- output sums: thread = row, half of the head's values ----
+        constexpr int CW = D / 2;
+        const int half = (warp - kSumWarp) >> 2, w4 = warp & 3, row = tid & 127;
+        const uint32_t to = tmem + ((uint32_t)(w4 * 32) << 16) + kTmO + half * CW;
+        T *out = reinterpret_cast<T *>(a.out);
+        // rows that no node owns get zeros
+        for (int s = blockIdx.x; s < a.S; s += gridDim.x) {
+            int first;
+            const int n = node_count(a, s, first);
+            auto clear = [&](long from, long to_) {
+                for (long e = from * a.NH * D + (tid - kSumWarp * 32); e < to_ * a.NH * D; e += 256) out[e] = from_f32<T>(0.0f);
+            };
+            if (s == 0) clear(0, first);
+            clear(first + n, s + 1 < a.S ? min(max(a.starts[s + 1], first), a.T) : a.T);
         }
-        bar_sync(1 + wg, 128);
-        if (own < kCols) {
-            const float v = (wmax[own] + wmax[kCols + own]) + (wmax[2 * kCols + own] + wmax[3 * kCols + own]);
-            cm_s[c0 + own] = make_float2(v, m_own);
-        }
-    }
-    // ---- output sums: thread = value of the head ----
-    float acc[NC];
-    const bool summing = warp >= kSW * 4 && warp < kSW * 4 + 4;
-    if (summing) {
-        const int d = tid & 127;
-        const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+        const Segment *g;
+        mbar_arrive(bar(fx.q_full));            // the first segment's queries, by all warps
+        while (ok && next(g)) {
+            const volatile Segment &sg = fx.seg[seg & 3];
+            const int nt = sg.nt;
+            const bool active = w4 * 32 < sg.rows;
+            float acc[CW];
 #pragma unroll
-        for (int c = 0; c < NC; ++c) acc[c] = 0.0f;
-        for (int i = 0; i < nt; ++i) {
-            const int b = i & 1;
-            // the factors were written before p_ready, on which the product waited
-            if (ok) ok = tc::mbar_wait(o_full + 8 * b, (i >> 1) & 1, &g_tree_timeout);
-            tc::tc_fence_after();
-            const float *al = alpha_s + (i & 3) * NC;
+            for (int c = 0; c < CW; ++c) acc[c] = 0.0f;
+            for (int k = 0; k < nt; ++k, ++i) {
+                if (k == nt - 1) {
+                    // the next segment's queries, while this one's last products run
+                    if (!(ok = warp_wait(bar(fx.seg_full[(seg + 1) & 3]), ((seg + 1) >> 2) & 1))) break;
+                    const Segment &gn = fx.seg[(seg + 1) & 3];
+                    if (gn.nt > 0) {
+                        if (seg > 0 && !(ok = warp_wait(bar(fx.seg_done[(seg + 1) & 1]), (((seg + 1) >> 1) - 1) & 1))) break;
+                        if (!(ok = warp_wait(bar(fx.q_empty), seg & 1))) break;
+                        stage_queries<T, C, D>(a, ly, gn, q_s, fx.cs[(seg + 1) & 1], warp - kSumWarp, 8, lane);
+                        fence_async_smem();
+                    }
+                    mbar_arrive(bar(fx.q_full));
+                }
+                const int b = i & 1;
+                if (!(ok = warp_wait(bar(fx.o_full[b]), (i >> 1) & 1))) break;
+                tc::tc_fence_after();
+                if (active) {
+                    // (written before the probabilities, on which the product waited)
+                    if (k > 0 && *reinterpret_cast<volatile uint32_t *>(&fx.moved[i & 3][w4])) {
+                        const float f = fx.alpha[i & 3][row];
 #pragma unroll
-            for (int c = 0; c < NC; c += 16) {
-                uint32_t r[16];
-                tc::tmem_ld16(tm_o + b * NC + lane_off + c, r);
-                tc::tmem_wait_ld();
+                        for (int c = 0; c < CW; ++c) acc[c] *= f;
+                    }
 #pragma unroll
-                for (int e = 0; e < 16; e += 4) {
-                    const float4 f = *reinterpret_cast<const float4 *>(al + c + e);
-                    acc[c + e] = fmaf(acc[c + e], f.x, __uint_as_float(r[e]));
-                    acc[c + e + 1] = fmaf(acc[c + e + 1], f.y, __uint_as_float(r[e + 1]));
-                    acc[c + e + 2] = fmaf(acc[c + e + 2], f.z, __uint_as_float(r[e + 2]));
-                    acc[c + e + 3] = fmaf(acc[c + e + 3], f.w, __uint_as_float(r[e + 3]));
+                    for (int c = 0; c < CW; c += 16) {
+                        uint32_t r[16];
+                        tc::tmem_ld16(to + b * 128 + c, r);
+                        tmem_wait_ld(r);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) acc[c + e] += __uint_as_float(r[e]);
+                    }
+                    const int t0 = (sg.tile0 + k) * kTile, ctx = sg.ctx;
+                    if (t0 + kTile > ctx) {
+                        const uint32_t *anc = anc_s + ((seg & 1) * a.max_nodes + min((sg.r0 + row) / G, sg.n - 1)) * ly.words;
+                        // values that were held back from the product: infinities and NaN
+                        for (int w = 0; w < 4; ++w) {
+                            const uint32_t bad = *reinterpret_cast<volatile uint32_t *>(&fx.bad[i & 7][w]);
+                            if (!bad) continue;
+                            for (uint32_t x = bad & seen_word(anc, ly.words, t0 + 32 * w, ctx, sg.L); x; x &= x - 1) {
+                                const int t = t0 + 32 * w + __ffs(x) - 1;
+                                const int pg = a.table[(size_t)g->s * a.maxp + t / a.P];
+                                const C *v = reinterpret_cast<const C *>(a.v_pages) +
+                                             (((long)pg * a.NKV + g->kvh) * a.P + t % a.P) * D + half * CW;
+#pragma unroll
+                                for (int c = 0; c < CW; c += 2) {
+                                    const float2 y = unpack2<C>(*reinterpret_cast<const volatile uint32_t *>(v + c));
+                                    if (!(fabsf(y.x) <= 3.402823466e38f)) acc[c] += y.x;
+                                    if (!(fabsf(y.y) <= 3.402823466e38f)) acc[c + 1] += y.y;
+                                }
+                            }
+                        }
+                        __syncwarp();
+                    }
+                }
+                tc::tc_fence_before();
+                mbar_arrive(bar(fx.o_empty[b]));
+            }
+            if (!ok || !(ok = warp_wait(bar(fx.l_bar[seg & 1]), (seg >> 1) & 1))) break;
+            if (row < g->rows) {
+                const float l = fx.l[seg & 1][0][row] + fx.l[seg & 1][1][row];
+                if (g->part < 0) {
+                    const int node = (g->r0 + row) / G, h = g->r0 + row - node * G;
+                    T *o = out + ((long)(g->first + node) * a.NH + g->kvh * G + h) * D + half * CW;
+                    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+                    for (int c = 0; c < CW; c += 8) store8(o + c, acc + c, l == 0.0f, inv);
+                } else {
+                    const size_t at = ((size_t)blockIdx.x * 2 + g->part) * kRows + row;
+#pragma unroll
+                    for (int c = 0; c < CW; c += 4)
+                        *reinterpret_cast<float4 *>(ws.acc + at * D + half * CW + c) =
+                            make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+                    if (half == 0) ws.ml[at] = make_float2(fx.m[seg & 1][row], l);
                 }
             }
-            tc::tc_fence_before();
-            const int t0 = (tile0 + i) * kTile;
-            if (t0 + kTile > ctx) {
-                // values that were taken out of the product: infinities and NaN
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(fx.seg_done[seg & 1]));
+            done();
+        }
+    } else {
+        // ---- values of tiles that hold drafted tokens or end the context: rows past
+        // the end are zeroed; of the drafted ones, which some rows do not see,
+        // what is not finite would reach every row through 0 * v: it is taken out
+        // here and added to the rows that see it by the summing warps.  Before
+        // them, the ancestors ----
+        const Segment *g;
+        int fixes = 0;
+        Turn vt;
+        while (ok && next(g)) {
+            const int nt = g->nt, tile0 = g->tile0, ctx = g->ctx, L = g->L;
+            if (seg > 1 && !(ok = warp_wait(bar(fx.seg_done[seg & 1]), ((seg >> 1) - 1) & 1))) break;
+            if ((tile0 + nt) * kTile > ctx) stage_ancestors(a, *g, anc_s + (seg & 1) * a.max_nodes * ly.words, ly.words, lane);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(fx.anc_full[seg & 1]));
+            for (int k = 0; k < nt; ++k, ++i, vt.step(ly.nv)) {
+                const int t0 = (tile0 + k) * kTile;
+                if (t0 + kTile <= ctx) continue;
+                if (!(ok = warp_wait(bar(fx.fix_ask), fixes++ & 1))) break;
+                if (!(ok = warp_wait(bar(fx.v_full[vt.slot]), vt.parity))) break;
                 for (int w = 0; w < 4; ++w) {
-                    uint32_t m = *reinterpret_cast<volatile uint32_t *>(&bad_s[(i & 3) * 4 + w]);
-                    for (; m; m &= m - 1) {
-                        const int t = t0 + w * 32 + __ffs(m) - 1;
-                        if (t < ctx || t >= L || d >= D) continue;
-                        const int pg = a.table[(size_t)s * a.maxp + t / a.P];
-                        const C v = reinterpret_cast<const C *>(a.v_pages)[(((long)pg * a.NKV + kvh) * a.P + t % a.P) * D + d];
-                        const float x = to_f32(v);
-                        if (fabsf(x) <= 3.402823466e38f) continue;
-                        const uint32_t *see = tmask + (t - ctx) * kWordsC;
-#pragma unroll
-                        for (int c = 0; c < NC; ++c)
-                            if ((see[c / 32] >> (c % 32)) & 1u) acc[c] += x;
+                    const int j = w * 32 + lane, t = t0 + j;
+                    bool bad = false;
+                    if (t >= ctx) {
+                        unsigned char *vr = v_s + vt.slot * F::kSlot + j * 128;
+#pragma unroll 4
+                        for (int ch = 0; ch < D / 8; ++ch) {
+                            uint4 *p = reinterpret_cast<uint4 *>(vr + (ch >> 3) * (kTile * 128) + (((ch & 7) ^ (j & 7)) << 4));
+                            if (t >= L) {
+                                *p = make_uint4(0, 0, 0, 0);
+                                continue;
+                            }
+                            uint4 v = *p;
+                            if (finite2<C>(v.x) & finite2<C>(v.y) & finite2<C>(v.z) & finite2<C>(v.w)) continue;
+                            bad = true;
+                            v.x = held2<C>(v.x);
+                            v.y = held2<C>(v.y);
+                            v.z = held2<C>(v.z);
+                            v.w = held2<C>(v.w);
+                            *p = v;
+                        }
                     }
+                    const uint32_t x = __ballot_sync(~0u, bad);
+                    if (lane == 0) fx.bad[i & 7][w] = x;
                 }
-                bar_sync(3, 128);
-                if (d < 4) bad_s[(i & 3) * 4 + d] = 0;
+                fence_async_smem();
+                mbar_arrive(bar(fx.fix_done));
             }
-            mbar_arrive(o_empty + 8 * b);
+            if (ok) done();
         }
     }
     __syncwarp();
     tc::tc_fence_before();
     __syncthreads();
-    if (warp == kMmaWarp) tc::tmem_dealloc(tmem, F::kTmem);
-    if (!ok) return;
-    if (summing) {
-        const int d = tid & 127;
-        float *part = reinterpret_cast<float *>(a.workspace);
-        const long heads = (long)a.T * a.NH;
-        float2 *ml = reinterpret_cast<float2 *>(part + (size_t)pl.splits * heads * D);
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            if (c < rows) {
-                const int node = (r0 + c) / G;
-                const long row = (long)(first + node) * a.NH + kvh * G + (r0 + c - node * G);
-                const float2 st = cm_s[c];
-                if (nsl == 1) {
-                    if (d < D) out[row * D + d] = from_f32<T>(st.x == 0.0f ? 0.0f : acc[c] / st.x);
-                } else {
-                    if (d < D) part[(z * heads + row) * D + d] = acc[c];
-                    if (d == 0) ml[z * heads + row] = make_float2(st.y, st.x);
-                }
-            }
-        }
-    }
+    if (warp == kMmaWarp) tc::tmem_dealloc(tmem, kTmCols);
 }
 
-// Joins the slices of each row: weights 2^(m_z - max m).  One warp per row and head.
+// Joins the parts of the pairs that more than one CTA worked on: weights
+// 2^(m_part - max m).  grid (CTAs, rows / 8): block (c, y) has the pair whose
+// first part is CTA c's last segment; one warp a row.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ Plan pl) {
+__global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ TreeArgs a, int ctas) {
     pdl_launch_dependents();
     pdl_wait();
-    const long heads = (long)a.T * a.NH;
-    const long w = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (w >= heads) return;
-    const int lane = threadIdx.x & 31, row = (int)(w / a.NH);
-    // the request that owns the row: the last one that starts at or before it
-    int lo = 0, hi = a.S;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.starts[mid] <= row) lo = mid;
-        else hi = mid;
+    const Workspace ws = workspace_of(a.workspace, D);
+    const int lane = threadIdx.x & 31, row = blockIdx.y * 8 + (threadIdx.x >> 5), c0 = blockIdx.x;
+    const Part p = ws.part[c0 * 2 + 1];
+    if (row >= p.rows) return;
+    // the parts: this CTA's last segment and the first ones of the CTAs behind it
+    int behind = 0;
+    for (int c = c0 + 1; c < ctas; c += 32) {
+        const Part q = c + lane < ctas ? ws.part[(c + lane) * 2] : Part{};
+        const uint32_t e = __ballot_sync(~0u, q.rows == 0 || q.ends);
+        if (e) {
+            behind = c - c0 + __ffs(e) - 1;
+            break;
+        }
     }
-    int first, ctx;
-    const int n = node_count(a, lo, first);
-    if (row < first || row >= first + n) return;
-    const int nsl = slices(context(a, lo, n, ctx), pl);
-    if (nsl == 1) return;
-    const float *part = reinterpret_cast<const float *>(a.workspace);
-    const float2 *ml = reinterpret_cast<const float2 *>(part + (size_t)pl.splits * heads * D);
+    auto at = [&](int k) { return ((size_t)(c0 + k) * 2 + (k == 0)) * kRows + row; };
     float m = -INFINITY;
-    for (int z = lane; z < nsl; z += 32) m = fmaxf(m, ml[z * heads + w].x);
+    for (int k = lane; k <= behind; k += 32) m = fmaxf(m, ws.ml[at(k)].x);
 #pragma unroll
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
     constexpr int E = D / 32;
     float acc[E], l = 0.0f;
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-    for (int z = 0; z < nsl; ++z) {
-        const float2 st = ml[z * heads + w];
+#pragma unroll 4
+    for (int k = 0; k <= behind; ++k) {
+        const float2 st = ws.ml[at(k)];
+        float v[E];
+        load_e<float, E>(ws.acc + at(k) * D + lane * E, v);
         const float f = st.x == m ? 1.0f : ex2(st.x - m);
         l = fmaf(st.y, f, l);
-        const float *p = part + (z * heads + w) * D + lane * E;
-        if constexpr (E == 4) {
-            const float4 v = *reinterpret_cast<const float4 *>(p);
-            acc[0] = fmaf(v.x, f, acc[0]);
-            acc[1] = fmaf(v.y, f, acc[1]);
-            acc[2] = fmaf(v.z, f, acc[2]);
-            acc[3] = fmaf(v.w, f, acc[3]);
-        } else {
-            const float2 v = *reinterpret_cast<const float2 *>(p);
-            acc[0] = fmaf(v.x, f, acc[0]);
-            acc[1] = fmaf(v.y, f, acc[1]);
-        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(v[e], f, acc[e]);
     }
-    T *o = reinterpret_cast<T *>(a.out) + w * D + lane * E;
+    const int G = a.NH / a.NKV, node = (p.r0 + row) / G, h = p.r0 + row - node * G;
+    T *o = reinterpret_cast<T *>(a.out) + ((long)(p.first + node) * a.NH + p.kvh * G + h) * D + lane * E;
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = from_f32<T>(l == 0.0f ? 0.0f : acc[e] / l);
 }
@@ -734,60 +1033,57 @@ bool map_cache(CUtensorMap *m, const void *base, uint64_t rows, int D, int box, 
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int columns_for(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
-
-Plan plan_for(int S, int max_ctx, int max_nodes, int NH, int NKV) {
-    Plan p{};
-    const int rows = max_nodes * (NH / NKV), nc = columns_for(rows);
-    p.row_tiles = (rows + nc - 1) / nc;
-    const long tiles = ((long)max_ctx + kTile - 1) / kTile;
-    const long ctas = 148l * (nc > 32 ? 1 : 2);
-    // a few slices per resident CTA even out requests of different lengths
-    long chunk = (tiles * S * NKV * p.row_tiles + 4 * ctas - 1) / (4 * ctas);
-    chunk = chunk < 1 ? 1 : chunk > tiles ? tiles : chunk;
-    p.chunk = (int)chunk;
-    p.splits = (int)((tiles + chunk - 1) / chunk);
-    return p;
+// Room for the rows that a tile has at most; the rest of shared memory in slots.
+template <typename T, int D>
+Layout layout_for(const TreeArgs &a) {
+    using F = Conf<T, D>;
+    Layout ly{};
+    const long qrows = (long)a.max_nodes * (a.NH / a.NKV);
+    ly.rows = qrows <= 32 ? 32 : qrows <= 64 ? 64 : kRows;
+    ly.q_bytes = ly.rows * D * 2;
+    ly.words = (a.max_nodes + 31) / 32;
+    ly.box = 16;
+    while (ly.box < kTile && a.P % (2 * ly.box) == 0) ly.box *= 2;
+    // (the MMA reads 128 rows of Q whatever there is room for: slots lie behind it)
+    const int rest = (((int)sizeof(Fixed) + 1023) & ~1023) + F::kQHalves * ly.q_bytes + 2 * a.max_nodes * ly.words * 4;
+    const int slots = std::min(2 * F::kMaxRing, (227 * 1024 - rest) / F::kSlot);
+    ly.nk = slots / 2;
+    ly.nv = slots - ly.nk;
+    ly.smem = rest + slots * F::kSlot;
+    return ly;
 }
 
-template <typename T, typename C, int D, int NC>
-cudaError_t launch_nc(const TreeArgs &a, Plan pl, cudaStream_t st) {
-    using F = Conf<T, D, NC>;
-    pl.box = 16;
-    while (pl.box < kTile && a.P % (2 * pl.box) == 0) pl.box *= 2;
+template <typename T, typename C, int D>
+cudaError_t launch_d(const TreeArgs &a, cudaStream_t st) {
+    const Layout ly = layout_for<T, D>(a);
     CUtensorMap mk, mv;
     const uint64_t rows = (uint64_t)a.num_pages * a.NKV * a.P;
     const bool bf = a.kv_dtype == QVL_DTYPE_BF16;
-    if (!map_cache(&mk, a.k_pages, rows, D, pl.box, bf) || !map_cache(&mv, a.v_pages, rows, D, pl.box, bf))
+    if (!map_cache(&mk, a.k_pages, rows, D, ly.box, bf) || !map_cache(&mv, a.v_pages, rows, D, ly.box, bf))
         return cudaErrorInvalidValue;
-    auto kern = tree_tc_kernel<T, C, D, NC>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
+    // no more CTAs than there can be units
+    const long qrows = (long)a.max_nodes * (a.NH / a.NKV);
+    const long units = (long)a.S * a.NKV * ((qrows + kRows - 1) / kRows) * (((long)a.max_ctx + kTile - 1) / kTile);
+    const int ctas = (int)(units < kSMs ? units : kSMs);
+    auto kern = tree_tc_kernel<T, C, D>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ly.smem);
     if (e != cudaSuccess) return e;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(pl.splits * pl.row_tiles, a.NKV, a.S);
-    cfg.blockDim = dim3(F::kThreads);
-    cfg.dynamicSmemBytes = F::kSmem;
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = ly.smem;
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kern, mk, mv, a, pl);
-    if (e != cudaSuccess || pl.splits == 1) return e;
-    cfg.gridDim = dim3((unsigned)(((long)a.T * a.NH + 7) / 8));
+    e = cudaLaunchKernelEx(&cfg, kern, mk, mv, a, ly);
+    if (e != cudaSuccess || ctas == 1) return e;
+    cfg.gridDim = dim3(ctas, (unsigned)((std::min(qrows, (long)kRows) + 7) / 8));
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
-    return cudaLaunchKernelEx(&cfg, tree_join_kernel<T, D>, a, pl);
-}
-template <typename T, typename C, int D>
-cudaError_t launch_d(const TreeArgs &a, cudaStream_t st) {
-    const Plan pl = plan_for(a.S, a.max_ctx, a.max_nodes, a.NH, a.NKV);
-    switch (columns_for(a.max_nodes * (a.NH / a.NKV))) {
-    case 16: return launch_nc<T, C, D, 16>(a, pl, st);
-    case 32: return launch_nc<T, C, D, 32>(a, pl, st);
-    default: return launch_nc<T, C, D, 64>(a, pl, st);
-    }
+    return cudaLaunchKernelEx(&cfg, tree_join_kernel<T, D>, a, ctas);
 }
 template <typename T, typename C>
 cudaError_t launch_t(const TreeArgs &a, cudaStream_t st) {
@@ -800,11 +1096,7 @@ int *tree_timeout_word() {
     return cudaGetSymbolAddress(&p, g_tree_timeout) == cudaSuccess ? static_cast<int *>(p) : nullptr;
 }
 
-size_t tree_workspace_bytes(int S, int T, int max_ctx, int max_nodes, int NH, int NKV, int D) {
-    const Plan p = plan_for(S, max_ctx, max_nodes, NH, NKV);
-    if (p.splits == 1) return 0;
-    return ((size_t)p.splits * T * NH * (D * sizeof(float) + sizeof(float2)) + 255) & ~(size_t)255;
-}
+size_t tree_workspace_bytes(int D) { return (part_bytes(D) + 255) & ~(size_t)255; }
 
 cudaError_t launch_tree_attention(const TreeArgs &a, cudaStream_t st) {
     if (a.kv_dtype == QVL_DTYPE_BF16) return launch_t<__nv_bfloat16, __nv_bfloat16>(a, st);
