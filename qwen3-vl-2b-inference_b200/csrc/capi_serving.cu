@@ -119,6 +119,8 @@ int qvl_tree_attention(const void *q, int dtype, size_t q_stride, const void *k_
     const bool types = (kv_dtype == QVL_DTYPE_FP16 && (dtype == QVL_DTYPE_FP16 || dtype == QVL_DTYPE_FP32)) ||
                        (kv_dtype == QVL_DTYPE_BF16 && dtype == QVL_DTYPE_BF16);
     if (!types || (D != 64 && D != 128) || max_nodes > qvl::kTreeMaxNodes) return QVL_ERR_UNSUPPORTED;
+    // the heads of a key head are more than 128: more than a tile of rows
+    if (dims->num_heads / dims->num_kv_heads > 128) return QVL_ERR_UNSUPPORTED;
     if (n_rows == 0) return QVL_OK;
     if (!k_pages || !v_pages || !page_table || !ctx_lens || !starts || !parents || !out) return QVL_ERR_INVALID;
     const size_t NH = dims->num_heads;

@@ -20,16 +20,23 @@
 //
 // Warps of a CTA:
 //   TMA      cuts the stretch into segments, finds the pages, fills a ring of slots for K
-//            and one for V (a slot: 128 positions, 128-byte swizzle)
+//            and one for V (a slot: 128 positions, 128-byte swizzle); a segment's Q goes
+//            through the K ring ahead of its keys
 //   MMA      S = Q K^T [128 rows, 128 positions], O = P V [128 rows, D], one thread;
-//            S, P and O in tensor memory, two buffers each, P over S
+//            Q, S, P (over S) and O in tensor memory, so that shared memory, whose
+//            bandwidth the products would need most of otherwise, is read for K and V alone
 //   softmax  two warpgroups, half of a tile's positions each; thread = row, so that maximum
 //            and sum need one exchange with the partner warp.  The maximum is left as it is
 //            until a score passes it by 2^7, which p held times 2^8 in fp16 allows: almost
-//            no tile rescales anything
+//            no tile rescales anything.  Between segments they bring the next one's Q to
+//            tensor memory
+//            A tile of at most 32 (64) rows is there four times (twice) over, in as many
+//            blocks of the 128 rows: each block takes its share of the positions and
+//            has p = 0 elsewhere, so that all warps have work, and the blocks are
+//            added at the end like parts of a context
 //   sums     two warpgroups (half of D each) add each tile's O to fp32 registers: the
 //            tensor cores do not round their sums to nearest, so no chain of them is
-//            longer than a tile; and they bring the next segment's Q to shared memory
+//            longer than a tile
 //   fixer    the nodes' ancestors as bits, and values of the drafted tile that some
 //            row does not see: 0 * NaN
 // fp32 queries are split q = hi + lo (fp16 each, after a power of two per row
@@ -73,14 +80,6 @@ __device__ __forceinline__ uint64_t sdesc_mn_sw128(uint32_t addr, uint32_t chunk
     return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)(chunk >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
            (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc)
-        : "memory");
-}
 // A from tensor memory: row = lane, two 16-bit values a column.
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
@@ -102,6 +101,9 @@ __device__ __forceinline__ void tmem_ld32(uint32_t t, uint32_t (&r)[32]) {
 __device__ __forceinline__ void tmem_st8(uint32_t t, const uint32_t (&r)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::QVL_V8(r, 0), "r"(t) : "memory");
 }
+__device__ __forceinline__ void tmem_ld8(uint32_t t, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : QVL_R8(r, 0) : "r"(t));
+}
 // Waits for this thread's loads; the values in r are not looked at before.
 #define QVL_RW8(r, o) "+r"(r[o]), "+r"(r[o + 1]), "+r"(r[o + 2]), "+r"(r[o + 3]), "+r"(r[o + 4]), "+r"(r[o + 5]), "+r"(r[o + 6]), "+r"(r[o + 7])
 __device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[16]) {
@@ -114,11 +116,6 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
 #undef QVL_R8
 #undef QVL_V8
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ float redux_max(float v) {
-    float r;
-    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-    return r;
-}
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -131,6 +128,28 @@ __device__ __forceinline__ float ex2(float x) {
 // A whole warp's wait: false for all lanes where one gave up.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
     return __all_sync(~0u, tc::mbar_wait(bar, parity, &g_tree_timeout));
+}
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t two(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 parts(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 
 // Two floats to packed 16-bit values (a low, b high) and what is left of them.
@@ -150,6 +169,16 @@ template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
 template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
     return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
 }
+// A pair as hi + lo, 16 bits each: hi is cut off, not rounded, so that what is
+// left needs no conversion back.
+template <typename C> __device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t &lo) {
+    constexpr uint32_t m = std::is_same<C, __half>::value ? 0xffffe000u : 0xffff0000u;
+    const float ha = __uint_as_float(__float_as_uint(a) & m), hb = __uint_as_float(__float_as_uint(b) & m);
+    if constexpr (std::is_same<C, __half>::value) hi = pack2<C>(ha, hb);
+    else hi = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+    const float2 l = parts(add2(two(a, b), two(-ha, -hb)));
+    lo = pack2<C>(l.x, l.y);
+}
 // Both halves of a packed pair are finite; the pair with those that are not set to 0.
 template <typename C> __device__ __forceinline__ bool finite2(uint32_t v) {
     constexpr uint32_t e = std::is_same<C, __half>::value ? 0x7c00u : 0x7f80u;
@@ -158,6 +187,11 @@ template <typename C> __device__ __forceinline__ bool finite2(uint32_t v) {
 template <typename C> __device__ __forceinline__ uint32_t held2(uint32_t v) {
     constexpr uint32_t e = std::is_same<C, __half>::value ? 0x7c00u : 0x7f80u;
     return ((v & e) == e ? 0u : v & 0xffffu) | (((v >> 16) & e) == e ? 0u : v & 0xffff0000u);
+}
+template <typename T> __device__ __forceinline__ void store4(T *o, const float4 &acc, bool none, float inv) {
+    const float4 x = none ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(o) = x;
+    else *reinterpret_cast<uint2 *>(o) = make_uint2(pack2<T>(x.x, x.y), pack2<T>(x.z, x.w));
 }
 // Eight outputs acc / l (`inv` = 1 / l), rounded once.
 template <typename T> __device__ __forceinline__ void store8(T *o, const float *acc, bool none, float inv) {
@@ -194,7 +228,8 @@ __device__ __forceinline__ Request request_of(const TreeArgs &a, int s) {
     r.n = node_count(a, s, r.first);
     r.L = context(a, s, r.n, r.ctx);
     r.tiles = (r.L + kTile - 1) / kTile;
-    r.row_tiles = (r.n * (a.NH / a.NKV) + kRows - 1) / kRows;
+    const int per = kRows / (a.NH / a.NKV);     // whole nodes of a tile of rows
+    r.row_tiles = (r.n + per - 1) / per;
     r.units = (long)r.tiles * r.row_tiles * a.NKV;
     return r;
 }
@@ -215,26 +250,29 @@ struct Conf {
     static constexpr int kQHalves = kSplitQ ? 2 : 1;
     static constexpr int kSlot = kTile * D * 2;
     static constexpr int kMaxRing = 4;
+    static constexpr int kOB = D == 64 ? 2 : 1;             // buffers of O
 };
-// Shared memory of a launch: the rest of an SM's after Q goes to the rings.
+// Shared memory of a launch: what an SM has goes to the rings.
 struct Layout {
-    int rows;           // of a tile that Q has room for
-    int q_bytes;        // of one half of Q
     int nk, nv;         // slots for K and for V
     int words;          // of a node's ancestors
-    int box;            // positions per TMA box
+    int box, box_log2;  // positions per TMA box
+    uint32_t all;       // a bit for each box of a tile (and half of D)
+    int q_rows;         // query rows of a tile: whole nodes
     int smem;
 };
-// What does not depend on the launch, behind Q.
+// What does not depend on the launch.
 struct Fixed {
     float alpha[4][kRows];          // factors of the sums, by tile
     float cs[2][kRows];             // score factors, by segment
     float l[2][2][kRows];           // sums of p, by segment and warpgroup
     float m[2][kRows];              // maxima, by segment
     float px[2][2][kRows];          // maxima of a tile's halves, by tile and warpgroup
+    float qmax[2][kRows];           // maxima of a query row's halves
+    float blocks[2][kRows][20];     // 16 values of each block's rows, to be added, by half of D
     Segment seg[4];
     uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], p_ready[2], o_full[2], o_empty[2], x_bar[2][8], q_full,
-        q_empty, anc_full[2], seg_full[4], seg_empty[4], l_bar[2], seg_done[2], fix_ask, fix_done;
+        q_empty, anc_full[2], seg_full[4], seg_empty[4], l_bar[2], seg_done[2], qmax_bar, block_bar[2], fix_ask, fix_done;
     uint32_t valid[8];              // boxes of a tile that exist, by tile
     uint32_t bad[8][4];             // positions with values held back, by tile
     uint32_t moved[4][4];           // some maximum moved, by tile and warp
@@ -243,8 +281,8 @@ struct Fixed {
     uint32_t tmem;
     int off;
 };
-// Tensor memory columns: S/P (128 each), O (128 each)
-constexpr uint32_t kTmO = 256, kTmCols = 512;
+// Tensor memory columns: S/P (128 each, two), O (D: one buffer of 128 or two of 64), Q
+constexpr uint32_t kTmO = 256, kTmQ = 384, kTmCols = 512;
 
 __host__ __device__ constexpr size_t part_floats(int D) { return (size_t)kRows * D; }
 __host__ __device__ constexpr size_t part_bytes(int D) {
@@ -263,54 +301,6 @@ __device__ __forceinline__ Workspace workspace_of(void *p, int D) {
     return w;
 }
 
-// One row of Q into shared memory, K-major with 128-byte swizzle, by a warp
-// (lane: E consecutive values); rows past the last one are zero.
-template <typename T, typename C, int D>
-__device__ __forceinline__ void stage_row(float (&x)[D / 32], int r, float qmul, const Layout &ly, unsigned char *q_s,
-                                          float *cs_s, int lane) {
-    using F = Conf<T, D>;
-    constexpr int E = D / 32;
-    float cs = fabsf(qmul);
-    if constexpr (F::kSplitQ) {
-        float mx = 0.0f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            x[e] *= qmul;
-            mx = fmaxf(mx, fabsf(x[e]));
-        }
-        mx = redux_max(mx);
-        // largest value into [2^9, 2^10)
-        int ex = (int)(__float_as_uint(mx) >> 23);
-        if (mx == 0.0f || ex == 255) ex = 127 + 9;
-        ex = max(ex, 10);
-        const float f = __uint_as_float((uint32_t)min(254, 263 - ex) << 23);
-        cs = __uint_as_float((uint32_t)(ex - 9) << 23);
-#pragma unroll
-        for (int e = 0; e < E; ++e) x[e] *= f;
-    } else if (qmul < 0.0f) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = -x[e];
-    }
-    const int half = (lane * E) >> 6, in = (lane * E) & 63;
-    unsigned char *dst = q_s + half * (ly.rows * 128) + r * 128 + ((((in * 2) >> 4) ^ (r & 7)) << 4) + ((in * 2) & 15);
-    uint32_t hi[E / 2], lo[E / 2];
-#pragma unroll
-    for (int e = 0; e < E; e += 2) {
-        hi[e / 2] = pack2<C>(x[e], x[e + 1]);
-        if constexpr (F::kSplitQ) {
-            const float2 h = unpack2<C>(hi[e / 2]);
-            lo[e / 2] = pack2<C>(x[e] - h.x, x[e + 1] - h.y);
-        }
-    }
-    if constexpr (E == 4) {
-        *reinterpret_cast<uint2 *>(dst) = make_uint2(hi[0], hi[1]);
-        if constexpr (F::kSplitQ) *reinterpret_cast<uint2 *>(dst + ly.q_bytes) = make_uint2(lo[0], lo[1]);
-    } else {
-        *reinterpret_cast<uint32_t *>(dst) = hi[0];
-        if constexpr (F::kSplitQ) *reinterpret_cast<uint32_t *>(dst + ly.q_bytes) = lo[0];
-    }
-    if (lane == 0) cs_s[r] = cs;
-}
 template <typename T, int E>
 __device__ __forceinline__ void load_e(const T *p, float (&x)[E]) {
     if constexpr (sizeof(T) * E == 16) {
@@ -330,31 +320,72 @@ __device__ __forceinline__ void load_e(const T *p, float (&x)[E]) {
         for (int e = 0; e < E; ++e) x[e] = to_f32(t[e]);
     }
 }
-// The segment's query rows, warp w of nw; several rows' loads in flight.
+// Half of a query row from the K ring's slots (rows of 128 bytes, 128-byte swizzle) into
+// tensor memory (columns of two 16-bit values, hi and then lo) by the thread of the row,
+// and the row's score factor.  False where a wait gave up.
 template <typename T, typename C, int D>
-__device__ __forceinline__ void stage_queries(const TreeArgs &a, const Layout &ly, const Segment &g, unsigned char *q_s,
-                                              float *cs_s, int w, int nw, int lane) {
-    constexpr int E = D / 32, U = 4;
-    const int G = a.NH / a.NKV;
+__device__ __forceinline__ bool stage_queries(const TreeArgs &a, Fixed &fx, const unsigned char *const (&slot)[2], float *cs_s,
+                                              uint32_t tq, int half, int row, int cap, int turn) {
+    using F = Conf<T, D>;
+    constexpr int H = D / 2, V = 16 / sizeof(T);             // values of 16 bytes
+    const int lane = threadIdx.x & 31, src = row & (cap - 1);
     const float qmul = a.scale * kLog2e;
-    const int nr = (g.rows + 7) & ~7;           // rows past these are never looked at
-    for (int r = w; r < nr; r += nw * U) {
-        float x[U][E];
+    // values [c, c + V) of the half
+    auto load = [&](int c, float (&x)[V]) {
+        const int byte = (half * H + c) * (int)sizeof(T), chunk = byte >> 7;
+        const unsigned char *p = slot[chunk / (F::kSlot / 16384)] + chunk % (F::kSlot / 16384) * 16384;
+        const uint4 v = *reinterpret_cast<const uint4 *>(p + src * 128 + ((((byte >> 4) & 7) ^ (src & 7)) << 4));
+        const T *t = reinterpret_cast<const T *>(&v);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int rr = r + u * nw;
+        for (int e = 0; e < V; ++e) x[e] = to_f32(t[e]);
+    };
+    float f = qmul < 0.0f ? -1.0f : 1.0f, cs = fabsf(qmul);
+    if constexpr (F::kSplitQ) {
+        float mx = 0.0f;
 #pragma unroll
-            for (int e = 0; e < E; ++e) x[u][e] = 0.0f;
-            if (rr < g.rows) {
-                const int node = (g.r0 + rr) / G, h = (g.r0 + rr) - node * G;
-                load_e<T, E>(reinterpret_cast<const T *>(a.q) + (long)(g.first + node) * a.q_stride +
-                                 (long)(g.kvh * G + h) * D + lane * E, x[u]);
+        for (int c = 0; c < H; c += V) {
+            float x[V];
+            load(c, x);
+#pragma unroll
+            for (int e = 0; e < V; ++e) mx = fmaxf(mx, fabsf(x[e] * qmul));
+        }
+        fx.qmax[half][row] = mx;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(tc::smem_u32(&fx.qmax_bar));
+        if (!warp_wait(tc::smem_u32(&fx.qmax_bar), turn & 1)) return false;
+        mx = fmaxf(mx, fx.qmax[half ^ 1][row]);
+        // largest value into [2^9, 2^10)
+        int ex = (int)(__float_as_uint(mx) >> 23);
+        if (mx == 0.0f || ex == 255) ex = 127 + 9;
+        ex = max(ex, 10);
+        f = __uint_as_float((uint32_t)min(254, 263 - ex) << 23);
+        cs = __uint_as_float((uint32_t)(ex - 9) << 23);
+    }
+#pragma unroll
+    for (int c = 0; c < H; c += 16) {
+        uint32_t hi[8], lo[8];
+#pragma unroll
+        for (int v = 0; v < 16 / V; ++v) {
+            float x[V];
+            load(c + v * V, x);
+#pragma unroll
+            for (int e = 0; e < V; e += 2) {
+                const int at = (v * V + e) / 2;
+                const float y = F::kSplitQ ? x[e] * qmul * f : x[e] * f, z = F::kSplitQ ? x[e + 1] * qmul * f : x[e + 1] * f;
+                hi[at] = pack2<C>(y, z);
+                if constexpr (F::kSplitQ) {
+                    const float2 w = unpack2<C>(hi[at]);
+                    lo[at] = pack2<C>(y - w.x, z - w.y);
+                }
             }
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (r + u * nw < nr) stage_row<T, C, D>(x[u], r + u * nw, qmul, ly, q_s, cs_s, lane);
+        tmem_st8(tq + half * (H / 2) + c / 2, hi);
+        if constexpr (F::kSplitQ) tmem_st8(tq + D / 2 + half * (H / 2) + c / 2, lo);
     }
+    tmem_wait_st();
+    tc::tc_fence_before();
+    if (half == 0) cs_s[row] = cs;
+    return true;
 }
 // Ancestors of every node as bits, its own among them: a node's are its parent's and itself.  One warp.
 __device__ __forceinline__ void stage_ancestors(const TreeArgs &a, const Segment &g, uint32_t *anc, int words, int lane) {
@@ -407,19 +438,26 @@ __device__ __forceinline__ void tma_load_once(uint32_t dst, const CUtensorMap *m
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar), "l"(pol)
         : "memory");
 }
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
 }  // namespace
 
-template <typename T, typename C, int D>
+// CAP: rows of a block (32, 64 or 128).
+template <typename T, typename C, int D, int CAP>
 __global__ void __launch_bounds__(kThreads, 1)
 tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+               const __grid_constant__ CUtensorMap tm_q,
                const __grid_constant__ TreeArgs a, const __grid_constant__ Layout ly) {
     using F = Conf<T, D>;
     // (addresses in it are constants, which keeps them out of the registers)
     extern __shared__ __align__(1024) unsigned char smem[];
     Fixed &fx = *reinterpret_cast<Fixed *>(smem);
     constexpr int kHead = ((int)sizeof(Fixed) + 1023) & ~1023;
-    unsigned char *q_s = smem + kHead;                              // hi, then lo
-    unsigned char *k_s = q_s + F::kQHalves * ly.q_bytes;            // slots of K, of V
+    unsigned char *k_s = smem + kHead;                              // slots of K, of V
     unsigned char *v_s = k_s + ly.nk * F::kSlot;
     uint32_t *anc_s = reinterpret_cast<uint32_t *>(v_s + ly.nv * F::kSlot);     // [2][node][words], by segment
     auto bar = [](uint64_t &b) { return tc::smem_u32(&b); };
@@ -448,11 +486,15 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
         }
         tc::mbar_init(bar(fx.q_full), 256);
         tc::mbar_init(bar(fx.q_empty), 1);
+        tc::mbar_init(bar(fx.qmax_bar), 8);
+        tc::mbar_init(bar(fx.block_bar[0]), 4);
+        tc::mbar_init(bar(fx.block_bar[1]), 4);
         tc::mbar_init(bar(fx.fix_ask), 1);
         tc::mbar_init(bar(fx.fix_done), 32);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         tc::prefetch_tmap(&tm_k);
         tc::prefetch_tmap(&tm_v);
+        tc::prefetch_tmap(&tm_q);
     }
     if (warp == kMmaWarp) {
         tc::tmem_alloc(tc::smem_u32(&fx.tmem), kTmCols);
@@ -485,8 +527,16 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
         }
         // (fewer units than CTAs: the last CTAs have none, so that a pair's parts
         // are in consecutive CTAs)
-        const long ctas = min((long)gridDim.x, max(total, 1l)), me = min((long)blockIdx.x, ctas);
-        const long lo = total * me / ctas, hi = total * min(me + 1, ctas) / ctas;
+        const long ctas = min((long)gridDim.x, max(total, 1l)), me = blockIdx.x;
+        long each, more;
+        if (total < 1l << 31) {
+            each = (uint32_t)total / (uint32_t)ctas;
+            more = (uint32_t)total % (uint32_t)ctas;
+        } else {
+            each = total / ctas;
+            more = total % ctas;
+        }
+        const long lo = min(each * me + min(me, more), total), hi = min(lo + each + (me < more ? 1 : 0), total);
         if (lo < hi && before <= lo && lo < before + mine) {
             int s = s0;
             long u = request_of(a, s).units;
@@ -518,16 +568,6 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
         ++seg;
     };
 
-    if (warp < kTmaWarp) {
-        // the first segment's queries: the warps that have nothing to do yet
-        if (ok) ok = warp_wait(bar(fx.seg_full[0]), 0);
-        if (ok && fx.seg[0].nt > 0) {
-            stage_queries<T, C, D>(a, ly, fx.seg[0], q_s, fx.cs[0], warp, kTmaWarp, lane);
-            fence_async_smem();
-        }
-        asm volatile("bar.sync 1, %0;" ::"n"(kTmaWarp * 32) : "memory");
-    }
-
     if (warp == kTmaWarp) {
         // ---- segments, pages and loads ----
         int s = (int)fx.range[0];
@@ -537,12 +577,12 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
         if (lane < 2) ws.part[blockIdx.x * 2 + lane].rows = 0;
         __syncwarp();
         // lane l: box l / (D / 64) of the tile's 64-value half l % (D / 64)
-        const int lanes = kTile / ly.box * (D / 64);
+        const int lanes = (kTile >> ly.box_log2) * (D / 64);
         const int bx = lane / (D / 64), half = lane % (D / 64);
         const int oob = (int)(a.num_pages * a.NKV * a.P);          // past the last row: zeros
         const int to = half * (kTile * 128) + bx * ly.box * 128;
         Turn kt, vt;
-        int loads = 0;                                             // K slots filled; V slots are one behind at most
+        int loads = 0;                                             // slots of the K ring filled
         uint64_t once;
         asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(once));
         while (ok) {
@@ -552,11 +592,12 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                     off -= rq.units;
                     rq = request_of(a, ++s);
                 }
-                const int pair = (int)(off / rq.tiles);            // key head, then tile of rows
+                // key head, then tile of rows
+                const int pair = off < 1l << 31 ? (int)((uint32_t)off / (uint32_t)rq.tiles) : (int)(off / rq.tiles);
                 g.s = s;
                 g.kvh = pair / rq.row_tiles;
-                g.r0 = (pair - g.kvh * rq.row_tiles) * kRows;
-                g.rows = min(kRows, rq.n * G - g.r0);
+                g.r0 = (pair - g.kvh * rq.row_tiles) * ly.q_rows;
+                g.rows = min(ly.q_rows, rq.n * G - g.r0);
                 g.tile0 = (int)(off - (long)pair * rq.tiles);
                 g.nt = (int)min(left, (long)(rq.tiles - g.tile0));
                 g.ctx = rq.ctx;
@@ -578,6 +619,16 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             }
             ++seg;
             if (g.nt == 0) break;
+            for (int h = 0; h < F::kQHalves; ++h, ++loads, kt.step(ly.nk)) {
+                constexpr int per = F::kSlot / 16384;               // boxes of 128 bytes a row
+                if (loads >= ly.nk && !(ok = warp_wait(bar(fx.k_empty[kt.slot]), kt.parity ^ 1))) break;
+                if (lane == 0) tc::mbar_expect_tx(bar(fx.k_full[kt.slot]), per * ly.q_rows * 128);
+                __syncwarp();
+                if (lane < per)
+                    tma_load_3d(tc::smem_u32(k_s + kt.slot * F::kSlot + lane * 16384), &tm_q,
+                                (h * per + lane) * (128 / (int)sizeof(T)), g.kvh * G, g.first + g.r0 / G, bar(fx.k_full[kt.slot]));
+            }
+            if (!ok) break;
             for (int k = 0; k < g.nt; ++k, ++i) {
                 const int t = (g.tile0 + k) * kTile + bx * ly.box;
                 int y = oob;
@@ -587,7 +638,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                     if (pg >= 0 && pg < a.num_pages) y = (int)(((long)pg * a.NKV + g.kvh) * a.P + (t - c * a.P));
                 }
                 const uint32_t there = __ballot_sync(~0u, y != oob);
-                if (i >= ly.nk && !(ok = warp_wait(bar(fx.k_empty[kt.slot]), kt.parity ^ 1))) break;
+                if (loads >= ly.nk && !(ok = warp_wait(bar(fx.k_empty[kt.slot]), kt.parity ^ 1))) break;
                 if (lane == 0) {
                     // (keys are loaded at most nk + 2 tiles ahead of the softmax
                     // that reads this)
@@ -620,26 +671,30 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
         if (lane == 0) {
             constexpr uint32_t id_s = idesc_16<C>(kTile, false), id_o = idesc_16<C>(D, true);
             // descriptors: the address is their low end, in units of 16 bytes
-            const uint64_t qd = tc::sdesc_k_sw128(tc::smem_u32(q_s)), kd = tc::sdesc_k_sw128(tc::smem_u32(k_s));
-            const uint64_t vd = sdesc_mn_sw128(tc::smem_u32(v_s), kTile * 128);
-            const uint32_t q_lo = ly.q_bytes >> 4, q_half = (ly.rows * 128) >> 4;
+            const uint64_t kd = tc::sdesc_k_sw128(tc::smem_u32(k_s)), vd = sdesc_mn_sw128(tc::smem_u32(v_s), kTile * 128);
+            constexpr int OB = F::kOB;
             int qseg = 0, qk = 0, qnt = 0, qi = 0;        // scores: segment, tile in it, its tiles, tile in all
-            bool more = ok;
+            bool more = ok, begun = false;
             Turn kt, vt;
             auto wait = [&](uint64_t &b, uint32_t parity) { return ok = tc::mbar_wait(bar(b), parity, &g_tree_timeout); };
             // low halves first: what they add up to is small, and exact beside the
             // roundings of the high halves' sums
-            auto scores = [&] {
+            auto scores = [&](bool must) {
                 if (!more) return;
-                if (qk == 0) {
+                if (!begun) {
                     if (!wait(fx.seg_full[qseg & 3], (qseg >> 2) & 1)) return;
                     qnt = *reinterpret_cast<volatile int *>(&fx.seg[qseg & 3].nt);
                     if (qnt == 0) {
                         more = false;
                         return;
                     }
+                    // (what is still on its way does not hold up an O that is due)
+                    if (!must && !tc::mbar_try_wait(bar(fx.q_full), qseg & 1)) return;
                     if (!wait(fx.q_full, qseg & 1)) return;
+                    for (int h = 0; h < F::kQHalves; ++h, kt.step(ly.nk)) mbar_arrive(bar(fx.k_empty[kt.slot]));
+                    begun = true;
                 }
+                if (!must && !tc::mbar_try_wait(bar(fx.k_full[kt.slot]), kt.parity)) return;
                 if (!wait(fx.k_full[kt.slot], kt.parity)) return;
                 tc::tc_fence_after();
                 const uint64_t kb = kd + (uint32_t)(kt.slot * (F::kSlot >> 4));
@@ -648,8 +703,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                 for (int l = F::kQHalves - 1; l >= 0; --l)
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k)
-                        mma_ss(d, qd + (l * q_lo + (k >> 2) * q_half + (k & 3) * 2), kb + ((k >> 2) * (kTile * 8) + (k & 3) * 2),
-                               id_s, l < F::kQHalves - 1 || k ? 1u : 0u);
+                        mma_ts(d, tmem + kTmQ + l * (D / 2) + k * 8, kb + ((k >> 2) * (kTile * 8) + (k & 3) * 2), id_s,
+                               l < F::kQHalves - 1 || k ? 1u : 0u);
                 tc::tc_commit(bar(fx.s_full[qi & 1]));
                 tc::tc_commit(bar(fx.k_empty[kt.slot]));
                 kt.step(ly.nk);
@@ -657,11 +712,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                 if (++qk == qnt) {
                     tc::tc_commit(bar(fx.q_empty));
                     qk = 0;
+                    begun = false;
                     ++qseg;
                 }
             };
-            scores();
-            if (ok) scores();
             int fixes = 0;
             while (ok && wait(fx.seg_full[seg & 3], (seg >> 2) & 1)) {
                 const volatile Segment &sg = fx.seg[seg & 3];
@@ -670,27 +724,31 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                 for (int k = 0; k < nt; ++k, ++i) {
                     const int b = i & 1;
                     const bool tail = k >= plain;
-                    if (tail) {
-                        if (!wait(fx.v_full[vt.slot], vt.parity)) break;
-                        mbar_arrive(bar(fx.fix_ask));
-                    }
-                    if (i >= 2 && !wait(fx.o_empty[b], ((i >> 1) - 1) & 1)) break;
+                    if (qi == i) scores(true);
+                    if (ok && qi == i + 1) scores(false);
+                    if (!ok) break;
+                    // (the fixer is told one tile ahead: the slot of the tile's V then has its
+                    // turn, and it waits for the load itself)
+                    if (k == 0 && tail) mbar_arrive(bar(fx.fix_ask));
+                    const bool ask = k + 1 < nt && k + 1 >= plain;
+                    if (ask && !tail) mbar_arrive(bar(fx.fix_ask));
+                    const int ob = i % OB;
+                    if (i >= OB && !wait(fx.o_empty[ob], (i / OB - 1) & 1)) break;
                     if (!wait(fx.v_full[vt.slot], vt.parity)) break;
                     if (tail && !wait(fx.fix_done, fixes++ & 1)) break;
+                    if (ask && tail) mbar_arrive(bar(fx.fix_ask));
                     if (!wait(fx.p_ready[b], (i >> 1) & 1)) break;
                     tc::tc_fence_after();
                     const uint64_t vb = vd + (uint32_t)(vt.slot * (F::kSlot >> 4));
-                    const uint32_t pb = tmem + b * kTile, d = tmem + kTmO + b * 128;
+                    const uint32_t pb = tmem + b * kTile, d = tmem + kTmO + ob * 64;
 #pragma unroll
                     for (int l = 1; l >= 0; --l)
 #pragma unroll
                         for (int c = 0; c < kTile / 16; ++c)
-                            mma_ts(d, pb + (c >> 2) * 64 + l * 32 + (c & 3) * 8, vb + c * (2048 >> 4), id_o, l == 0 || c ? 1u : 0u);
-                    tc::tc_commit(bar(fx.o_full[b]));
+                            mma_ts(d, pb + c * 16 + l * 8, vb + c * (2048 >> 4), id_o, l == 0 || c ? 1u : 0u);
+                    tc::tc_commit(bar(fx.o_full[ob]));
                     tc::tc_commit(bar(fx.v_empty[vt.slot]));
                     vt.step(ly.nv);
-                    scores();
-                    if (!ok) break;
                 }
                 if (!ok) break;
                 mbar_arrive(bar(fx.seg_empty[seg & 3]));
@@ -700,100 +758,186 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
     } else if (warp < kSumWarp) {
         // ---- softmax: thread = row, positions 64 wg .. 64 wg + 63 of each tile ----
         const int wg = warp >> 2, w4 = warp & 3, row = tid & 127;
-        const uint32_t ts = tmem + ((uint32_t)(w4 * 32) << 16) + wg * 64;
+        const uint32_t ts = tmem + ((uint32_t)(w4 * 32) << 16) + wg * 64, tq = tmem + ((uint32_t)(w4 * 32) << 16) + kTmQ;
         const Segment *g;
+        // the queries of segment n, after the products with those before them
+        Turn qt;
+        auto queries = [&](int n) {
+            if (!(ok = warp_wait(bar(fx.seg_full[n & 3]), (n >> 2) & 1))) return;
+            if (fx.seg[n & 3].nt == 0) return;
+            if (n > 0 && !(ok = warp_wait(bar(fx.q_empty), (n - 1) & 1))) return;
+            const unsigned char *slot[2];
+            for (int h = 0; h < F::kQHalves; ++h, qt.step(ly.nk)) {
+                if (!(ok = warp_wait(bar(fx.k_full[qt.slot]), qt.parity))) return;
+                slot[h] = k_s + qt.slot * F::kSlot;
+            }
+            tc::tc_fence_after();
+            if ((ok = stage_queries<T, C, D>(a, fx, slot, fx.cs[n & 1], tq, wg, row, CAP, n))) mbar_arrive(bar(fx.q_full));
+        };
+        if (ok) queries(0);
         while (ok && next(g)) {
             // (what is seldom needed is read from shared memory where it is)
             const volatile Segment &sg = fx.seg[seg & 3];
             const int nt = sg.nt;
-            const bool active = w4 * 32 < sg.rows;
+            constexpr int cap = CAP;
+            const int r = row & (cap - 1);          // the row, in its block
+            const bool active = (w4 * 32 & (cap - 1)) < sg.rows;
+            // the block's share of the 64 positions: 1, 2 or 4 chunks of 16 from c0 on
+            const int c0 = cap == 32 ? w4 : cap == 64 ? w4 & 2 : 0;
             float m = -INFINITY, l = 0.0f;
             for (int k = 0; k < nt; ++k, ++i) {
                 const int b = i & 1;
+                qt.step(ly.nk);
                 if (!(ok = warp_wait(bar(fx.s_full[b]), (i >> 1) & 1))) break;
                 tc::tc_fence_after();
                 const int t0 = (sg.tile0 + k) * kTile + wg * 64, ctx = sg.ctx;
                 const uint32_t there = *reinterpret_cast<volatile uint32_t *>(&fx.valid[i & 7]);
-                const bool plain = t0 + 64 <= ctx && there == (1u << (kTile / ly.box * (D / 64))) - 1u;
+                const bool plain = t0 + 64 <= ctx && there == ly.all;
                 if (t0 + 64 > ctx && !(ok = warp_wait(bar(fx.anc_full[seg & 1]), (seg >> 1) & 1))) break;
-                uint32_t r[2][32];
+                // what the row sees of its block's positions: chunks 0 and 1 of its share, and
+                // (a share of 64) 2 and 3
+                uint32_t see0 = ~0u, see1 = ~0u;
+                if (!plain) {
+                    const uint32_t *anc = anc_s + ((seg & 1) * a.max_nodes + min((sg.r0 + r) / G, sg.n - 1)) * ly.words;
+                    auto word = [&](int w) {
+                        const int at = wg * 64 + w * 32;
+                        const uint32_t lo = (there >> ((at >> ly.box_log2) * (D / 64))) & 1u;
+                        const uint32_t hi = (there >> (((at + 16) >> ly.box_log2) * (D / 64))) & 1u;
+                        return seen_word(anc, ly.words, t0 + w * 32, ctx, sg.L) & ((lo ? 0xffffu : 0u) | (hi ? 0xffff0000u : 0u));
+                    };
+                    see0 = word(c0 >> 1) >> (c0 & 1) * 16;
+                    if constexpr (cap == kRows) see1 = word(1);
+                }
+                const uint32_t sb = ts + b * kTile;
                 float top = -INFINITY;
                 if (active) {
-                    tmem_ld32(ts + b * kTile, r[0]);
-                    tmem_ld32(ts + b * kTile + 32, r[1]);
-                    uint32_t see[2];
-                    if (!plain) {
-                        const uint32_t *anc = anc_s + ((seg & 1) * a.max_nodes + min((sg.r0 + row) / G, sg.n - 1)) * ly.words;
+                    constexpr int n = cap / 2;          // the share's positions
+                    uint32_t v[n];
+                    if constexpr (n == 16) {
+                        tc::tmem_ld16(sb + c0 * 16, v);
+                        tmem_wait_ld(v);
+                    } else {
 #pragma unroll
-                        for (int w = 0; w < 2; ++w) {
-                            const int at = wg * 64 + w * 32;
-                            const uint32_t lo = (there >> (at / ly.box * (D / 64))) & 1u;
-                            const uint32_t hi = (there >> ((at + 16) / ly.box * (D / 64))) & 1u;
-                            see[w] = seen_word(anc, ly.words, t0 + w * 32, ctx, sg.L) &
-                                     ((lo ? 0xffffu : 0u) | (hi ? 0xffff0000u : 0u));
-                        }
+                        for (int c = 0; c < n; c += 32) tmem_ld32(sb + c0 * 16 + c, *reinterpret_cast<uint32_t(*)[32]>(v + c));
+#pragma unroll
+                        for (int c = 0; c < n; c += 32) tmem_wait_ld(*reinterpret_cast<uint32_t(*)[32]>(v + c));
                     }
-                    tmem_wait_ld(r[0]);
-                    tmem_wait_ld(r[1]);
-                    if (!plain) {
-                        // (scores are finite or NaN times a factor >= 0: -inf stays -inf)
+                    float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                        for (int e = 0; e < 64; ++e)
-                            if (!((see[e / 32] >> (e % 32)) & 1u)) r[e / 32][e % 32] = __float_as_uint(-INFINITY);
+                    for (int e = 0; e < n; ++e) {
+                        float x = __uint_as_float(v[e]);
+                        if (!plain) x = ((e < 32 ? see0 : see1) >> (e % 32)) & 1u ? x : -INFINITY;
+                        t4[e % 4] = fmaxf(t4[e % 4], x);
                     }
-#pragma unroll
-                    for (int e = 0; e < 64; ++e) top = fmaxf(top, __uint_as_float(r[e / 32][e % 32]));
+                    top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
                 }
-                // the tile's maximum: the partner warp has the other positions of these rows
+                // The partner warp has the other positions of these rows.  Its maximum is
+                // asked for at once only where this half's own does not fit under
+                // the old one (the first tile, almost always the only one); otherwise
+                // p is made with the old maximum first, and if then the partner's half
+                // turns out not to fit, p is scaled down after all.
                 fx.px[b][wg][row] = top;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(fx.x_bar[b][wg * 4 + w4]));
-                if (!(ok = warp_wait(bar(fx.x_bar[b][(wg ^ 1) * 4 + w4]), (i >> 1) & 1))) break;
-                top = fmaxf(top, fx.px[b][wg ^ 1][row]);
                 const float cs = fx.cs[seg & 1][row];
-                const float mt = top == -INFINITY ? top : top * cs;
-                const bool move = mt > m + 7.0f && row < sg.rows;
-                const bool moved = __any_sync(~0u, move);
-                if (moved) {
-                    const float f = move ? ex2(m - mt) : 1.0f;
-                    if (wg == 0) fx.alpha[i & 3][row] = f;
-                    l *= f;
-                    if (move) m = mt;
-                }
-                if (wg == 0 && lane == 0) fx.moved[i & 3][w4] = moved;
+                float f = 1.0f;                 // what a new maximum takes everything before down by
+                auto joint = [&] {
+                    if (!(ok = warp_wait(bar(fx.x_bar[b][(wg ^ 1) * 4 + w4]), (i >> 1) & 1))) return false;
+                    top = fmaxf(top, fx.px[b][wg ^ 1][row]);
+                    const float mt = top == -INFINITY ? top : top * cs;
+                    if (mt > m + 7.0f && r < sg.rows) {
+                        f = ex2(m - mt);
+                        m = mt;
+                        l *= f;
+                    }
+                    return true;
+                };
+                const bool early = __any_sync(~0u, (top == -INFINITY ? top : top * cs) > m + 7.0f && r < sg.rows);
+                if (early && !joint()) break;
                 if (active) {
                     const float mm = m == -INFINITY ? 0.0f : m - kPBias;
-                    // (a factor of 0 -- scale 0 -- keeps what is masked at -inf too)
-                    const float c1 = cs == 0.0f ? 1e-38f : cs;
-                    float la = 0.0f, lb = 0.0f;
-#pragma unroll
-                    for (int c = 0; c < 64; c += 16) {
+                    uint64_t ls = two(0.0f, 0.0f);
+                    const uint64_t cs2 = two(cs, cs), mm2 = two(-mm, -mm);
+                    // 16 scores at a time, the next ones on their way; the high and low halves
+                    // of their p take the 16 columns that they leave
+                    auto part = [&](int c, const uint32_t (&r)[16], uint32_t bits) {
                         uint32_t hi[8], lo[8];
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
-                            const int x = c + 2 * e;
-                            const float pa = ex2(fmaf(__uint_as_float(r[x / 32][x % 32]), c1, -mm));
-                            const float pb = ex2(fmaf(__uint_as_float(r[x / 32][x % 32 + 1]), c1, -mm));
-                            la += pa;
-                            lb += pb;
-                            hi[e] = pack2<C>(pa, pb);
-                            const float2 h = unpack2<C>(hi[e]);
-                            lo[e] = pack2<C>(pa - h.x, pb - h.y);
+                            float2 x = parts(fma2(two(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), cs2, mm2));
+                            if (!plain) {
+                                x.x = (bits >> (2 * e)) & 1u ? x.x : -INFINITY;
+                                x.y = (bits >> (2 * e)) & 2u ? x.y : -INFINITY;
+                            }
+                            const float pa = ex2(x.x), pb = ex2(x.y);
+                            ls = add2(ls, two(pa, pb));
+                            split2<C>(pa, pb, hi[e], lo[e]);
                         }
-                        tmem_st8(ts + b * kTile + c / 2, hi);
-                        tmem_st8(ts + b * kTile + 32 + c / 2, lo);
+                        tmem_st8(sb + c * 16, hi);
+                        tmem_st8(sb + c * 16 + 8, lo);
+                    };
+                    uint32_t ra[16], rb[16];
+                    tc::tmem_ld16(sb + c0 * 16, ra);
+                    if constexpr (cap != 32) tc::tmem_ld16(sb + c0 * 16 + 16, rb);
+                    tmem_wait_ld(ra);
+                    part(c0, ra, see0);
+                    if constexpr (cap != 32) {
+                        tmem_wait_ld(rb);
+                        if constexpr (cap == kRows) tc::tmem_ld16(sb + 32, ra);
+                        part(c0 + 1, rb, see0 >> 16);
                     }
-                    l += la + lb;
+                    if constexpr (cap == kRows) {
+                        tmem_wait_ld(ra);
+                        tc::tmem_ld16(sb + 48, rb);
+                        part(2, ra, see1);
+                        tmem_wait_ld(rb);
+                        part(3, rb, see1 >> 16);
+                    } else {
+                        // the other blocks' positions
+                        const uint32_t none[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+                            if (cap == 32 ? c != c0 : c >> 1 != c0 >> 1) {
+                                tmem_st8(sb + c * 16, none);
+                                tmem_st8(sb + c * 16 + 8, none);
+                            }
+                    }
+                    l += parts(ls).x + parts(ls).y;
                     tmem_wait_st();
                 }
+                if (!early && !joint()) break;
+                const bool moved = __any_sync(~0u, f != 1.0f);
+                if (moved) {
+                    if (wg == 0) fx.alpha[i & 3][row] = f;
+                    if (!early && active) {
+#pragma unroll 1
+                        for (int c = c0 * 16; c < c0 * 16 + cap / 2; c += 16) {
+                            uint32_t hi[8], lo[8];
+                            tmem_ld8(sb + c, hi);
+                            tmem_ld8(sb + c + 8, lo);
+                            tc::tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const float2 h = unpack2<C>(hi[e]), w = unpack2<C>(lo[e]);
+                                const float pa = (h.x + w.x) * f, pb = (h.y + w.y) * f;
+                                split2<C>(pa, pb, hi[e], lo[e]);
+                            }
+                            tmem_st8(sb + c, hi);
+                            tmem_st8(sb + c + 8, lo);
+                        }
+                        tmem_wait_st();
+                    }
+                }
+                if (wg == 0 && lane == 0) fx.moved[i & 3][w4] = moved;
                 tc::tc_fence_before();
                 mbar_arrive(bar(fx.p_ready[b]));
             }
-            if (!ok) break;
+            if (!ok || (seg > 1 && !(ok = warp_wait(bar(fx.seg_done[seg & 1]), ((seg >> 1) - 1) & 1)))) break;
             fx.l[seg & 1][wg][row] = l;
             if (wg == 0) fx.m[seg & 1][row] = m;
             mbar_arrive(bar(fx.l_bar[seg & 1]));
             if (lane == 0) mbar_arrive(bar(fx.seg_done[seg & 1]));
+            queries(seg + 1);
             done();
         }
     } else if (warp < kTmaWarp) {
@@ -813,53 +957,48 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             clear(first + n, s + 1 < a.S ? min(max(a.starts[s + 1], first), a.T) : a.T);
         }
         const Segment *g;
-        mbar_arrive(bar(fx.q_full));            // the first segment's queries, by all warps
+        int meets = 0;
         while (ok && next(g)) {
             const volatile Segment &sg = fx.seg[seg & 3];
             const int nt = sg.nt;
-            const bool active = w4 * 32 < sg.rows;
-            float acc[CW];
+            constexpr int cap = CAP;
+            const int r = row & (cap - 1);          // the row, in its block
+            const bool active = (w4 * 32 & (cap - 1)) < sg.rows;
+            uint64_t acc2[CW / 2];
 #pragma unroll
-            for (int c = 0; c < CW; ++c) acc[c] = 0.0f;
+            for (int c = 0; c < CW / 2; ++c) acc2[c] = two(0.0f, 0.0f);
             for (int k = 0; k < nt; ++k, ++i) {
-                if (k == nt - 1) {
-                    // the next segment's queries, while this one's last products run
-                    if (!(ok = warp_wait(bar(fx.seg_full[(seg + 1) & 3]), ((seg + 1) >> 2) & 1))) break;
-                    const Segment &gn = fx.seg[(seg + 1) & 3];
-                    if (gn.nt > 0) {
-                        if (seg > 0 && !(ok = warp_wait(bar(fx.seg_done[(seg + 1) & 1]), (((seg + 1) >> 1) - 1) & 1))) break;
-                        if (!(ok = warp_wait(bar(fx.q_empty), seg & 1))) break;
-                        stage_queries<T, C, D>(a, ly, gn, q_s, fx.cs[(seg + 1) & 1], warp - kSumWarp, 8, lane);
-                        fence_async_smem();
-                    }
-                    mbar_arrive(bar(fx.q_full));
-                }
-                const int b = i & 1;
-                if (!(ok = warp_wait(bar(fx.o_full[b]), (i >> 1) & 1))) break;
+                constexpr int OB = F::kOB;
+                const int ob = i % OB;
+                if (!(ok = warp_wait(bar(fx.o_full[ob]), (i / OB) & 1))) break;
                 tc::tc_fence_after();
                 if (active) {
                     // (written before the probabilities, on which the product waited)
                     if (k > 0 && *reinterpret_cast<volatile uint32_t *>(&fx.moved[i & 3][w4])) {
-                        const float f = fx.alpha[i & 3][row];
+                        const uint64_t f = two(fx.alpha[i & 3][row], fx.alpha[i & 3][row]), z = two(-0.0f, -0.0f);
 #pragma unroll
-                        for (int c = 0; c < CW; ++c) acc[c] *= f;
+                        for (int c = 0; c < CW / 2; ++c) acc2[c] = fma2(acc2[c], f, z);
                     }
 #pragma unroll
                     for (int c = 0; c < CW; c += 16) {
-                        uint32_t r[16];
-                        tc::tmem_ld16(to + b * 128 + c, r);
-                        tmem_wait_ld(r);
+                        uint32_t v[16];
+                        tc::tmem_ld16(to + ob * 64 + c, v);
+                        tmem_wait_ld(v);
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) acc[c + e] += __uint_as_float(r[e]);
+                        for (int e = 0; e < 16; e += 2)
+                            acc2[(c + e) / 2] = add2(acc2[(c + e) / 2], two(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
                     }
                     const int t0 = (sg.tile0 + k) * kTile, ctx = sg.ctx;
                     if (t0 + kTile > ctx) {
-                        const uint32_t *anc = anc_s + ((seg & 1) * a.max_nodes + min((sg.r0 + row) / G, sg.n - 1)) * ly.words;
+                        const uint32_t *anc = anc_s + ((seg & 1) * a.max_nodes + min((sg.r0 + r) / G, sg.n - 1)) * ly.words;
                         // values that were held back from the product: infinities and NaN
                         for (int w = 0; w < 4; ++w) {
                             const uint32_t bad = *reinterpret_cast<volatile uint32_t *>(&fx.bad[i & 7][w]);
                             if (!bad) continue;
-                            for (uint32_t x = bad & seen_word(anc, ly.words, t0 + 32 * w, ctx, sg.L); x; x &= x - 1) {
+                            // (by the block that has the position)
+                            const uint32_t mine = cap == kRows ? ~0u : (w & 1) != w4 >> 1 ? 0u : cap == 64 ? ~0u
+                                                                     : w4 & 1 ? 0xffff0000u : 0xffffu;
+                            for (uint32_t x = bad & mine & seen_word(anc, ly.words, t0 + 32 * w, ctx, sg.L); x; x &= x - 1) {
                                 const int t = t0 + 32 * w + __ffs(x) - 1;
                                 const int pg = a.table[(size_t)g->s * a.maxp + t / a.P];
                                 const C *v = reinterpret_cast<const C *>(a.v_pages) +
@@ -867,8 +1006,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
 #pragma unroll
                                 for (int c = 0; c < CW; c += 2) {
                                     const float2 y = unpack2<C>(*reinterpret_cast<const volatile uint32_t *>(v + c));
-                                    if (!(fabsf(y.x) <= 3.402823466e38f)) acc[c] += y.x;
-                                    if (!(fabsf(y.y) <= 3.402823466e38f)) acc[c + 1] += y.y;
+                                    acc2[c / 2] = add2(acc2[c / 2], two(fabsf(y.x) <= 3.402823466e38f ? 0.0f : y.x,
+                                                                        fabsf(y.y) <= 3.402823466e38f ? 0.0f : y.y));
                                 }
                             }
                         }
@@ -876,26 +1015,76 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                     }
                 }
                 tc::tc_fence_before();
-                mbar_arrive(bar(fx.o_empty[b]));
+                mbar_arrive(bar(fx.o_empty[ob]));
             }
             if (!ok || !(ok = warp_wait(bar(fx.l_bar[seg & 1]), (seg >> 1) & 1))) break;
-            if (row < g->rows) {
-                const float l = fx.l[seg & 1][0][row] + fx.l[seg & 1][1][row];
-                if (g->part < 0) {
-                    const int node = (g->r0 + row) / G, h = g->r0 + row - node * G;
-                    T *o = out + ((long)(g->first + node) * a.NH + g->kvh * G + h) * D + half * CW;
-                    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            float acc[CW];
 #pragma unroll
-                    for (int c = 0; c < CW; c += 8) store8(o + c, acc + c, l == 0.0f, inv);
-                } else {
-                    const size_t at = ((size_t)blockIdx.x * 2 + g->part) * kRows + row;
-#pragma unroll
-                    for (int c = 0; c < CW; c += 4)
-                        *reinterpret_cast<float4 *>(ws.acc + at * D + half * CW + c) =
-                            make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
-                    if (half == 0) ws.ml[at] = make_float2(fx.m[seg & 1][row], l);
-                }
+            for (int c = 0; c < CW / 2; ++c) {
+                const float2 v = parts(acc2[c]);
+                acc[2 * c] = v.x;
+                acc[2 * c + 1] = v.y;
             }
+            const float (*lp)[kRows] = fx.l[seg & 1];
+            const float *mp = fx.m[seg & 1];
+            const int node = (sg.r0 + r) / G, h = sg.r0 + r - node * G;
+            T *o = out + ((long)(sg.first + node) * a.NH + sg.kvh * G + h) * D + half * CW;
+            const int part = sg.part;
+            const size_t at = ((size_t)blockIdx.x * 2 + max(part, 0)) * kRows + r;
+            float m = mp[r], l = lp[0][r] + lp[1][r];
+            if constexpr (cap == kRows) {
+                if (r < sg.rows) {
+                    if (part < 0) {
+                        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+                        for (int c = 0; c < CW; c += 8) store8(o + c, acc + c, l == 0.0f, inv);
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < CW; c += 4)
+                            *reinterpret_cast<float4 *>(ws.acc + at * D + half * CW + c) =
+                                make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+                    }
+                }
+            } else {
+                // the blocks of a row are added, 16 values at a time; each of its
+                // threads has a share of them
+                constexpr int nb = kRows / cap, share = 16 / nb;
+                const int mine = row / cap;
+#pragma unroll
+                for (int b = 1; b < nb; ++b) m = fmaxf(m, mp[b * cap + r]);
+                l = 0.0f;
+                for (int b = 0; b < nb; ++b) {
+                    const float mb = mp[b * cap + r];
+                    l += (lp[0][b * cap + r] + lp[1][b * cap + r]) * (mb == m ? 1.0f : ex2(mb - m));
+                }
+                const float f = mp[row] == m ? 1.0f : ex2(mp[row] - m), inv = l == 0.0f ? 0.0f : 1.0f / l;
+                auto meet = [&] {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(fx.block_bar[half]));
+                    return ok = warp_wait(bar(fx.block_bar[half]), meets++ & 1);
+                };
+#pragma unroll
+                for (int c = 0; c < CW; c += 16) {
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4)
+                        *reinterpret_cast<float4 *>(&fx.blocks[half][row][e]) =
+                            make_float4(acc[c + e] * f, acc[c + e + 1] * f, acc[c + e + 2] * f, acc[c + e + 3] * f);
+                    if (!meet()) break;
+                    if (r < sg.rows)
+                        for (int e = mine * share; e < (mine + 1) * share; e += 4) {
+                            float4 v = *reinterpret_cast<const float4 *>(&fx.blocks[half][r][e]);
+                            for (int b = 1; b < nb; ++b) {
+                                const float4 w = *reinterpret_cast<const float4 *>(&fx.blocks[half][b * cap + r][e]);
+                                v = make_float4(v.x + w.x, v.y + w.y, v.z + w.z, v.w + w.w);
+                            }
+                            if (part < 0) store4(o + c + e, v, l == 0.0f, inv);
+                            else *reinterpret_cast<float4 *>(ws.acc + at * D + half * CW + c + e) = v;
+                        }
+                    if (!meet()) break;
+                }
+                if (!ok) break;
+            }
+            if (part >= 0 && half == 0 && row < sg.rows) ws.ml[at] = make_float2(m, l);
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(fx.seg_done[seg & 1]));
             done();
@@ -922,24 +1111,28 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                 if (!(ok = warp_wait(bar(fx.v_full[vt.slot]), vt.parity))) break;
                 for (int w = 0; w < 4; ++w) {
                     const int j = w * 32 + lane, t = t0 + j;
+                    unsigned char *vr = v_s + vt.slot * F::kSlot + j * 128;
+                    auto piece = [&](int ch) {
+                        return reinterpret_cast<uint4 *>(vr + (ch >> 3) * (kTile * 128) + (((ch & 7) ^ (j & 7)) << 4));
+                    };
                     bool bad = false;
-                    if (t >= ctx) {
-                        unsigned char *vr = v_s + vt.slot * F::kSlot + j * 128;
-#pragma unroll 4
-                        for (int ch = 0; ch < D / 8; ++ch) {
-                            uint4 *p = reinterpret_cast<uint4 *>(vr + (ch >> 3) * (kTile * 128) + (((ch & 7) ^ (j & 7)) << 4));
-                            if (t >= L) {
-                                *p = make_uint4(0, 0, 0, 0);
-                                continue;
+                    if (t0 + w * 32 >= L) {
+#pragma unroll
+                        for (int ch = 0; ch < D / 8; ++ch) *piece(ch) = make_uint4(0, 0, 0, 0);
+                    } else if (t0 + w * 32 + 31 >= ctx) {
+                        for (int c8 = 0; c8 < D / 8; c8 += 8) {
+                            uint4 v[8];
+#pragma unroll
+                            for (int ch = 0; ch < 8; ++ch) v[ch] = *piece(c8 + ch);
+#pragma unroll
+                            for (int ch = 0; ch < 8; ++ch) {
+                                if (t >= L) {
+                                    *piece(c8 + ch) = make_uint4(0, 0, 0, 0);
+                                } else if (t >= ctx && !(finite2<C>(v[ch].x) & finite2<C>(v[ch].y) & finite2<C>(v[ch].z) & finite2<C>(v[ch].w))) {
+                                    bad = true;
+                                    *piece(c8 + ch) = make_uint4(held2<C>(v[ch].x), held2<C>(v[ch].y), held2<C>(v[ch].z), held2<C>(v[ch].w));
+                                }
                             }
-                            uint4 v = *p;
-                            if (finite2<C>(v.x) & finite2<C>(v.y) & finite2<C>(v.z) & finite2<C>(v.w)) continue;
-                            bad = true;
-                            v.x = held2<C>(v.x);
-                            v.y = held2<C>(v.y);
-                            v.z = held2<C>(v.z);
-                            v.w = held2<C>(v.w);
-                            *p = v;
                         }
                     }
                     const uint32_t x = __ballot_sync(~0u, bad);
@@ -1033,19 +1226,36 @@ bool map_cache(CUtensorMap *m, const void *base, uint64_t rows, int D, int box, 
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Room for the rows that a tile has at most; the rest of shared memory in slots.
+// The queries as [rows][heads][values]; a box is 128 bytes of each head of a key
+// head's group, of as many rows as a tile takes.
+bool map_queries(CUtensorMap *m, const TreeArgs &a, size_t bytes) {
+    const EncodeTiled enc = encode_fn();
+    if (!enc) return false;
+    const int G = a.NH / a.NKV;
+    cuuint64_t dims[3] = {(cuuint64_t)a.D, (cuuint64_t)a.NH, (cuuint64_t)a.T};
+    // (of one row, the distance to the next is never used, but has to be one)
+    const cuuint64_t row = (cuuint64_t)(a.T > 1 ? a.q_stride : (long)a.NH * a.D) * bytes;
+    cuuint64_t strides[2] = {(cuuint64_t)a.D * bytes, row};
+    cuuint32_t bx[3] = {(cuuint32_t)(128 / bytes), (cuuint32_t)G, (cuuint32_t)(kRows / G)};
+    cuuint32_t es[3] = {1, 1, 1};
+    const CUtensorMapDataType t = bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                  : a.dtype == QVL_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    return enc(m, t, 3, const_cast<void *>(a.q), dims, strides, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int D>
 Layout layout_for(const TreeArgs &a) {
     using F = Conf<T, D>;
     Layout ly{};
-    const long qrows = (long)a.max_nodes * (a.NH / a.NKV);
-    ly.rows = qrows <= 32 ? 32 : qrows <= 64 ? 64 : kRows;
-    ly.q_bytes = ly.rows * D * 2;
     ly.words = (a.max_nodes + 31) / 32;
-    ly.box = 16;
-    while (ly.box < kTile && a.P % (2 * ly.box) == 0) ly.box *= 2;
-    // (the MMA reads 128 rows of Q whatever there is room for: slots lie behind it)
-    const int rest = (((int)sizeof(Fixed) + 1023) & ~1023) + F::kQHalves * ly.q_bytes + 2 * a.max_nodes * ly.words * 4;
+    ly.box_log2 = 4;
+    while ((1 << ly.box_log2) < kTile && a.P % (2 << ly.box_log2) == 0) ++ly.box_log2;
+    ly.box = 1 << ly.box_log2;
+    ly.all = (1u << ((kTile >> ly.box_log2) * (D / 64))) - 1u;
+    const int G = a.NH / a.NKV;
+    ly.q_rows = kRows / G * G;
+    const int rest = (((int)sizeof(Fixed) + 1023) & ~1023) + 2 * a.max_nodes * ly.words * 4;
     const int slots = std::min(2 * F::kMaxRing, (227 * 1024 - rest) / F::kSlot);
     ly.nk = slots / 2;
     ly.nv = slots - ly.nk;
@@ -1053,19 +1263,20 @@ Layout layout_for(const TreeArgs &a) {
     return ly;
 }
 
-template <typename T, typename C, int D>
-cudaError_t launch_d(const TreeArgs &a, cudaStream_t st) {
+template <typename T, typename C, int D, int CAP>
+cudaError_t launch_cap(const TreeArgs &a, cudaStream_t st) {
     const Layout ly = layout_for<T, D>(a);
-    CUtensorMap mk, mv;
+    CUtensorMap mk, mv, mq;
     const uint64_t rows = (uint64_t)a.num_pages * a.NKV * a.P;
     const bool bf = a.kv_dtype == QVL_DTYPE_BF16;
-    if (!map_cache(&mk, a.k_pages, rows, D, ly.box, bf) || !map_cache(&mv, a.v_pages, rows, D, ly.box, bf))
+    if (!map_cache(&mk, a.k_pages, rows, D, ly.box, bf) || !map_cache(&mv, a.v_pages, rows, D, ly.box, bf) ||
+        !map_queries(&mq, a, sizeof(T)))
         return cudaErrorInvalidValue;
     // no more CTAs than there can be units
     const long qrows = (long)a.max_nodes * (a.NH / a.NKV);
-    const long units = (long)a.S * a.NKV * ((qrows + kRows - 1) / kRows) * (((long)a.max_ctx + kTile - 1) / kTile);
+    const long units = (long)a.S * a.NKV * ((qrows + ly.q_rows - 1) / ly.q_rows) * (((long)a.max_ctx + kTile - 1) / kTile);
     const int ctas = (int)(units < kSMs ? units : kSMs);
-    auto kern = tree_tc_kernel<T, C, D>;
+    auto kern = tree_tc_kernel<T, C, D, CAP>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ly.smem);
     if (e != cudaSuccess) return e;
     cudaLaunchAttribute attr[1];
@@ -1078,12 +1289,18 @@ cudaError_t launch_d(const TreeArgs &a, cudaStream_t st) {
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kern, mk, mv, a, ly);
+    e = cudaLaunchKernelEx(&cfg, kern, mk, mv, mq, a, ly);
     if (e != cudaSuccess || ctas == 1) return e;
     cfg.gridDim = dim3(ctas, (unsigned)((std::min(qrows, (long)kRows) + 7) / 8));
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
     return cudaLaunchKernelEx(&cfg, tree_join_kernel<T, D>, a, ctas);
+}
+// Rows of a request that has max_nodes: up to 32 or 64 go in blocks.
+template <typename T, typename C, int D>
+cudaError_t launch_d(const TreeArgs &a, cudaStream_t st) {
+    const int rows = a.max_nodes * (a.NH / a.NKV);
+    return rows <= 32 ? launch_cap<T, C, D, 32>(a, st) : rows <= 64 ? launch_cap<T, C, D, 64>(a, st) : launch_cap<T, C, D, 128>(a, st);
 }
 template <typename T, typename C>
 cudaError_t launch_t(const TreeArgs &a, cudaStream_t st) {
