@@ -22,8 +22,8 @@
 //   TMA      cuts the stretch into segments, finds the pages, fills a ring of slots for K
 //            and one for V (a slot: 128 positions, 128-byte swizzle); a segment's Q goes
 //            through the K ring ahead of its keys
-//   MMA      S = Q K^T [128 rows, 128 positions], O = P V [128 rows, D], one thread;
-//            Q, S, P (over S) and O in tensor memory, so that shared memory, whose
+//   MMA      S = Q K^T [128 rows, 128 positions], O = P V [128 rows, D], a thread each, so
+//            that one has its next product ready while the other's is under way.  Q, S, P (over S) and O in tensor memory, so that shared memory, whose
 //            bandwidth the products would need most of otherwise, is read for K and V alone
 //   softmax  two warpgroups, half of a tile's positions each; thread = row, so that maximum
 //            and sum need one exchange with the partner warp.  The maximum is left as it is
@@ -60,8 +60,8 @@ namespace {
 constexpr int kTile = 128;              // positions per tile
 constexpr int kRows = 128;              // query rows per tile
 constexpr int kSMs = 148;
-constexpr int kThreads = 19 * 32;       // 96 registers each
-constexpr int kSumWarp = 8, kTmaWarp = 16, kMmaWarp = 17;           // the fixer is the last one
+constexpr int kThreads = 20 * 32;       // 96 registers each
+constexpr int kSumWarp = 8, kTmaWarp = 16, kScoreWarp = 17, kOutWarp = 18;          // the fixer is the last one
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kPBias = 8.0f;          // p is held times 2^8: its low half stays normal
 
@@ -221,7 +221,8 @@ __device__ __forceinline__ int context(const TreeArgs &a, int s, int n, int &ctx
 }
 struct Request {
     int first, n, ctx, L, tiles, row_tiles;
-    long units;
+    // A pair (key head, tile of rows) has `begin` units ahead of its tiles.
+    __device__ __forceinline__ long units(int NKV, int begin) const { return (long)(tiles + begin) * row_tiles * NKV; }
 };
 __device__ __forceinline__ Request request_of(const TreeArgs &a, int s) {
     Request r;
@@ -230,7 +231,6 @@ __device__ __forceinline__ Request request_of(const TreeArgs &a, int s) {
     r.tiles = (r.L + kTile - 1) / kTile;
     const int per = kRows / (a.NH / a.NKV);     // whole nodes of a tile of rows
     r.row_tiles = (r.n + per - 1) / per;
-    r.units = (long)r.tiles * r.row_tiles * a.NKV;
     return r;
 }
 // A range of the tiles of one pair.  part: -1 whole pair; otherwise the place in
@@ -256,6 +256,7 @@ struct Conf {
 struct Layout {
     int nk, nv;         // slots for K and for V
     int words;          // of a node's ancestors
+    int anc_bytes;
     int box, box_log2;  // positions per TMA box
     uint32_t all;       // a bit for each box of a tile (and half of D)
     int q_rows;         // query rows of a tile: whole nodes
@@ -269,15 +270,12 @@ struct Fixed {
     float m[2][kRows];              // maxima, by segment
     float px[2][2][kRows];          // maxima of a tile's halves, by tile and warpgroup
     float qmax[2][kRows];           // maxima of a query row's halves
-    float blocks[2][kRows][20];     // 16 values of each block's rows, to be added, by half of D
     Segment seg[4];
-    uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], p_ready[2], o_full[2], o_empty[2], x_bar[2][8], q_full,
+    uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], s_free[2], p_ready[2], o_full[2], o_empty[2], x_bar[2][8], q_full,
         q_empty, anc_full[2], seg_full[4], seg_empty[4], l_bar[2], seg_done[2], qmax_bar, block_bar[2], fix_ask, fix_done;
     uint32_t valid[8];              // boxes of a tile that exist, by tile
     uint32_t bad[8][4];             // positions with values held back, by tile
     uint32_t moved[4][4];           // some maximum moved, by tile and warp
-    long range[3];                  // the stretch's request, offset in it, length
-    long wsum[kThreads / 32];
     uint32_t tmem;
     int off;
 };
@@ -333,7 +331,7 @@ __device__ __forceinline__ bool stage_queries(const TreeArgs &a, Fixed &fx, cons
     // values [c, c + V) of the half
     auto load = [&](int c, float (&x)[V]) {
         const int byte = (half * H + c) * (int)sizeof(T), chunk = byte >> 7;
-        const unsigned char *p = slot[chunk / (F::kSlot / 16384)] + chunk % (F::kSlot / 16384) * 16384;
+        const unsigned char *p = (chunk < F::kSlot / 16384 ? slot[0] : slot[1]) + chunk % (F::kSlot / 16384) * 16384;
         const uint4 v = *reinterpret_cast<const uint4 *>(p + src * 128 + ((((byte >> 4) & 7) ^ (src & 7)) << 4));
         const T *t = reinterpret_cast<const T *>(&v);
 #pragma unroll
@@ -342,7 +340,7 @@ __device__ __forceinline__ bool stage_queries(const TreeArgs &a, Fixed &fx, cons
     float f = qmul < 0.0f ? -1.0f : 1.0f, cs = fabsf(qmul);
     if constexpr (F::kSplitQ) {
         float mx = 0.0f;
-#pragma unroll
+#pragma unroll 4
         for (int c = 0; c < H; c += V) {
             float x[V];
             load(c, x);
@@ -361,7 +359,7 @@ __device__ __forceinline__ bool stage_queries(const TreeArgs &a, Fixed &fx, cons
         f = __uint_as_float((uint32_t)min(254, 263 - ex) << 23);
         cs = __uint_as_float((uint32_t)(ex - 9) << 23);
     }
-#pragma unroll
+#pragma unroll 1
     for (int c = 0; c < H; c += 16) {
         uint32_t hi[8], lo[8];
 #pragma unroll
@@ -460,6 +458,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
     unsigned char *k_s = smem + kHead;                              // slots of K, of V
     unsigned char *v_s = k_s + ly.nk * F::kSlot;
     uint32_t *anc_s = reinterpret_cast<uint32_t *>(v_s + ly.nv * F::kSlot);     // [2][node][words], by segment
+    // the blocks' sums, to be added: [half of D][row][pitch]
+    constexpr int kPitch = D / 2 + 4;
+    float *blocks_s = reinterpret_cast<float *>(v_s + ly.nv * F::kSlot + ly.anc_bytes);
     auto bar = [](uint64_t &b) { return tc::smem_u32(&b); };
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -472,10 +473,11 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             tc::mbar_init(bar(fx.v_full[i]), 1);
             tc::mbar_init(bar(fx.v_empty[i]), 1);
             tc::mbar_init(bar(fx.seg_full[i]), 1);
-            tc::mbar_init(bar(fx.seg_empty[i]), 18);
+            tc::mbar_init(bar(fx.seg_empty[i]), 19);
         }
         for (int i = 0; i < 2; ++i) {
             tc::mbar_init(bar(fx.s_full[i]), 1);
+            tc::mbar_init(bar(fx.s_free[i]), 1);
             tc::mbar_init(bar(fx.p_ready[i]), 256);
             tc::mbar_init(bar(fx.o_full[i]), 1);
             tc::mbar_init(bar(fx.o_empty[i]), 256);
@@ -496,59 +498,13 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
         tc::prefetch_tmap(&tm_v);
         tc::prefetch_tmap(&tm_q);
     }
-    if (warp == kMmaWarp) {
+    if (warp == kScoreWarp) {
         tc::tmem_alloc(tc::smem_u32(&fx.tmem), kTmCols);
         tc::tmem_relinquish();
     }
     pdl_wait();
     if (tid == 0) fx.off = *reinterpret_cast<volatile int *>(&g_tree_timeout);
 
-    // this CTA's stretch of the units
-    {
-        const int per = (a.S + kThreads - 1) / kThreads;
-        const int s0 = min(tid * per, a.S), s1 = min(s0 + per, a.S);
-        long mine = 0;
-        for (int s = s0; s < s1; ++s) mine += request_of(a, s).units;
-        long inc = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long up = __shfl_up_sync(~0u, inc, o);
-            if (lane >= o) inc += up;
-        }
-        if (lane == 31) fx.wsum[warp] = inc;
-        if (tid == 0) fx.range[2] = 0;
-        __syncthreads();
-        long before = inc - mine, total = 0;
-#pragma unroll 1
-        for (int w = 0; w < kThreads / 32; ++w) {
-            const long v = fx.wsum[w];
-            if (w < warp) before += v;
-            total += v;
-        }
-        // (fewer units than CTAs: the last CTAs have none, so that a pair's parts
-        // are in consecutive CTAs)
-        const long ctas = min((long)gridDim.x, max(total, 1l)), me = blockIdx.x;
-        long each, more;
-        if (total < 1l << 31) {
-            each = (uint32_t)total / (uint32_t)ctas;
-            more = (uint32_t)total % (uint32_t)ctas;
-        } else {
-            each = total / ctas;
-            more = total % ctas;
-        }
-        const long lo = min(each * me + min(me, more), total), hi = min(lo + each + (me < more ? 1 : 0), total);
-        if (lo < hi && before <= lo && lo < before + mine) {
-            int s = s0;
-            long u = request_of(a, s).units;
-            while (before + u <= lo) {
-                before += u;
-                u = request_of(a, ++s).units;
-            }
-            fx.range[0] = s;
-            fx.range[1] = lo - before;
-            fx.range[2] = hi - lo;
-        }
-    }
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
@@ -570,8 +526,55 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
 
     if (warp == kTmaWarp) {
         // ---- segments, pages and loads ----
-        int s = (int)fx.range[0];
-        long off = fx.range[1], left = ok ? fx.range[2] : 0;
+        // this CTA's stretch of all units: [lo, hi), found among the requests 32 at a time
+        long tiles = 0, pairs = 0;
+        for (int x = lane; x < a.S; x += 32) {
+            const Request r = request_of(a, x);
+            tiles += (long)r.tiles * r.row_tiles * a.NKV;
+            pairs += (long)r.row_tiles * a.NKV;
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            tiles += __shfl_xor_sync(~0u, tiles, o);
+            pairs += __shfl_xor_sync(~0u, pairs, o);
+        }
+        // What a pair costs beside its tiles, in tiles: about four where blocks have to be
+        // added and tiles are quick, one otherwise (32 requests of up to 16 nodes over 4096:
+        // 95 us with 0, 93 with 1, 85 with 2, 81 with 4; 12 of 132 rows over 6000: 55, 54,
+        // 55, 57).  Where there are fewer tiles than CTAs, each tile gets its own.
+        const int begin = tiles > gridDim.x ? (CAP < kRows ? 4 : 1) : 0;
+        const long total = tiles + pairs * begin;
+        // (fewer units than CTAs: the last CTAs have none, so that a pair's parts
+        // are in consecutive CTAs)
+        const long ctas = min((long)gridDim.x, max(total, 1l)), me = blockIdx.x;
+        long each, more;
+        if (total < 1l << 31) {
+            each = (uint32_t)total / (uint32_t)ctas;
+            more = (uint32_t)total % (uint32_t)ctas;
+        } else {
+            each = total / ctas;
+            more = total % ctas;
+        }
+        const long lo = min(each * me + min(me, more), total), hi = min(lo + each + (me < more ? 1 : 0), total);
+        int s = 0;
+        long off = lo, left = ok ? hi - lo : 0;
+        for (int base = 0; left > 0; base += 32) {
+            long inc = base + lane < a.S ? request_of(a, base + lane).units(a.NKV, begin) : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long up = __shfl_up_sync(~0u, inc, o);
+                if (lane >= o) inc += up;
+            }
+            const uint32_t past = __ballot_sync(~0u, inc > off);
+            if (past) {
+                const int at = __ffs(past) - 1;
+                const long before = __shfl_sync(~0u, inc, max(at - 1, 0));
+                s = base + at;
+                off -= at ? before : 0;
+                break;
+            }
+            off -= __shfl_sync(~0u, inc, 31);
+        }
         Request rq{};
         if (left > 0) rq = request_of(a, s);
         if (lane < 2) ws.part[blockIdx.x * 2 + lane].rows = 0;
@@ -587,19 +590,24 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
         asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(once));
         while (ok) {
             Segment g{};
-            if (left > 0) {
-                while (off >= rq.units) {
-                    off -= rq.units;
+            while (left > 0) {
+                while (off >= rq.units(a.NKV, begin)) {
+                    off -= rq.units(a.NKV, begin);
                     rq = request_of(a, ++s);
                 }
-                // key head, then tile of rows
-                const int pair = off < 1l << 31 ? (int)((uint32_t)off / (uint32_t)rq.tiles) : (int)(off / rq.tiles);
+                // key head, then tile of rows, then the units of the pair
+                const int len = rq.tiles + begin;
+                const int pair = off < 1l << 31 ? (int)((uint32_t)off / (uint32_t)len) : (int)(off / len);
+                const int u0 = (int)(off - (long)pair * len), u1 = (int)min((long)u0 + left, (long)len);
+                off += u1 - u0;
+                left -= u1 - u0;
+                g.tile0 = max(u0 - begin, 0);
+                g.nt = max(u1 - begin, 0) - g.tile0;
+                if (g.nt <= 0) continue;                           // ended before the pair's first tile
                 g.s = s;
                 g.kvh = pair / rq.row_tiles;
                 g.r0 = (pair - g.kvh * rq.row_tiles) * ly.q_rows;
                 g.rows = min(ly.q_rows, rq.n * G - g.r0);
-                g.tile0 = (int)(off - (long)pair * rq.tiles);
-                g.nt = (int)min(left, (long)(rq.tiles - g.tile0));
                 g.ctx = rq.ctx;
                 g.L = rq.L;
                 g.first = rq.first;
@@ -608,9 +616,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                 g.part = starts && ends ? -1 : starts ? 1 : 0;
                 if (g.part >= 0 && lane == 0)
                     ws.part[blockIdx.x * 2 + g.part] = {g.first, g.kvh, g.r0, g.rows, starts, ends};
-                off += g.nt;
-                left -= g.nt;
+                break;
             }
+            g.nt = max(g.nt, 0);
             if (seg >= 4) ok = warp_wait(bar(fx.seg_empty[seg & 3]), ((seg >> 2) - 1) & 1);
             if (!ok) break;
             if (lane == 0) {
@@ -629,14 +637,24 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                                 (h * per + lane) * (128 / (int)sizeof(T)), g.kvh * G, g.first + g.r0 / G, bar(fx.k_full[kt.slot]));
             }
             if (!ok) break;
+            // rows of the cache that 32 boxes start at (those of several tiles), one a lane, a
+            // group ahead: behind the loads of K and V an answer takes microseconds
+            const int nb = kTile >> ly.box_log2, group = 32 / nb;
+            auto rows_of = [&](int k) {
+                const int t = (g.tile0 + k + lane / nb) * kTile + (lane % nb << ly.box_log2);
+                if (t >= g.L || k + lane / nb >= g.nt) return oob;
+                const int c = t / a.P;
+                const int pg = a.table[(size_t)g.s * a.maxp + c];
+                return pg >= 0 && pg < a.num_pages ? (int)(((long)pg * a.NKV + g.kvh) * a.P + (t - c * a.P)) : oob;
+            };
+            int ahead = rows_of(0), rows_now = 0;
             for (int k = 0; k < g.nt; ++k, ++i) {
-                const int t = (g.tile0 + k) * kTile + bx * ly.box;
-                int y = oob;
-                if (lane < lanes && t < g.L) {
-                    const int c = t / a.P;
-                    const int pg = a.table[(size_t)g.s * a.maxp + c];
-                    if (pg >= 0 && pg < a.num_pages) y = (int)(((long)pg * a.NKV + g.kvh) * a.P + (t - c * a.P));
+                if (k % group == 0) {
+                    rows_now = ahead;
+                    ahead = k + group < g.nt ? rows_of(k + group) : oob;
                 }
+                int y = __shfl_sync(~0u, rows_now, (k % group * nb + bx) & 31);
+                if (lane >= lanes) y = oob;
                 const uint32_t there = __ballot_sync(~0u, y != oob);
                 if (loads >= ly.nk && !(ok = warp_wait(bar(fx.k_empty[kt.slot]), kt.parity ^ 1))) break;
                 if (lane == 0) {
@@ -664,75 +682,62 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             for (int n = 0; n < min(loads, ly.nk); ++n) tc::mbar_wait(bar(fx.k_full[n]), (((loads - 1 - n) / ly.nk) & 1), nullptr);
             for (int n = 0; n < min(i, ly.nv); ++n) tc::mbar_wait(bar(fx.v_full[n]), (((i - 1 - n) / ly.nv) & 1), nullptr);
         }
-    } else if (warp == kMmaWarp) {
-        // ---- products: the scores of the tile after next behind each O.  One thread,
-        // which an issue holds until the tensor cores take it: what stands between
-        // two products is kept short ----
+    } else if (warp == kScoreWarp) {
+        // ---- scores.  Low halves first: what they add up to is small, and exact beside
+        // the roundings of the high halves' sums ----
         if (lane == 0) {
-            constexpr uint32_t id_s = idesc_16<C>(kTile, false), id_o = idesc_16<C>(D, true);
-            // descriptors: the address is their low end, in units of 16 bytes
-            const uint64_t kd = tc::sdesc_k_sw128(tc::smem_u32(k_s)), vd = sdesc_mn_sw128(tc::smem_u32(v_s), kTile * 128);
-            constexpr int OB = F::kOB;
-            int qseg = 0, qk = 0, qnt = 0, qi = 0;        // scores: segment, tile in it, its tiles, tile in all
-            bool more = ok, begun = false;
-            Turn kt, vt;
+            constexpr uint32_t id = idesc_16<C>(kTile, false);
+            const uint64_t kd = tc::sdesc_k_sw128(tc::smem_u32(k_s));     // the address is its low end, in units of 16 bytes
+            Turn kt;
             auto wait = [&](uint64_t &b, uint32_t parity) { return ok = tc::mbar_wait(bar(b), parity, &g_tree_timeout); };
-            // low halves first: what they add up to is small, and exact beside the
-            // roundings of the high halves' sums
-            auto scores = [&](bool must) {
-                if (!more) return;
-                if (!begun) {
-                    if (!wait(fx.seg_full[qseg & 3], (qseg >> 2) & 1)) return;
-                    qnt = *reinterpret_cast<volatile int *>(&fx.seg[qseg & 3].nt);
-                    if (qnt == 0) {
-                        more = false;
-                        return;
-                    }
-                    // (what is still on its way does not hold up an O that is due)
-                    if (!must && !tc::mbar_try_wait(bar(fx.q_full), qseg & 1)) return;
-                    if (!wait(fx.q_full, qseg & 1)) return;
-                    for (int h = 0; h < F::kQHalves; ++h, kt.step(ly.nk)) mbar_arrive(bar(fx.k_empty[kt.slot]));
-                    begun = true;
-                }
-                if (!must && !tc::mbar_try_wait(bar(fx.k_full[kt.slot]), kt.parity)) return;
-                if (!wait(fx.k_full[kt.slot], kt.parity)) return;
-                tc::tc_fence_after();
-                const uint64_t kb = kd + (uint32_t)(kt.slot * (F::kSlot >> 4));
-                const uint32_t d = tmem + (qi & 1) * kTile;
+            while (ok && wait(fx.seg_full[seg & 3], (seg >> 2) & 1)) {
+                const int nt = *reinterpret_cast<volatile int *>(&fx.seg[seg & 3].nt);
+                if (nt == 0 || !wait(fx.q_full, seg & 1)) break;
+                for (int h = 0; h < F::kQHalves; ++h, kt.step(ly.nk)) mbar_arrive(bar(fx.k_empty[kt.slot]));
+                for (int k = 0; k < nt; ++k, ++i) {
+                    const int b = i & 1;
+                    if (i >= 2 && !wait(fx.s_free[b], ((i >> 1) - 1) & 1)) break;
+                    if (!wait(fx.k_full[kt.slot], kt.parity)) break;
+                    tc::tc_fence_after();
+                    const uint64_t kb = kd + (uint32_t)(kt.slot * (F::kSlot >> 4));
+                    const uint32_t d = tmem + b * kTile;
 #pragma unroll
-                for (int l = F::kQHalves - 1; l >= 0; --l)
+                    for (int l = F::kQHalves - 1; l >= 0; --l)
 #pragma unroll
-                    for (int k = 0; k < D / 16; ++k)
-                        mma_ts(d, tmem + kTmQ + l * (D / 2) + k * 8, kb + ((k >> 2) * (kTile * 8) + (k & 3) * 2), id_s,
-                               l < F::kQHalves - 1 || k ? 1u : 0u);
-                tc::tc_commit(bar(fx.s_full[qi & 1]));
-                tc::tc_commit(bar(fx.k_empty[kt.slot]));
-                kt.step(ly.nk);
-                ++qi;
-                if (++qk == qnt) {
-                    tc::tc_commit(bar(fx.q_empty));
-                    qk = 0;
-                    begun = false;
-                    ++qseg;
+                        for (int c = 0; c < D / 16; ++c)
+                            mma_ts(d, tmem + kTmQ + l * (D / 2) + c * 8, kb + ((c >> 2) * (kTile * 8) + (c & 3) * 2), id,
+                                   l < F::kQHalves - 1 || c ? 1u : 0u);
+                    tc::tc_commit(bar(fx.s_full[b]));
+                    tc::tc_commit(bar(fx.k_empty[kt.slot]));
+                    kt.step(ly.nk);
                 }
-            };
+                if (!ok) break;
+                tc::tc_commit(bar(fx.q_empty));
+                mbar_arrive(bar(fx.seg_empty[seg & 3]));
+                ++seg;
+            }
+        }
+    } else if (warp == kOutWarp) {
+        // ---- outputs ----
+        if (lane == 0) {
+            constexpr uint32_t id = idesc_16<C>(D, true);
+            constexpr int OB = F::kOB;
+            const uint64_t vd = sdesc_mn_sw128(tc::smem_u32(v_s), kTile * 128);
+            Turn vt;
+            auto wait = [&](uint64_t &b, uint32_t parity) { return ok = tc::mbar_wait(bar(b), parity, &g_tree_timeout); };
             int fixes = 0;
             while (ok && wait(fx.seg_full[seg & 3], (seg >> 2) & 1)) {
                 const volatile Segment &sg = fx.seg[seg & 3];
                 const int nt = sg.nt, plain = max(0, sg.ctx / kTile - sg.tile0);      // tiles before the drafted ones
                 if (nt == 0) break;
                 for (int k = 0; k < nt; ++k, ++i) {
-                    const int b = i & 1;
+                    const int b = i & 1, ob = i % OB;
                     const bool tail = k >= plain;
-                    if (qi == i) scores(true);
-                    if (ok && qi == i + 1) scores(false);
-                    if (!ok) break;
                     // (the fixer is told one tile ahead: the slot of the tile's V then has its
                     // turn, and it waits for the load itself)
                     if (k == 0 && tail) mbar_arrive(bar(fx.fix_ask));
                     const bool ask = k + 1 < nt && k + 1 >= plain;
                     if (ask && !tail) mbar_arrive(bar(fx.fix_ask));
-                    const int ob = i % OB;
                     if (i >= OB && !wait(fx.o_empty[ob], (i / OB - 1) & 1)) break;
                     if (!wait(fx.v_full[vt.slot], vt.parity)) break;
                     if (tail && !wait(fx.fix_done, fixes++ & 1)) break;
@@ -745,8 +750,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                     for (int l = 1; l >= 0; --l)
 #pragma unroll
                         for (int c = 0; c < kTile / 16; ++c)
-                            mma_ts(d, pb + c * 16 + l * 8, vb + c * (2048 >> 4), id_o, l == 0 || c ? 1u : 0u);
+                            mma_ts(d, pb + c * 16 + l * 8, vb + c * (2048 >> 4), id, l == 0 || c ? 1u : 0u);
                     tc::tc_commit(bar(fx.o_full[ob]));
+                    tc::tc_commit(bar(fx.s_free[b]));
                     tc::tc_commit(bar(fx.v_empty[vt.slot]));
                     vt.step(ly.nv);
                 }
@@ -788,6 +794,12 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             for (int k = 0; k < nt; ++k, ++i) {
                 const int b = i & 1;
                 qt.step(ly.nk);
+                // the next segment's queries as soon as this one's last scores are made, so
+                // that its first ones are made beside this one's last probabilities
+                if (k == nt - 1) {
+                    queries(seg + 1);
+                    if (!ok) break;
+                }
                 if (!(ok = warp_wait(bar(fx.s_full[b]), (i >> 1) & 1))) break;
                 tc::tc_fence_after();
                 const int t0 = (sg.tile0 + k) * kTile + wg * 64, ctx = sg.ctx;
@@ -937,7 +949,6 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             if (wg == 0) fx.m[seg & 1][row] = m;
             mbar_arrive(bar(fx.l_bar[seg & 1]));
             if (lane == 0) mbar_arrive(bar(fx.seg_done[seg & 1]));
-            queries(seg + 1);
             done();
         }
     } else if (warp < kTmaWarp) {
@@ -1046,9 +1057,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                     }
                 }
             } else {
-                // the blocks of a row are added, 16 values at a time; each of its
-                // threads has a share of them
-                constexpr int nb = kRows / cap, share = 16 / nb;
+                // the blocks of a row are added; each of its threads has a share of the values
+                constexpr int nb = kRows / cap, share = CW / nb;
                 const int mine = row / cap;
 #pragma unroll
                 for (int b = 1; b < nb; ++b) m = fmaxf(m, mp[b * cap + r]);
@@ -1063,24 +1073,25 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                     if (lane == 0) mbar_arrive(bar(fx.block_bar[half]));
                     return ok = warp_wait(bar(fx.block_bar[half]), meets++ & 1);
                 };
+                float *mine_s = blocks_s + (half * kRows + row) * kPitch;
+                if (!meet()) break;                 // (the segment before this one is read)
 #pragma unroll
-                for (int c = 0; c < CW; c += 16) {
+                for (int c = 0; c < CW; c += 4)
+                    *reinterpret_cast<float4 *>(mine_s + c) = make_float4(acc[c] * f, acc[c + 1] * f, acc[c + 2] * f, acc[c + 3] * f);
+                if (!meet()) break;
+                if (r < sg.rows) {
+                    const float *from = blocks_s + (half * kRows + r) * kPitch;
+#pragma unroll 1
+                    for (int c = mine * share; c < (mine + 1) * share; c += 4) {
+                        float4 v = *reinterpret_cast<const float4 *>(from + c);
 #pragma unroll
-                    for (int e = 0; e < 16; e += 4)
-                        *reinterpret_cast<float4 *>(&fx.blocks[half][row][e]) =
-                            make_float4(acc[c + e] * f, acc[c + e + 1] * f, acc[c + e + 2] * f, acc[c + e + 3] * f);
-                    if (!meet()) break;
-                    if (r < sg.rows)
-                        for (int e = mine * share; e < (mine + 1) * share; e += 4) {
-                            float4 v = *reinterpret_cast<const float4 *>(&fx.blocks[half][r][e]);
-                            for (int b = 1; b < nb; ++b) {
-                                const float4 w = *reinterpret_cast<const float4 *>(&fx.blocks[half][b * cap + r][e]);
-                                v = make_float4(v.x + w.x, v.y + w.y, v.z + w.z, v.w + w.w);
-                            }
-                            if (part < 0) store4(o + c + e, v, l == 0.0f, inv);
-                            else *reinterpret_cast<float4 *>(ws.acc + at * D + half * CW + c + e) = v;
+                        for (int b = 1; b < nb; ++b) {
+                            const float4 w = *reinterpret_cast<const float4 *>(from + b * cap * kPitch + c);
+                            v = make_float4(v.x + w.x, v.y + w.y, v.z + w.z, v.w + w.w);
                         }
-                    if (!meet()) break;
+                        if (part < 0) store4(o + c, v, l == 0.0f, inv);
+                        else *reinterpret_cast<float4 *>(ws.acc + at * D + half * CW + c) = v;
+                    }
                 }
                 if (!ok) break;
             }
@@ -1109,6 +1120,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                 if (t0 + kTile <= ctx) continue;
                 if (!(ok = warp_wait(bar(fx.fix_ask), fixes++ & 1))) break;
                 if (!(ok = warp_wait(bar(fx.v_full[vt.slot]), vt.parity))) break;
+#pragma unroll 1
                 for (int w = 0; w < 4; ++w) {
                     const int j = w * 32 + lane, t = t0 + j;
                     unsigned char *vr = v_s + vt.slot * F::kSlot + j * 128;
@@ -1116,22 +1128,16 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                         return reinterpret_cast<uint4 *>(vr + (ch >> 3) * (kTile * 128) + (((ch & 7) ^ (j & 7)) << 4));
                     };
                     bool bad = false;
-                    if (t0 + w * 32 >= L) {
-#pragma unroll
-                        for (int ch = 0; ch < D / 8; ++ch) *piece(ch) = make_uint4(0, 0, 0, 0);
-                    } else if (t0 + w * 32 + 31 >= ctx) {
-                        for (int c8 = 0; c8 < D / 8; c8 += 8) {
-                            uint4 v[8];
-#pragma unroll
-                            for (int ch = 0; ch < 8; ++ch) v[ch] = *piece(c8 + ch);
-#pragma unroll
-                            for (int ch = 0; ch < 8; ++ch) {
-                                if (t >= L) {
-                                    *piece(c8 + ch) = make_uint4(0, 0, 0, 0);
-                                } else if (t >= ctx && !(finite2<C>(v[ch].x) & finite2<C>(v[ch].y) & finite2<C>(v[ch].z) & finite2<C>(v[ch].w))) {
-                                    bad = true;
-                                    *piece(c8 + ch) = make_uint4(held2<C>(v[ch].x), held2<C>(v[ch].y), held2<C>(v[ch].z), held2<C>(v[ch].w));
-                                }
+                    // (short code rather than fast: its first run waits for each line of it)
+                    if (t0 + w * 32 + 31 >= ctx) {
+#pragma unroll 1
+                        for (int ch = 0; ch < D / 8; ++ch) {
+                            const uint4 v = *piece(ch);
+                            if (t >= L) {
+                                *piece(ch) = make_uint4(0, 0, 0, 0);
+                            } else if (t >= ctx && !(finite2<C>(v.x) & finite2<C>(v.y) & finite2<C>(v.z) & finite2<C>(v.w))) {
+                                bad = true;
+                                *piece(ch) = make_uint4(held2<C>(v.x), held2<C>(v.y), held2<C>(v.z), held2<C>(v.w));
                             }
                         }
                     }
@@ -1147,7 +1153,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
     __syncwarp();
     tc::tc_fence_before();
     __syncthreads();
-    if (warp == kMmaWarp) tc::tmem_dealloc(tmem, kTmCols);
+    if (warp == kScoreWarp) tc::tmem_dealloc(tmem, kTmCols);
 }
 
 // Joins the parts of the pairs that more than one CTA worked on: weights
@@ -1244,7 +1250,7 @@ bool map_queries(CUtensorMap *m, const TreeArgs &a, size_t bytes) {
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int D>
+template <typename T, int D, int CAP>
 Layout layout_for(const TreeArgs &a) {
     using F = Conf<T, D>;
     Layout ly{};
@@ -1255,7 +1261,9 @@ Layout layout_for(const TreeArgs &a) {
     ly.all = (1u << ((kTile >> ly.box_log2) * (D / 64))) - 1u;
     const int G = a.NH / a.NKV;
     ly.q_rows = kRows / G * G;
-    const int rest = (((int)sizeof(Fixed) + 1023) & ~1023) + 2 * a.max_nodes * ly.words * 4;
+    ly.anc_bytes = (2 * a.max_nodes * ly.words * 4 + 15) & ~15;
+    // (3 + 3 slots where there is room measure as 2 + 2 do)
+    const int rest = (((int)sizeof(Fixed) + 1023) & ~1023) + ly.anc_bytes + (CAP < kRows ? 2 * kRows * (D / 2 + 4) * 4 : 0);
     const int slots = std::min(2 * F::kMaxRing, (227 * 1024 - rest) / F::kSlot);
     ly.nk = slots / 2;
     ly.nv = slots - ly.nk;
@@ -1265,7 +1273,7 @@ Layout layout_for(const TreeArgs &a) {
 
 template <typename T, typename C, int D, int CAP>
 cudaError_t launch_cap(const TreeArgs &a, cudaStream_t st) {
-    const Layout ly = layout_for<T, D>(a);
+    const Layout ly = layout_for<T, D, CAP>(a);
     CUtensorMap mk, mv, mq;
     const uint64_t rows = (uint64_t)a.num_pages * a.NKV * a.P;
     const bool bf = a.kv_dtype == QVL_DTYPE_BF16;
