@@ -32,6 +32,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 import numpy as np
 import torch
@@ -159,6 +160,7 @@ def load_library(path: str = LIB_PATH):
     L.qvl_tree_attention.argtypes = ([_P, _I, _Z, _P, _P, _I, _Z] + [_P] * 4 + [_Z, _Z, _I, _I, ctypes.c_float, _P,
                                      ctypes.POINTER(AttnDims), _P, _Z, _P])
     L.qvl_token_logprobs.argtypes = [_P, _I, _Z, _P, _Z, _Z, _I] + [_P] * 5
+    L.qvl_internal_serving.argtypes = [_I, ctypes.c_char_p]
     _lib = L
     return L
 
@@ -584,7 +586,26 @@ def attention_q16(q, kv: PagedKV, seq_ids, positions, max_ctx, out, q_out, q_out
 
 
 # ------------------------------------------------- drafted and multimodal tokens
+# These are called for every layer of a step of a few tokens, where the host's
+# time counts: checks are a few attribute reads, and the arguments cross the C ABI as
+# one buffer of 64-bit words.
 _FLOAT_DTYPES = {torch.float32: DTYPE_FP32, torch.float16: DTYPE_FP16, torch.bfloat16: DTYPE_BF16}
+_PLAN, _ROPE, _TREE, _LOGPROBS = range(4)
+_WORDS = (struct.Struct("<17q"), struct.Struct("<26qd2q"), struct.Struct("<15qd5q"), struct.Struct("<12q"))
+_serving = None
+
+
+def _call(op: int, what: str, *words) -> None:
+    global _serving
+    if _serving is None:
+        _serving = load_library().qvl_internal_serving
+    rc = _serving(op, _WORDS[op].pack(*words))
+    if rc:
+        _check(rc, what)
+
+
+def _raw_stream(stream) -> int:
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()) if stream is None else stream.cuda_stream
 
 
 def _dtype(t: torch.Tensor) -> int:
@@ -594,31 +615,28 @@ def _dtype(t: torch.Tensor) -> int:
     return d
 
 
-def _i32(t: torch.Tensor, n: int | None = None, what: str = "index") -> int:
-    """Pointer of a contiguous int32 tensor of n values."""
-    if t.dtype != torch.int32 or (n is not None and t.numel() != n):
-        raise QvlError(f"{what}: expected int32{'' if n is None else f' [{n}]'}, got {t.dtype} {tuple(t.shape)}")
-    return _ptr(t)
-
-
-def _rows(t: torch.Tensor, shape, what: str) -> int:
-    """Pointer of a tensor of `shape` whose rows (all but the first dimension)
-    are contiguous; rows may lie apart."""
-    if not t.is_cuda:
-        raise QvlError(f"{what}: expected a CUDA tensor")
-    if tuple(t.shape) != tuple(shape):
-        raise QvlError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
-    st, want = t.stride(), 1
-    for i in range(t.dim() - 1, 0, -1):
-        if t.shape[i] != 1 and st[i] != want:
-            raise QvlError(f"{what}: each token's values must be contiguous")
-        want *= t.shape[i]
+def _addr(t: torch.Tensor, what: str) -> int:
+    if not (t.is_cuda and t.is_contiguous()):
+        raise QvlError(f"{what}: expected a contiguous CUDA tensor")
     return t.data_ptr()
 
 
-def _row_stride(t: torch.Tensor) -> int:
-    """Elements between rows (of one row: its width, whatever the stride says)."""
-    return t.stride(0) if t.shape[0] > 1 else t[0].numel() if t.shape[0] else t.stride(0)
+def _i32(t: torch.Tensor, n: int | None, what: str) -> int:
+    """Pointer of a contiguous int32 tensor (of n values)."""
+    if t.dtype is not torch.int32 or (n is not None and t.numel() != n):
+        raise QvlError(f"{what}: expected int32{'' if n is None else f' [{n}]'}, got {t.dtype} {tuple(t.shape)}")
+    return _addr(t, what)
+
+
+def _heads(t: torch.Tensor, T: int, H: int, D: int, what: str):
+    """(pointer, elements between rows) of a tensor [T, H, D] whose rows are
+    contiguous; rows may lie apart."""
+    if t.shape != (T, H, D) or not t.is_cuda:
+        raise QvlError(f"{what}: expected a CUDA tensor {(T, H, D)}, got {tuple(t.shape)}")
+    st = t.stride()
+    if (st[2] != 1 and D != 1) or (st[1] != D and H != 1):
+        raise QvlError(f"{what}: each token's values must be contiguous")
+    return t.data_ptr(), st[0] if T > 1 else H * D
 
 
 class PagePlan:
@@ -643,19 +661,19 @@ def plan_pages(old_lengths, new_lengths, page_table, free_pages, free_count, pag
     or no page left: plan.missing counts these tokens).  A plan that is not
     wanted is dropped by keeping the old lengths and the old free_count."""
     S = old_lengths.numel()
-    if page_table.dim() != 2 or page_table.shape[0] != S:
-        raise QvlError(f"page_table: expected {S} rows, got {tuple(page_table.shape)}")
+    shape = page_table.shape
+    if len(shape) != 2 or shape[0] != S:
+        raise QvlError(f"page_table: expected {S} rows, got {tuple(shape)}")
     if plan is None:
         plan = PagePlan(S, max_tokens, old_lengths.device)
     elif plan.n_seqs != S or plan.max_tokens != max_tokens:
         raise QvlError("plan was made for another number of requests or tokens")
     p = plan.buf.data_ptr()
     tok = p + 4 * (S + 3)
-    _check(load_library().qvl_plan_pages(
-        _i32(old_lengths, S, "old_lengths"), _i32(new_lengths, S, "new_lengths"), S, _i32(page_table, None, "page_table"),
-        page_size, page_table.shape[1], _i32(free_pages, None, "free_pages"), _i32(free_count, 1, "free_count"),
-        free_pages.numel(), p, p + 4, p + 8, tok, tok + 4 * max_tokens, tok + 8 * max_tokens, max_tokens,
-        _stream(stream)), "plan_pages")
+    _call(_PLAN, "plan_pages", _i32(old_lengths, S, "old_lengths"), _i32(new_lengths, S, "new_lengths"), S,
+          _i32(page_table, None, "page_table"), page_size, shape[1], _i32(free_pages, None, "free_pages"),
+          _i32(free_count, 1, "free_count"), free_pages.numel(), p, p + 4, p + 8, tok, tok + 4 * max_tokens,
+          tok + 8 * max_tokens, max_tokens, _raw_stream(stream))
     return plan
 
 
@@ -679,15 +697,15 @@ def _norm_weight(w, D, what):
     """(pointer, scales, dtype, group) of a norm weight: None, a float tensor [D]
     or (int8 [D], fp32 scales [D / group], group)."""
     if w is None:
-        return None, None, DTYPE_FP32, 0
+        return 0, 0, DTYPE_FP32, 0
     if isinstance(w, tuple):
         w, s, group = w
-        if w.dtype != torch.int8 or s.dtype != torch.float32 or w.numel() != D or s.numel() * group != D:
+        if w.dtype is not torch.int8 or s.dtype is not torch.float32 or w.numel() != D or s.numel() * group != D:
             raise QvlError(f"{what}: expected int8 [{D}] with fp32 scales [{D} / group]")
-        return _ptr(w), _ptr(s), DTYPE_INT8, group
+        return _addr(w, what), _addr(s, what), DTYPE_INT8, group
     if w.numel() != D:
         raise QvlError(f"{what}: expected {D} weights")
-    return _ptr(w), None, _dtype(w), 0
+    return _addr(w, what), 0, _dtype(w), 0
 
 
 def qknorm_mrope_kv_append(q, k, v, kv: PagedKV, slots, positions, axes, rope_cos, rope_sin, q_norm=None, k_norm=None,
@@ -700,33 +718,37 @@ def qknorm_mrope_kv_append(q, k, v, kv: PagedKV, slots, positions, axes, rope_co
     positions int32 [n_axes, T]; axes int32 [D/2] (mrope_axes); q_norm, k_norm:
     None, a float weight [D] or (int8 weight, fp32 scales, group).  Returns the
     normed, rotated queries (out, or a new tensor; out may be q)."""
-    T, NH, D = q.shape
     d = kv.dims
-    if (NH, D) != (d.num_heads, d.head_dim):
-        raise QvlError(f"q: expected {d.num_heads} heads of {d.head_dim}, got {NH} of {D}")
-    dt, kdt = _dtype(q), _dtype(kv.k)
-    if k.dtype != q.dtype or v.dtype != q.dtype or kv.v.dtype != kv.k.dtype:
+    T, NH, NKV, D, kp, vp = q.shape[0], d.num_heads, d.num_kv_heads, d.head_dim, kv.k, kv.v
+    dt = q.dtype
+    if k.dtype is not dt or v.dtype is not dt or vp.dtype is not kp.dtype:
         raise QvlError("q, k and v must have one type, and so must the cache's two halves")
     if out is None:
-        out = torch.empty((T, NH, D), dtype=q.dtype, device=q.device)
-    elif out.dtype != q.dtype or out.shape != q.shape:
+        out = torch.empty(q.shape, dtype=dt, device=q.device)
+    elif out.dtype is not dt or out.shape != q.shape:
         raise QvlError("out must have q's shape and type")
-    if positions.dim() != 2 or positions.shape[1] != T or axes.numel() != D // 2:
-        raise QvlError(f"positions: expected [axes, {T}], axes: [{D // 2}]")
-    if rope_cos.shape != rope_sin.shape or rope_cos.shape != (d.max_pos, D // 2) or rope_cos.dtype != torch.float32 or \
-            rope_sin.dtype != torch.float32:
-        raise QvlError(f"rope tables: expected fp32 [{d.max_pos}, {D // 2}]")
+    at = positions.shape
+    if len(at) != 2 or at[1] != T:
+        raise QvlError(f"positions: expected [axes, {T}], got {tuple(at)}")
+    table = (d.max_pos, D // 2)
+    if rope_cos.shape != table or rope_sin.shape != table or rope_cos.dtype is not torch.float32 or \
+            rope_sin.dtype is not torch.float32:
+        raise QvlError(f"rope tables: expected fp32 {table}")
     qw, qs, wd, g = _norm_weight(q_norm, D, "q_norm")
     kw, ks, wd2, g2 = _norm_weight(k_norm, D, "k_norm")
-    if (wd, g) != (wd2, g2):
+    if wd != wd2 or g != g2:
         raise QvlError("q_norm and k_norm must be of one kind")
-    shape = (T, d.num_kv_heads, D)
-    _check(load_library().qvl_qknorm_mrope_kv_append(
-        _rows(q, (T, NH, D), "q"), _rows(k, shape, "k"), _rows(v, shape, "v"), dt, _row_stride(q), _row_stride(k),
-        _row_stride(v), _ptr(out), _ptr(kv.k), _ptr(kv.v), kdt, kv.k.shape[0], _i32(slots, T, "slots"),
-        _i32(positions, None, "positions"), T, positions.shape[0], _i32(axes, None, "axes"), T, _ptr(rope_cos),
-        _ptr(rope_sin), qw, qs, kw, ks, wd, g, eps, ctypes.byref(d), _stream(stream)), "qknorm_mrope_kv_append")
+    qa, q_st = _heads(q, T, NH, D, "q")
+    ka, k_st = _heads(k, T, NKV, D, "k")
+    va, v_st = _heads(v, T, NKV, D, "v")
+    _call(_ROPE, "qknorm_mrope_kv_append", qa, ka, va, _dtype(q), q_st, k_st, v_st, _addr(out, "out"), _addr(kp, "k pages"),
+          _addr(vp, "v pages"), _dtype(kp), kp.shape[0], _i32(slots, T, "slots"), _i32(positions, None, "positions"), T,
+          at[0], _i32(axes, D // 2, "axes"), T, _addr(rope_cos, "rope_cos"), _addr(rope_sin, "rope_sin"), qw, qs, kw, ks, wd,
+          g, eps, ctypes.addressof(d), _raw_stream(stream))
     return out
+
+
+_tree_bytes: dict = {}
 
 
 def tree_attention(q, kv: PagedKV, ctx_lens, starts, parents, max_ctx, max_nodes, scale=None, out=None, workspace=None,
@@ -739,25 +761,24 @@ def tree_attention(q, kv: PagedKV, ctx_lens, starts, parents, max_ctx, max_nodes
     its parent's index in the request (-1: a root).  max_ctx bounds ctx_lens +
     nodes, max_nodes the nodes of a request (<= 256).  fp32 or fp16 queries
     over an fp16 cache, bf16 over bf16; rows that see nothing get zeros."""
-    T, NH, D = q.shape
     d = kv.dims
-    if (NH, D) != (d.num_heads, d.head_dim):
-        raise QvlError(f"q: expected {d.num_heads} heads of {d.head_dim}, got {NH} of {D}")
+    T, D, kp, vp, table = q.shape[0], d.head_dim, kv.k, kv.v, kv.page_table
     S = ctx_lens.numel()
-    if kv.page_table.shape[0] < S or kv.v.dtype != kv.k.dtype:
+    if table.shape[0] < S or vp.dtype is not kp.dtype:
         raise QvlError("the page table has fewer rows than there are requests, or the cache has two types")
     if out is None:
-        out = torch.empty((T, NH, D), dtype=q.dtype, device=q.device)
-    elif out.dtype != q.dtype or out.shape != q.shape:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.dtype is not q.dtype or out.shape != q.shape:
         raise QvlError("out must have q's shape and type")
-    L = load_library()
-    dims = ctypes.byref(d)
-    ws = _ws(workspace, q.device).get(L.qvl_tree_attention_workspace_bytes(S, T, max_ctx, max_nodes, dims))
-    _check(L.qvl_tree_attention(
-        _rows(q, (T, NH, D), "q"), _dtype(q), _row_stride(q), _ptr(kv.k), _ptr(kv.v), _dtype(kv.k), kv.k.shape[0],
-        _i32(kv.page_table, None, "page_table"), _i32(ctx_lens, S, "ctx_lens"), _i32(starts, S + 1, "starts"),
-        _i32(parents, T, "parents"), S, T, max_ctx, max_nodes, D ** -0.5 if scale is None else scale, _ptr(out), dims,
-        _ptr(ws), ws.numel(), _stream(stream)), "tree_attention")
+    nbytes = _tree_bytes.get(D)          # the head's size alone decides
+    if nbytes is None:
+        nbytes = _tree_bytes[D] = load_library().qvl_tree_attention_workspace_bytes(1, 1, 1, 1, ctypes.byref(d))
+    ws = _ws(workspace, q.device).get(nbytes)
+    qa, q_st = _heads(q, T, d.num_heads, D, "q")
+    _call(_TREE, "tree_attention", qa, _dtype(q), q_st, _addr(kp, "k pages"), _addr(vp, "v pages"), _dtype(kp), kp.shape[0],
+          _i32(table, None, "page_table"), _i32(ctx_lens, S, "ctx_lens"), _i32(starts, S + 1, "starts"),
+          _i32(parents, T, "parents"), S, T, max_ctx, max_nodes, D ** -0.5 if scale is None else scale, _addr(out, "out"),
+          ctypes.addressof(d), ws.data_ptr(), ws.numel(), _raw_stream(stream))
     return out
 
 
@@ -765,6 +786,7 @@ class TokenLogprobs:
     """What token_logprobs writes: logprobs, entropy [T], top_ids, top_logprobs [T, k]."""
 
     def __init__(self, rows: int, top_k: int, device):
+        self.rows, self.top_k = rows, top_k
         self.logprobs, self.entropy = torch.empty((2, rows), dtype=torch.float32, device=device)
         self.top_ids = torch.empty((rows, top_k), dtype=torch.int32, device=device)
         self.top_logprobs = torch.empty((rows, top_k), dtype=torch.float32, device=device)
@@ -775,12 +797,13 @@ def token_logprobs(logits, tokens, top_k=0, out: TokenLogprobs | None = None, st
     each row of logits [T, V] (fp32, fp16, bf16; rows may lie apart), the row's
     entropy in nats and its top_k alternatives (<= 64), ties to the lowest id."""
     T, V = logits.shape
+    if not logits.is_cuda or (V > 1 and logits.stride(1) != 1):
+        raise QvlError("logits: expected a CUDA tensor with contiguous rows")
     if out is None:
         out = TokenLogprobs(T, top_k, logits.device)
-    elif tuple(out.top_ids.shape) != (T, top_k):
+    elif out.rows != T or out.top_k != top_k:
         raise QvlError("out was made for another number of rows or alternatives")
-    _check(load_library().qvl_token_logprobs(
-        _rows(logits, (T, V), "logits"), _dtype(logits), max(_row_stride(logits), V), _i32(tokens, T, "tokens"), T, V,
-        top_k, out.logprobs.data_ptr(), out.entropy.data_ptr(), out.top_ids.data_ptr(), out.top_logprobs.data_ptr(),
-        _stream(stream)), "token_logprobs")
+    _call(_LOGPROBS, "token_logprobs", logits.data_ptr(), _dtype(logits), logits.stride(0) if T > 1 else V,
+          _i32(tokens, T, "tokens"), T, V, top_k, out.logprobs.data_ptr(), out.entropy.data_ptr(), out.top_ids.data_ptr(),
+          out.top_logprobs.data_ptr(), _raw_stream(stream))
     return out

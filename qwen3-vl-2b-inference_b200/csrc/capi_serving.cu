@@ -1,5 +1,6 @@
 // C ABI of the operators that serve drafted and multimodal tokens over the
 // paged cache: argument checks, then one launcher each (serving.cuh).
+#include <cstring>
 #include "serving.cuh"
 
 namespace {
@@ -163,6 +164,38 @@ int qvl_token_logprobs(const void *logits, int dtype, size_t stride, const int32
                              (int)vocab, top_k, dtype};
     QVL_CUDA_TRY(qvl::launch_token_logprobs(a, (cudaStream_t)stream));
     return QVL_OK;
+}
+
+// The same calls with their arguments as 64-bit words in the order of the
+// declarations (floats as doubles), the stream last: a binding converts one
+// buffer instead of three dozen arguments.
+int qvl_internal_serving(int op, const int64_t *w) {
+    auto p = [w](int i) { return reinterpret_cast<void *>(w[i]); };
+    auto i32 = [w](int i) { return reinterpret_cast<int32_t *>(w[i]); };
+    auto f32 = [w](int i) { return reinterpret_cast<float *>(w[i]); };
+    auto z = [w](int i) { return (size_t)w[i]; };
+    auto n = [w](int i) { return (int)w[i]; };
+    auto real = [w](int i) {
+        double d;
+        memcpy(&d, &w[i], sizeof(d));
+        return (float)d;
+    };
+    auto dims = [w](int i) { return reinterpret_cast<const qvl_attn_dims *>(w[i]); };
+    switch (op) {
+    case 0:
+        return qvl_plan_pages(i32(0), i32(1), z(2), i32(3), n(4), n(5), i32(6), i32(7), z(8), i32(9), i32(10), i32(11),
+                              i32(12), i32(13), i32(14), z(15), p(16));
+    case 1:
+        return qvl_qknorm_mrope_kv_append(p(0), p(1), p(2), n(3), z(4), z(5), z(6), p(7), p(8), p(9), n(10), z(11), i32(12),
+                                          i32(13), z(14), n(15), i32(16), z(17), f32(18), f32(19), p(20), f32(21), p(22),
+                                          f32(23), n(24), z(25), real(26), dims(27), p(28));
+    case 2:
+        return qvl_tree_attention(p(0), n(1), z(2), p(3), p(4), n(5), z(6), i32(7), i32(8), i32(9), i32(10), z(11), z(12),
+                                  n(13), n(14), real(15), p(16), dims(17), p(18), z(19), p(20));
+    case 3:
+        return qvl_token_logprobs(p(0), n(1), z(2), i32(3), z(4), z(5), n(6), f32(7), f32(8), i32(9), f32(10), p(11));
+    }
+    return QVL_ERR_INVALID;
 }
 
 }  // extern "C"

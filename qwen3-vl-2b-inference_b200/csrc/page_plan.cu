@@ -165,8 +165,10 @@ __global__ void __launch_bounds__(kThreads) plan_pages_kernel(PlanArgs a) {
 
 cudaError_t launch_plan_pages(const PlanArgs &a, cudaStream_t st) {
     const size_t smem = (size_t)3 * (a.S + 1) * sizeof(int);
-    cudaError_t e = cudaFuncSetAttribute(plan_pages_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
+    if (smem > 40 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(plan_pages_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+    }
     const int want = (a.max_tokens + kThreads - 1) / kThreads;
     plan_pages_kernel<<<want < 1 ? 1 : want > 148 ? 148 : want, kThreads, smem, st>>>(a);
     return cudaGetLastError();

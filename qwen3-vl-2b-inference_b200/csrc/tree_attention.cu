@@ -48,6 +48,7 @@
 // Every wait is bounded (2 s); one that gives up sets this kernel's timeout word,
 // and while it is set the kernel computes nothing (qvl_tc_timeout_status).
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 #include "serving.cuh"
 #include "tc_common.cuh"
@@ -1285,8 +1286,15 @@ cudaError_t launch_cap(const TreeArgs &a, cudaStream_t st) {
     const long units = (long)a.S * a.NKV * ((qrows + ly.q_rows - 1) / ly.q_rows) * (((long)a.max_ctx + kTile - 1) / kTile);
     const int ctas = (int)(units < kSMs ? units : kSMs);
     auto kern = tree_tc_kernel<T, C, D, CAP>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ly.smem);
+    static std::atomic<uint64_t> allowed{0};       // devices on which the kernel may use all shared memory
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
+    if (dev >= 64 || !((allowed.load(std::memory_order_relaxed) >> dev) & 1)) {
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
