@@ -7,259 +7,433 @@
 // A masked logit (-inf) adds nothing to any of the sums; a row of nothing but
 // -inf has log-probabilities of -inf and entropy 0.
 //
-// Memory bound.  A cluster of CTAs takes a row, each a slice of the
-// vocabulary with 16-byte loads; statistics and candidates meet in the first
-// CTA's shared memory.
+// Memory bound: one read of the logits, 16 bytes a load and four of them in flight a
+// thread.  A cluster of CTAs takes a row, each a slice of the vocabulary;
+// statistics and candidates meet in the first CTA's shared memory.  Measured: 512
+// rows of 151936 fp32 without alternatives 51 us (6.1 TB/s); 1024 rows of bf16 with 5 of
+// them 77 us (4.0 TB/s; 66 us without: one exponential a logit and its conversions take
+// the issue slots at two bytes a logit); 27 rows of fp32 with 20 of them 13.3 us.
 //
-// Candidates: the k-th largest of the threads' maxima over the first block
-// of a slice is a lower bound of the slice's k-th largest value (k values reach
-// it), so that only values that reach it can be among the alternatives: a few
-// hundred of a slice's tens of thousands, kept in shared memory and ranked
-// once.  A slice with more of them than the buffer holds (sorted or constant
-// rows) finds its k largest one after another instead, each with a pass over
-// the slice.
+// Sums: a thread's exponentials are taken against a maximum that moves only when a
+// logit passes it by 44, so that almost no load rescales anything.
+//
+// Candidates: the pass leaves each thread with the largest of its logits.  A thread whose
+// maximum is passed by k others has nothing among the alternatives; the logits of the
+// rest (about k of 512) are looked through once more, mostly in L2, by all threads.  To
+// know them without
+// sorting 512 values: with W warps and r = ceil(k / W), the smallest of the warps' r-th
+// largest maxima is reached by k maxima at least, so that only those that reach
+// it (about a hundred) are counted against one another.  What reaches it in the logits
+// of the threads that are left is kept in shared memory and ranked.  A slice
+// with more of that than the buffer holds (one value all over) finds its k largest
+// one after another instead, a pass each.
+#include <type_traits>
 #include <cooperative_groups.h>
 #include "serving.cuh"
 namespace cg = cooperative_groups;
 
 namespace qvl {
 namespace {
-constexpr int kThreads = 256;
+constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kCand = 1024;
 constexpr int kMaxCluster = 8;
+constexpr int kShare = 128;             // candidates that a slice may hand on unranked
 constexpr float kLog2e = 1.4426950408889634f;
 
-// (value, index) order of the alternatives: larger value first, then lower index.
-__device__ __forceinline__ bool before(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
+// Value and index as one number, larger where the alternative comes first: by value, then
+// by lower index (both zeros are one value).
+using Key = unsigned long long;
+__device__ __forceinline__ Key key_of(float v, int i) {
+    const uint32_t b = __float_as_uint(v + 0.0f);
+    return (Key)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | (uint32_t)~i;
+}
+__device__ __forceinline__ float value_of(Key k) {
+    const uint32_t b = (uint32_t)(k >> 32);
+    return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
+}
+__device__ __forceinline__ int index_of(Key k) { return (int)~(uint32_t)k; }
+// How many of keys[0, n) come before k; keys are 16-byte aligned, and what lies between n
+// and the next even number is 0.
+__device__ __forceinline__ int rank_of(const Key *keys, int n, Key k) {
+    int r = 0;
+#pragma unroll 4
+    for (int d = 0; d < n; d += 2) {
+        const ulonglong2 x = *reinterpret_cast<const ulonglong2 *>(keys + d);
+        r += (x.x > k) + (x.y > k);
+    }
+    return r;
+}
 
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float redux_max(float v) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// A reference m, z = sum e^(x - m), s = sum (x - m) e^(x - m).
 struct Stats {
-    float m, z, s;          // max, sum of e^(x - m), sum of x e^(x - m)
+    float m, z, s;
 };
-__device__ __forceinline__ float scale_of(float m, float mm) { return m == mm ? 1.0f : exp2f((m - mm) * kLog2e); }
-__device__ __forceinline__ Stats join(const Stats &a, const Stats &b) {
-    const float m = fmaxf(a.m, b.m);
-    const float fa = scale_of(a.m, m), fb = scale_of(b.m, m);
-    return {m, a.z * fa + b.z * fb, a.s * fa + b.s * fb};
+__device__ __forceinline__ Stats rebase(const Stats &a, float m) {
+    if (a.z == 0.0f || a.m == m) return {m, a.z, a.s};
+    const float d = a.m - m, f = ex2(d * kLog2e);
+    return {m, a.z * f, (a.s + a.z * d) * f};
 }
-__device__ __forceinline__ void take(Stats &t, float x) {
-    if (x > t.m) {
-        const float f = scale_of(t.m, x);
-        t.z *= f;
-        t.s *= f;
-        t.m = x;
+__device__ __forceinline__ Stats warp_join(const Stats &t) {
+    const float m = redux_max(t.z == 0.0f ? -INFINITY : t.m);
+    Stats r = rebase(t, m == -INFINITY ? 0.0f : m);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        r.z += __shfl_xor_sync(~0u, r.z, o);
+        r.s += __shfl_xor_sync(~0u, r.s, o);
     }
-    if (x != -INFINITY) {           // NaN stays in the sums
-        const float e = exp2f((x - t.m) * kLog2e);
-        t.z += e;
-        t.s += x * e;
-    }
+    return r;
 }
+// Two fp32 operations in one instruction: the sums are bound by issue next to memory.
+__device__ __forceinline__ uint64_t two(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 parts(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+// N logits (even); `top` is the largest of them.
+template <int N> __device__ __forceinline__ void take(Stats &t, const float (&x)[N], float top) {
+    if (top > t.m + 44.0f || t.z == 0.0f) t = rebase(t, top == -INFINITY ? 0.0f : top);
+    uint64_t z = two(t.z, 0.0f), s = two(t.s, 0.0f);
+    const uint64_t m = two(-t.m, -t.m), l = two(kLog2e, kLog2e);
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+        const uint64_t d = add2(two(x[e], x[e + 1]), m);
+        const float2 y = parts(mul2(d, l)), w = parts(d);
+        const uint64_t p = two(ex2(y.x), ex2(y.y));
+        z = add2(z, p);                     // (NaN stays in it)
+        s = fma2(p, two(fmaxf(w.x, -1000.0f), fmaxf(w.y, -1000.0f)), s);     // a masked logit: 0, not 0 * inf
+    }
+    t.z = parts(z).x + parts(z).y;
+    t.s = parts(s).x + parts(s).y;
+}
+template <typename T> struct Vec {
+    static constexpr int N = 16 / sizeof(T);
+    uint4 v;
+    __device__ __forceinline__ void unpack(float (&x)[N]) const {
+        const T *t = reinterpret_cast<const T *>(&v);
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] = to_f32(t[e]);
+    }
+    // The largest value; -inf where there is nothing but NaN.
+    __device__ __forceinline__ float largest() const {
+        float m;
+        if constexpr (sizeof(T) == 4) {
+            m = fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+        } else if constexpr (std::is_same<T, __half>::value) {
+            const __half2 *h = reinterpret_cast<const __half2 *>(&v);
+            const __half2 x = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+            m = __half2float(__hmax(__low2half(x), __high2half(x)));
+        } else {
+            const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&v);
+            const __nv_bfloat162 x = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+            m = __bfloat162float(__hmax(__low2bfloat16(x), __high2bfloat16(x)));
+        }
+        return m == m ? m : -INFINITY;
+    }
+};
 }  // namespace
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
-    constexpr int VE = 16 / sizeof(T);
-    __shared__ float cand_v[kCand];
-    __shared__ int cand_i[kCand];
-    __shared__ float top_v[kMaxTopK];
-    __shared__ int top_i[kMaxTopK];
-    __shared__ Stats wst[kThreads / 32];
+// kAhead: 16-byte loads of a thread in flight; kPerSM: CTAs on an SM.
+template <typename T, int kAhead, int kPerSM>
+__global__ void __launch_bounds__(kThreads, kPerSM) token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
+    constexpr int N = Vec<T>::N;
+    __shared__ __align__(16) Key cand[kCand + 2];
+    __shared__ __align__(16) Key all[kMaxCluster * kShare + 2];      // the first CTA's: everyone's candidates
+    __shared__ Stats wst[kWarps];
     __shared__ Stats cst;
-    __shared__ float tmax[kThreads];
-    __shared__ float tau_s, tok_x;
-    __shared__ int n_cand, n_top;
-    __shared__ float best_v[kThreads / 32];
-    __shared__ int best_i[kThreads / 32];
+    __shared__ float wtau[kWarps];
+    __shared__ float lse_s;
+    __shared__ float max_s[kThreads];
+    __shared__ int asked[kThreads];             // threads whose logits are looked through again
+    __shared__ int n_cand, n_max, n_asked;
+    __shared__ Key best[kWarps];
+    __shared__ int have[kMaxCluster + 1];
 
     cg::cluster_group cl = cg::this_cluster();
     const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
     const int row = blockIdx.x / C;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const T *x = reinterpret_cast<const T *>(a.logits) + (long)row * a.stride;
-    const int per = ((a.V + C - 1) / C + VE - 1) / VE * VE;
-    const int lo = min(rank * per, a.V), hi = min(lo + per, a.V);
+    // elements before the first 16-byte boundary, whole loads, and the rest; the first CTA
+    // takes what is not a whole load
+    const int head = min((int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T), a.V);
+    const int loads = (a.V - head) / N, tail = head + loads * N;
+    const int per = (loads + C - 1) / C, lo = min(rank * per, loads), hi = min(lo + per, loads);
+    const int loose = rank == 0 ? head + a.V - tail : 0;
+    const uint4 *xv = reinterpret_cast<const uint4 *>(x + head);
+    auto loose_at = [&](int i) { return i < head ? i : tail + i - head; };
 
+    pdl_launch_dependents();
     if (tid == 0) {
         n_cand = 0;
-        n_top = 0;
-        tau_s = -INFINITY;
+        n_max = 0;
+        n_asked = 0;
     }
-    // lower bound of the slice's k-th largest
-    float mx = -INFINITY;
-    for (int i = lo + tid; i < min(hi, lo + 16 * kThreads); i += kThreads) mx = fmaxf(mx, to_f32(x[i]));
-    tmax[tid] = mx;
-    __syncthreads();
-    if (a.k > 0 && a.k <= kThreads) {
-        int r = 0;
-        for (int i = 0; i < kThreads; ++i) r += before(tmax[i], i, mx, tid);
-        if (r == a.k - 1) tau_s = mx;
+    pdl_wait();
+    // no load: -inf, which weighs nothing
+    auto none = [] {
+        Vec<T> v;
+        T *t = reinterpret_cast<T *>(&v.v);
+#pragma unroll
+        for (int e = 0; e < N; ++e) t[e] = from_f32<T>(-INFINITY);
+        return v;
+    };
+    const float own = tid < loose ? to_f32(x[loose_at(tid)]) : -INFINITY;
+    float mx = own == own ? own : -INFINITY;
+    Stats st{0.0f, 0.0f, 0.0f};
+    if (tid < loose) {
+        const float f[2] = {own, -INFINITY};
+        take(st, f, mx);
     }
-    __syncthreads();
-    const float tau = tau_s;
-
-    Stats st{-INFINITY, 0.0f, 0.0f};
-    for (int i = lo + tid; i < hi; i += kThreads) {
-        const float v = to_f32(x[i]);
-        take(st, v);
-        if (a.k > 0 && v >= tau && v != -INFINITY) {
-            const int at = atomicAdd(&n_cand, 1);
-            if (at < kCand) {
-                cand_v[at] = v;
-                cand_i[at] = i;
-            }
+    for (int i = lo + tid; i < hi; i += kAhead * kThreads) {
+        Vec<T> v[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            if (i + u * kThreads < hi) v[u].v = __ldg(xv + i + u * kThreads);
+            else v[u] = none();
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            float f[N];
+            v[u].unpack(f);
+            const float top = v[u].largest();
+            take(st, f, top);
+            mx = fmaxf(mx, top);
         }
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const Stats b{__shfl_xor_sync(~0u, st.m, o), __shfl_xor_sync(~0u, st.z, o), __shfl_xor_sync(~0u, st.s, o)};
-        st = join(st, b);
-    }
+    st = warp_join(st);
     if (lane == 0) wst[warp] = st;
     __syncthreads();
-    if (tid == 0) {
-        Stats t = wst[0];
-        for (int w = 1; w < kThreads / 32; ++w) t = join(t, wst[w]);
-        cst = t;
+    if (warp == 0) {
+        st = warp_join(lane < kWarps ? wst[lane] : Stats{0.0f, 0.0f, 0.0f});
+        if (lane == 0) cst = st;
     }
-    const int nc = n_cand;
-    if (nc <= kCand) {
-        for (int c = tid; c < nc; c += kThreads) {
-            int r = 0;
-            const float v = cand_v[c];
-            const int i = cand_i[c];
-            for (int d = 0; d < nc; ++d) r += before(cand_v[d], cand_i[d], v, i);
-            if (r < a.k) {
-                top_v[r] = v;
-                top_i[r] = i;
+    int nc = 0;
+    if (a.k > 0) {
+        const int r = (a.k + kWarps - 1) / kWarps;
+        float t = -INFINITY, rest = mx;
+        for (int n = 0; n < r; ++n) {
+            t = redux_max(rest);
+            if (t == -INFINITY) break;
+            if (lane == __ffs(__ballot_sync(~0u, rest == t)) - 1) rest = -INFINITY;
+        }
+        if (lane == 0) wtau[warp] = t;
+        __syncthreads();
+        float tau = wtau[0];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) tau = fminf(tau, wtau[w]);
+        const bool in = mx >= tau && mx != -INFINITY;
+        if (in) max_s[atomicAdd(&n_max, 1)] = mx;
+        __syncthreads();
+        if (in) {
+            int passed = 0;
+#pragma unroll 8
+            for (int d = 0; d < n_max; ++d) passed += max_s[d] > mx;
+            if (passed < a.k) asked[atomicAdd(&n_asked, 1)] = tid;
+        }
+        __syncthreads();
+        auto offer = [&](float v, int i) {
+            if (v >= tau && v != -INFINITY) {
+                const int at = atomicAdd(&n_cand, 1);
+                if (at < kCand) cand[at] = key_of(v, i);
+            }
+        };
+        if (tid < loose) offer(own, loose_at(tid));
+        const int turns = (per + kThreads - 1) / kThreads;
+        for (int j = tid; j < n_asked * turns; j += kThreads) {
+            const int q = j / turns, i = lo + asked[q] + (j - q * turns) * kThreads;
+            if (i >= hi) continue;
+            Vec<T> w;
+            w.v = __ldg(xv + i);
+            if (w.largest() >= tau) {
+                float f[N];
+                w.unpack(f);
+#pragma unroll
+                for (int e = 0; e < N; ++e) offer(f[e], head + i * N + e);
             }
         }
-        if (tid == 0) n_top = min(nc, a.k);
-    } else {
-        float pv = INFINITY;
-        int pi = -1;
-        for (int r = 0; r < a.k; ++r) {
-            float bv = -INFINITY;
-            int bi = INT32_MAX;
-            for (int i = lo + tid; i < hi; i += kThreads) {
-                const float v = to_f32(x[i]);
-                if (v != -INFINITY && (v < pv || (v == pv && i > pi)) && before(v, i, bv, bi)) {
-                    bv = v;
-                    bi = i;
+        __syncthreads();
+        nc = n_cand;
+    }
+    if (nc > kCand) {
+        // one value after another
+        Key past = ~0ull;
+        int n = 0;
+        for (; n < a.k; ++n) {
+            Key b = 0;
+            auto look = [&](float w, int i) {
+                if (w > -INFINITY) {
+                    const Key k = key_of(w, i);
+                    if (k < past && k > b) b = k;
                 }
+            };
+            if (tid < loose) look(own, loose_at(tid));
+            for (int i = lo + tid; i < hi; i += kThreads) {
+                Vec<T> w;
+                w.v = __ldg(xv + i);
+                float f[N];
+                w.unpack(f);
+#pragma unroll
+                for (int e = 0; e < N; ++e) look(f[e], head + i * N + e);
             }
 #pragma unroll
-            for (int o = 16; o; o >>= 1) {
-                const float v = __shfl_xor_sync(~0u, bv, o);
-                const int i = __shfl_xor_sync(~0u, bi, o);
-                if (before(v, i, bv, bi)) {
-                    bv = v;
-                    bi = i;
-                }
-            }
-            if (lane == 0) {
-                best_v[warp] = bv;
-                best_i[warp] = bi;
-            }
+            for (int o = 16; o; o >>= 1) b = max(b, __shfl_xor_sync(~0u, b, o));
+            if (lane == 0) best[warp] = b;
             __syncthreads();
-            bv = best_v[0];
-            bi = best_i[0];
-            for (int w = 1; w < kThreads / 32; ++w)
-                if (before(best_v[w], best_i[w], bv, bi)) {
-                    bv = best_v[w];
-                    bi = best_i[w];
-                }
-            if (bi == INT32_MAX) break;
-            if (tid == 0) {
-                top_v[r] = bv;
-                top_i[r] = bi;
-                n_top = r + 1;
-            }
-            pv = bv;
-            pi = bi;
+            b = best[0];
+#pragma unroll
+            for (int w = 1; w < kWarps; ++w) b = max(b, best[w]);
             __syncthreads();
+            if (b == 0) break;
+            if (tid == 0) cand[n] = b;
+            past = b;
         }
+        nc = n;
+    } else if (nc > kShare) {
+        // (all candidates are read before the best are written over them)
+        if (tid < 2) cand[nc + tid] = 0;
+        __syncthreads();
+        Key mine[kCand / kThreads];
+        int at[kCand / kThreads];
+#pragma unroll
+        for (int u = 0; u < kCand / kThreads; ++u) {
+            const int c = tid + u * kThreads;
+            mine[u] = c < nc ? cand[c] : 0;
+            at[u] = c < nc ? rank_of(cand, nc, mine[u]) : kCand;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < kCand / kThreads; ++u)
+            if (at[u] < a.k) cand[at[u]] = mine[u];
+        nc = a.k;
     }
-    cl.sync();
+    __syncthreads();
+    if (tid == 0) n_cand = nc;
+    if (C > 1) cl.sync();
+    else __syncthreads();
     if (rank == 0) {
-        __shared__ int have[kMaxCluster + 1];
-        if (tid == 0) {
-            Stats t = cst;
-            int n = 0;
-            for (int c = 0; c < C; ++c) {
-                if (c) t = join(t, *cl.map_shared_rank(&cst, c));
-                have[c] = n;
-                n += *cl.map_shared_rank(&n_top, c);
+        if (warp == 0) {
+            const Stats t = warp_join(lane < C ? *cl.map_shared_rank(&cst, lane) : Stats{0.0f, 0.0f, 0.0f});
+            int upto = lane < C ? *cl.map_shared_rank(&n_cand, lane) : 0;
+#pragma unroll
+            for (int o = 1; o < kMaxCluster; o <<= 1) {
+                const int up = __shfl_up_sync(~0u, upto, o);
+                if (lane >= o) upto += up;
             }
-            have[C] = n;
-            const float lse = t.m == -INFINITY && t.z == 0.0f ? -INFINITY : t.m + logf(t.z);
-            const int tk = a.tokens[row];
-            float lp = 0.0f;
-            if (tk >= 0 && tk < a.V) {
-                const float v = to_f32(x[tk]);
-                lp = v == -INFINITY && t.z == t.z ? -INFINITY : v - lse;
+            if (lane < C) have[lane + 1] = upto;
+            if (lane == 0) {
+                have[0] = 0;
+                const float lz = logf(t.z), lse = t.z == 0.0f ? -INFINITY : t.m + lz;
+                const int tk = a.tokens[row];
+                float lp = 0.0f;
+                if (tk >= 0 && tk < a.V) {
+                    const float w = to_f32(x[tk]);
+                    // (the logits' own size does not round the difference)
+                    lp = w == -INFINITY && t.z == t.z ? -INFINITY : (w - t.m) - lz;
+                }
+                a.logprobs[row] = lp;
+                if (a.entropy) a.entropy[row] = t.z == 0.0f ? 0.0f : lz - t.s / t.z;
+                lse_s = lse;
+                cst = t;
             }
-            a.logprobs[row] = lp;
-            if (a.entropy) a.entropy[row] = t.z == 0.0f ? 0.0f : lse - t.s / t.z;
-            tok_x = lse;
         }
         __syncthreads();
         const int n = have[C];
-        const float lse = tok_x;
+        const float lse = lse_s, m = cst.m, lz = logf(cst.z);
         for (int e = tid; e < n; e += kThreads) {
             int c = 0;
             while (e >= have[c + 1]) ++c;
-            cand_v[e] = cl.map_shared_rank(top_v, c)[e - have[c]];
-            cand_i[e] = cl.map_shared_rank(top_i, c)[e - have[c]];
+            all[e] = cl.map_shared_rank(cand, c)[e - have[c]];
         }
+        if (tid < 2) all[n + tid] = 0;
         __syncthreads();
         for (int e = tid; e < n; e += kThreads) {
-            int r = 0;
-            for (int d = 0; d < n; ++d) r += before(cand_v[d], cand_i[d], cand_v[e], cand_i[e]);
-            if (r < a.k) {
-                a.top_ids[(long)row * a.k + r] = cand_i[e];
-                a.top_lp[(long)row * a.k + r] = cand_v[e] - lse;
+            const Key k = all[e];
+            const int at = rank_of(all, n, k);
+            if (at < a.k) {
+                a.top_ids[(long)row * a.k + at] = index_of(k);
+                a.top_lp[(long)row * a.k + at] = (value_of(k) - m) - lz;
             }
         }
         // fewer finite logits than alternatives: the lowest -inf ones follow
         if (n < a.k && warp == 0) {
-            int r = n;
-            for (int i0 = 0; i0 < a.V && r < a.k; i0 += 32) {
+            int at0 = n;
+            for (int i0 = 0; i0 < a.V && at0 < a.k; i0 += 32) {
                 const bool is = i0 + lane < a.V && to_f32(x[i0 + lane]) == -INFINITY;
                 const unsigned b = __ballot_sync(~0u, is);
-                const int at = r + __popc(b & ((1u << lane) - 1));
+                const int at = at0 + __popc(b & ((1u << lane) - 1));
                 if (is && at < a.k) {
                     a.top_ids[(long)row * a.k + at] = i0 + lane;
                     a.top_lp[(long)row * a.k + at] = lse == lse ? -INFINITY : lse;
                 }
-                r += __popc(b);
+                at0 += __popc(b);
             }
             // and then nothing is left but NaN
-            for (r += lane; r < a.k; r += 32) {
-                a.top_ids[(long)row * a.k + r] = -1;
-                a.top_lp[(long)row * a.k + r] = NAN;
+            for (at0 += lane; at0 < a.k; at0 += 32) {
+                a.top_ids[(long)row * a.k + at0] = -1;
+                a.top_lp[(long)row * a.k + at0] = NAN;
             }
         }
     }
-    cl.sync();
+    if (C > 1) cl.sync();           // (the first CTA reads the others' shared memory)
 }
 
 namespace {
 template <typename T>
 cudaError_t launch_t(const LogprobArgs &a, cudaStream_t st) {
+    // Slices of 2048 logits at least, and two CTAs per SM at most: what a CTA does beside
+    // its loads costs more than a shorter slice gives (128 rows of 151936 fp32, 20
+    // alternatives: 51 us with clusters of 8, 38 with 4, 33 with 2, 45 alone)
     int C = kMaxCluster;
-    while (C > 1 && a.V / C < 2048) C >>= 1;
+    while (C > 1 && (a.V / C < 2048 || (long)a.T * C > 2l * 148)) C >>= 1;
+    // One wave of CTAs: more loads in flight a thread; several: more CTAs on an SM, so that
+    // one's end goes on beside another's loads (27 rows of 151936 fp32: 14.5 and 19.3 us;
+    // 1024 of bf16: 106 and 87; both before the second look was shared out among threads)
+    const auto kern = (long)a.T * C <= 2l * 148 ? token_logprobs_kernel<T, 4, 2> : token_logprobs_kernel<T, 2, 4>;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)a.T * C);
     cfg.blockDim = dim3(kThreads);
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = C;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T>, a);
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kern, a);
 }
 }  // namespace
 
