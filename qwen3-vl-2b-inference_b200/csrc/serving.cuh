@@ -32,6 +32,9 @@ struct PlanArgs {
     int capacity;
     int32_t *free_count_out, *missing, *starts, *seq_ids, *positions, *slots;
     int max_tokens;
+    // set by the launcher
+    unsigned long long inv_p;
+    int page_ctas;
 };
 cudaError_t launch_plan_pages(const PlanArgs &a, cudaStream_t st);
 
