@@ -65,7 +65,7 @@ extern "C" {
 
 const char *qvl_status_string(int status);
 /* Tensor-core timeout word of the current device.  The tensor-core path
- * (M >= 16 products) bounds every wait; a wait that gives up sets the word,
+ * (M >= 16 products, tree attention) bounds every wait; a wait that gives up sets the word,
  * and while it is set every tensor-core launch on that device leaves without
  * computing.  Launches are asynchronous, so the call that timed out still
  * returned QVL_OK: this synchronises `stream`, stores 1 in *timed_out if the
@@ -495,7 +495,8 @@ int qvl_qknorm_mrope_kv_append(const void *q, const void *k, const void *v, int 
  * exist.  A row that sees nothing, a row of q outside [starts[0], starts[n_seqs]) and a
  * node past max_nodes get zeros.  max_ctx, a bound of ctx_lens + nodes, only
  * shapes the launch.  Types (q, cache): fp32 or fp16 over fp16, bf16 over
- * bf16.  D 64 or 128, max_nodes <= 256, page_size a multiple of 16. */
+ * bf16.  D 64 or 128, num_heads / num_kv_heads <= 128, max_nodes <= 256,
+ * page_size a multiple of 16. */
 size_t qvl_tree_attention_workspace_bytes(size_t n_seqs, size_t n_rows, int max_ctx, int max_nodes,
                                           const qvl_attn_dims *dims);
 int qvl_tree_attention(const void *q, int dtype, size_t q_stride, const void *k_pages, const void *v_pages,
