@@ -25,16 +25,17 @@
 //   MMA      S = Q K^T [128 rows, 128 positions], O = P V [128 rows, D], a thread each, so
 //            that one has its next product ready while the other's is under way.  Q, S, P (over S) and O in tensor memory, so that shared memory, whose
 //            bandwidth the products would need most of otherwise, is read for K and V alone
-//   softmax  two warpgroups, half of a tile's positions each; thread = row, so that maximum
-//            and sum need one exchange with the partner warp.  The maximum is left as it is
-//            until a score passes it by 2^7, which p held times 2^8 in fp16 allows: almost
-//            no tile rescales anything.  Between segments they bring the next one's Q to
-//            tensor memory
+//   softmax  two warpgroups, every other tile each, so that one's waits pass beside the
+//            other's work; thread = row.  A warpgroup's reference of a row (p = 2^(score -
+//            reference)) is left as it is until a score passes it by 2^7, which p held times
+//            2^8 in fp16 allows: almost no tile rescales anything, and scores are
+//            read once.  Between segments they bring the next one's Q to tensor memory
 //            A tile of at most 32 (64) rows is there four times (twice) over, in as many
 //            blocks of the 128 rows: each block takes its share of the positions and
 //            has p = 0 elsewhere, so that all warps have work, and the blocks are
 //            added at the end like parts of a context
-//   sums     two warpgroups (half of D each) add each tile's O to fp32 registers: the
+//   sums     two warpgroups (half of D each) add each tile's O to fp32 registers, times what
+//            its warpgroup's reference is below the largest: the
 //            tensor cores do not round their sums to nearest, so no chain of them is
 //            longer than a tile
 //   fixer    the nodes' ancestors as bits, and values of the drafted tile that some
@@ -92,13 +93,6 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
 }
 #define QVL_R8(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7])
 #define QVL_V8(r, o) "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7])
-__device__ __forceinline__ void tmem_ld32(uint32_t t, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : QVL_R8(r, 0), QVL_R8(r, 8), QVL_R8(r, 16), QVL_R8(r, 24)
-        : "r"(t));
-}
 __device__ __forceinline__ void tmem_st8(uint32_t t, const uint32_t (&r)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::QVL_V8(r, 0), "r"(t) : "memory");
 }
@@ -110,8 +104,8 @@ __device__ __forceinline__ void tmem_ld8(uint32_t t, uint32_t (&r)[8]) {
 __device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" : QVL_RW8(r, 0), QVL_RW8(r, 8)::"memory");
 }
-__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" : QVL_RW8(r, 0), QVL_RW8(r, 8), QVL_RW8(r, 16), QVL_RW8(r, 24)::"memory");
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[8], uint32_t (&q)[8]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : QVL_RW8(r, 0), QVL_RW8(q, 0)::"memory");
 }
 #undef QVL_RW8
 #undef QVL_R8
@@ -126,6 +120,13 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 2^(m - top) of what was held under the reference m <= top, which may be -inf both.
+__device__ __forceinline__ float weight(float m, float top) { return m == top ? 1.0f : ex2(m - top); }
 // A whole warp's wait: false for all lanes where one gave up.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
     return __all_sync(~0u, tc::mbar_wait(bar, parity, &g_tree_timeout));
@@ -265,18 +266,17 @@ struct Layout {
 };
 // What does not depend on the launch.
 struct Fixed {
-    float alpha[4][kRows];          // factors of the sums, by tile
+    float ref[4][kRows];            // references, by tile
     float cs[2][kRows];             // score factors, by segment
     float l[2][2][kRows];           // sums of p, by segment and warpgroup
-    float m[2][kRows];              // maxima, by segment
-    float px[2][2][kRows];          // maxima of a tile's halves, by tile and warpgroup
+    float m[2][2][kRows];           // references, by segment and warpgroup
     float qmax[2][kRows];           // maxima of a query row's halves
     Segment seg[4];
-    uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], s_free[2], p_ready[2], o_full[2], o_empty[2], x_bar[2][8], q_full,
+    uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], s_free[2], p_ready[2], o_full[2], o_empty[2], q_full,
         q_empty, anc_full[2], seg_full[4], seg_empty[4], l_bar[2], seg_done[2], qmax_bar, block_bar[2], fix_ask, fix_done;
     uint32_t valid[8];              // boxes of a tile that exist, by tile
     uint32_t bad[8][4];             // positions with values held back, by tile
-    uint32_t moved[4][4];           // some maximum moved, by tile and warp
+    uint32_t moved[4][4];           // some reference moved, by tile and warp
     uint32_t tmem;
     int off;
 };
@@ -338,7 +338,7 @@ __device__ __forceinline__ bool stage_queries(const TreeArgs &a, Fixed &fx, cons
 #pragma unroll
         for (int e = 0; e < V; ++e) x[e] = to_f32(t[e]);
     };
-    float f = qmul < 0.0f ? -1.0f : 1.0f, cs = fabsf(qmul);
+    float f = qmul < 0.0f ? -1.0f : 1.0f, cs = fmaxf(fabsf(qmul), 1.175494351e-38f);     // (times -inf: -inf)
     if constexpr (F::kSplitQ) {
         float mx = 0.0f;
 #pragma unroll 4
@@ -479,13 +479,12 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
         for (int i = 0; i < 2; ++i) {
             tc::mbar_init(bar(fx.s_full[i]), 1);
             tc::mbar_init(bar(fx.s_free[i]), 1);
-            tc::mbar_init(bar(fx.p_ready[i]), 256);
+            tc::mbar_init(bar(fx.p_ready[i]), 128);
             tc::mbar_init(bar(fx.o_full[i]), 1);
             tc::mbar_init(bar(fx.o_empty[i]), 256);
             tc::mbar_init(bar(fx.anc_full[i]), 1);
             tc::mbar_init(bar(fx.l_bar[i]), 256);
             tc::mbar_init(bar(fx.seg_done[i]), 16);
-            for (int w = 0; w < 8; ++w) tc::mbar_init(bar(fx.x_bar[i][w]), 1);
         }
         tc::mbar_init(bar(fx.q_full), 256);
         tc::mbar_init(bar(fx.q_empty), 1);
@@ -763,9 +762,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             }
         }
     } else if (warp < kSumWarp) {
-        // ---- softmax: thread = row, positions 64 wg .. 64 wg + 63 of each tile ----
+        // ---- softmax: thread = row, the tiles of this warpgroup's parity ----
         const int wg = warp >> 2, w4 = warp & 3, row = tid & 127;
-        const uint32_t ts = tmem + ((uint32_t)(w4 * 32) << 16) + wg * 64, tq = tmem + ((uint32_t)(w4 * 32) << 16) + kTmQ;
+        const uint32_t tr = tmem + ((uint32_t)(w4 * 32) << 16), sb = tr + wg * kTile;
         const Segment *g;
         // the queries of segment n, after the products with those before them
         Turn qt;
@@ -779,109 +778,94 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                 slot[h] = k_s + qt.slot * F::kSlot;
             }
             tc::tc_fence_after();
-            if ((ok = stage_queries<T, C, D>(a, fx, slot, fx.cs[n & 1], tq, wg, row, CAP, n))) mbar_arrive(bar(fx.q_full));
+            if ((ok = stage_queries<T, C, D>(a, fx, slot, fx.cs[n & 1], tr + kTmQ, wg, row, CAP, n))) mbar_arrive(bar(fx.q_full));
         };
         if (ok) queries(0);
         while (ok && next(g)) {
             // (what is seldom needed is read from shared memory where it is)
             const volatile Segment &sg = fx.seg[seg & 3];
             const int nt = sg.nt;
-            constexpr int cap = CAP;
+            constexpr int cap = CAP, nc = cap / 16;     // chunks of 16 positions of a block
             const int r = row & (cap - 1);          // the row, in its block
             const bool active = (w4 * 32 & (cap - 1)) < sg.rows;
-            // the block's share of the 64 positions: 1, 2 or 4 chunks of 16 from c0 on
-            const int c0 = cap == 32 ? w4 : cap == 64 ? w4 & 2 : 0;
+            const int c0 = row / cap * nc;          // the block's first chunk
+            const bool last = ((i + nt - 1) & 1) == wg;
             float m = -INFINITY, l = 0.0f;
             for (int k = 0; k < nt; ++k, ++i) {
-                const int b = i & 1;
                 qt.step(ly.nk);
                 // the next segment's queries as soon as this one's last scores are made, so
                 // that its first ones are made beside this one's last probabilities
-                if (k == nt - 1) {
+                if (k == nt - 1 && last) {
                     queries(seg + 1);
                     if (!ok) break;
                 }
-                if (!(ok = warp_wait(bar(fx.s_full[b]), (i >> 1) & 1))) break;
+                if ((i & 1) != wg) continue;
+                if (!(ok = warp_wait(bar(fx.s_full[wg]), (i >> 1) & 1))) break;
                 tc::tc_fence_after();
-                const int t0 = (sg.tile0 + k) * kTile + wg * 64, ctx = sg.ctx;
+                const int t0 = (sg.tile0 + k) * kTile, ctx = sg.ctx;
                 const uint32_t there = *reinterpret_cast<volatile uint32_t *>(&fx.valid[i & 7]);
-                const bool plain = t0 + 64 <= ctx && there == ly.all;
-                if (t0 + 64 > ctx && !(ok = warp_wait(bar(fx.anc_full[seg & 1]), (seg >> 1) & 1))) break;
-                // what the row sees of its block's positions: chunks 0 and 1 of its share, and
-                // (a share of 64) 2 and 3
-                uint32_t see0 = ~0u, see1 = ~0u;
-                if (!plain) {
-                    const uint32_t *anc = anc_s + ((seg & 1) * a.max_nodes + min((sg.r0 + r) / G, sg.n - 1)) * ly.words;
-                    auto word = [&](int w) {
-                        const int at = wg * 64 + w * 32;
-                        const uint32_t lo = (there >> ((at >> ly.box_log2) * (D / 64))) & 1u;
-                        const uint32_t hi = (there >> (((at + 16) >> ly.box_log2) * (D / 64))) & 1u;
-                        return seen_word(anc, ly.words, t0 + w * 32, ctx, sg.L) & ((lo ? 0xffffu : 0u) | (hi ? 0xffff0000u : 0u));
-                    };
-                    see0 = word(c0 >> 1) >> (c0 & 1) * 16;
-                    if constexpr (cap == kRows) see1 = word(1);
-                }
-                const uint32_t sb = ts + b * kTile;
-                float top = -INFINITY;
+                const bool plain = t0 + kTile <= ctx && there == ly.all;
+                if (t0 + kTile > ctx && !(ok = warp_wait(bar(fx.anc_full[seg & 1]), (seg >> 1) & 1))) break;
+                bool moved = false;
                 if (active) {
-                    constexpr int n = cap / 2;          // the share's positions
-                    uint32_t v[n];
-                    if constexpr (n == 16) {
-                        tc::tmem_ld16(sb + c0 * 16, v);
-                        tmem_wait_ld(v);
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < n; c += 32) tmem_ld32(sb + c0 * 16 + c, *reinterpret_cast<uint32_t(*)[32]>(v + c));
-#pragma unroll
-                        for (int c = 0; c < n; c += 32) tmem_wait_ld(*reinterpret_cast<uint32_t(*)[32]>(v + c));
-                    }
-                    float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int e = 0; e < n; ++e) {
-                        float x = __uint_as_float(v[e]);
-                        if (!plain) x = ((e < 32 ? see0 : see1) >> (e % 32)) & 1u ? x : -INFINITY;
-                        t4[e % 4] = fmaxf(t4[e % 4], x);
-                    }
-                    top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
-                }
-                // The partner warp has the other positions of these rows.  Its maximum is
-                // asked for at once only where this half's own does not fit under
-                // the old one (the first tile, almost always the only one); otherwise
-                // p is made with the old maximum first, and if then the partner's half
-                // turns out not to fit, p is scaled down after all.
-                fx.px[b][wg][row] = top;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(fx.x_bar[b][wg * 4 + w4]));
-                const float cs = fx.cs[seg & 1][row];
-                float f = 1.0f;                 // what a new maximum takes everything before down by
-                auto joint = [&] {
-                    if (!(ok = warp_wait(bar(fx.x_bar[b][(wg ^ 1) * 4 + w4]), (i >> 1) & 1))) return false;
-                    top = fmaxf(top, fx.px[b][wg ^ 1][row]);
-                    const float mt = top == -INFINITY ? top : top * cs;
-                    if (mt > m + 7.0f && r < sg.rows) {
-                        f = ex2(m - mt);
-                        m = mt;
-                        l *= f;
-                    }
-                    return true;
-                };
-                const bool early = __any_sync(~0u, (top == -INFINITY ? top : top * cs) > m + 7.0f && r < sg.rows);
-                if (early && !joint()) break;
-                if (active) {
-                    const float mm = m == -INFINITY ? 0.0f : m - kPBias;
+                    const float cs = fx.cs[seg & 1][row];
+                    const uint64_t cs2 = two(cs, cs);
+                    float mm = m == -INFINITY ? 0.0f : kPBias - m;
                     uint64_t ls = two(0.0f, 0.0f);
-                    const uint64_t cs2 = two(cs, cs), mm2 = two(-mm, -mm);
-                    // 16 scores at a time, the next ones on their way; the high and low halves
-                    // of their p take the 16 columns that they leave
-                    auto part = [&](int c, const uint32_t (&r)[16], uint32_t bits) {
+                    // 16 scores of chunk c; the high and low halves of their p take the 16 columns
+                    // that they leave
+                    auto part = [&](int c, uint32_t (&v)[16]) {
+                        if (!plain) {
+                            // what the row sees of them
+                            const uint32_t *anc = anc_s + ((seg & 1) * a.max_nodes + min((sg.r0 + r) / G, sg.n - 1)) * ly.words;
+                            const bool box = (there >> ((c * 16 >> ly.box_log2) * (D / 64))) & 1u;
+                            const uint32_t see = box ? seen_word(anc, ly.words, t0 + (c >> 1) * 32, ctx, sg.L) >> (c & 1) * 16 : 0u;
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) v[e] = (see >> e) & 1u ? v[e] : 0xff800000u;
+                        }
+                        float top = max3(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]));
+                        float top2 = max3(__uint_as_float(v[3]), __uint_as_float(v[4]), __uint_as_float(v[5]));
+#pragma unroll
+                        for (int e = 6; e < 14; e += 4) {
+                            top = max3(top, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+                            top2 = max3(top2, __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
+                        }
+                        top = max3(top, __uint_as_float(v[14]), __uint_as_float(v[15]));
+                        const float mt = fmaxf(top, top2) * cs;
+                        if (__any_sync(~0u, mt > m + 7.0f && r < sg.rows)) {
+                            // a new reference, a whole power of two; what the tile has under the old one is
+                            // taken down
+                            moved = true;
+                            float f = 1.0f;
+                            if (mt > m + 7.0f && r < sg.rows) {
+                                const float up = ceilf(mt);
+                                f = ex2(m - up);
+                                m = up;
+                                mm = kPBias - m;
+                                l *= f;
+                                ls = fma2(ls, two(f, f), two(-0.0f, -0.0f));
+                            }
+                            tmem_wait_st();
+#pragma unroll 1
+                            for (int x = c0; x < c; ++x) {
+                                uint32_t hi[8], lo[8];
+                                tmem_ld8(sb + x * 16, hi);
+                                tmem_ld8(sb + x * 16 + 8, lo);
+                                tmem_wait_ld(hi, lo);
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) {
+                                    const float2 h = unpack2<C>(hi[e]), w = unpack2<C>(lo[e]);
+                                    if (f != 1.0f) split2<C>((h.x + w.x) * f, (h.y + w.y) * f, hi[e], lo[e]);
+                                }
+                                tmem_st8(sb + x * 16, hi);
+                                tmem_st8(sb + x * 16 + 8, lo);
+                            }
+                        }
+                        const uint64_t mm2 = two(mm, mm);
                         uint32_t hi[8], lo[8];
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
-                            float2 x = parts(fma2(two(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), cs2, mm2));
-                            if (!plain) {
-                                x.x = (bits >> (2 * e)) & 1u ? x.x : -INFINITY;
-                                x.y = (bits >> (2 * e)) & 2u ? x.y : -INFINITY;
-                            }
+                            const float2 x = parts(fma2(two(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), cs2, mm2));
                             const float pa = ex2(x.x), pb = ex2(x.y);
                             ls = add2(ls, two(pa, pb));
                             split2<C>(pa, pb, hi[e], lo[e]);
@@ -891,26 +875,21 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                     };
                     uint32_t ra[16], rb[16];
                     tc::tmem_ld16(sb + c0 * 16, ra);
-                    if constexpr (cap != 32) tc::tmem_ld16(sb + c0 * 16 + 16, rb);
-                    tmem_wait_ld(ra);
-                    part(c0, ra, see0);
-                    if constexpr (cap != 32) {
-                        tmem_wait_ld(rb);
-                        if constexpr (cap == kRows) tc::tmem_ld16(sb + 32, ra);
-                        part(c0 + 1, rb, see0 >> 16);
-                    }
-                    if constexpr (cap == kRows) {
+#pragma unroll 1
+                    for (int c = c0; c < c0 + nc; c += 2) {
                         tmem_wait_ld(ra);
-                        tc::tmem_ld16(sb + 48, rb);
-                        part(2, ra, see1);
+                        tc::tmem_ld16(sb + c * 16 + 16, rb);
+                        part(c, ra);
                         tmem_wait_ld(rb);
-                        part(3, rb, see1 >> 16);
-                    } else {
+                        if (c + 2 < c0 + nc) tc::tmem_ld16(sb + c * 16 + 32, ra);
+                        part(c + 1, rb);
+                    }
+                    if constexpr (cap != kRows) {
                         // the other blocks' positions
                         const uint32_t none[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-                        for (int c = 0; c < 4; ++c)
-                            if (cap == 32 ? c != c0 : c >> 1 != c0 >> 1) {
+                        for (int c = 0; c < 8; ++c)
+                            if (c / nc != c0 / nc) {
                                 tmem_st8(sb + c * 16, none);
                                 tmem_st8(sb + c * 16 + 8, none);
                             }
@@ -918,36 +897,15 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                     l += parts(ls).x + parts(ls).y;
                     tmem_wait_st();
                 }
-                if (!early && !joint()) break;
-                const bool moved = __any_sync(~0u, f != 1.0f);
-                if (moved) {
-                    if (wg == 0) fx.alpha[i & 3][row] = f;
-                    if (!early && active) {
-#pragma unroll 1
-                        for (int c = c0 * 16; c < c0 * 16 + cap / 2; c += 16) {
-                            uint32_t hi[8], lo[8];
-                            tmem_ld8(sb + c, hi);
-                            tmem_ld8(sb + c + 8, lo);
-                            tc::tmem_wait_ld();
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                const float2 h = unpack2<C>(hi[e]), w = unpack2<C>(lo[e]);
-                                const float pa = (h.x + w.x) * f, pb = (h.y + w.y) * f;
-                                split2<C>(pa, pb, hi[e], lo[e]);
-                            }
-                            tmem_st8(sb + c, hi);
-                            tmem_st8(sb + c + 8, lo);
-                        }
-                        tmem_wait_st();
-                    }
-                }
-                if (wg == 0 && lane == 0) fx.moved[i & 3][w4] = moved;
+                if (moved) fx.ref[i & 3][row] = m;
+                if (lane == 0) fx.moved[i & 3][w4] = moved;
                 tc::tc_fence_before();
-                mbar_arrive(bar(fx.p_ready[b]));
+                mbar_arrive(bar(fx.p_ready[wg]));
             }
+            if (ok && !last) queries(seg + 1);
             if (!ok || (seg > 1 && !(ok = warp_wait(bar(fx.seg_done[seg & 1]), ((seg >> 1) - 1) & 1)))) break;
             fx.l[seg & 1][wg][row] = l;
-            if (wg == 0) fx.m[seg & 1][row] = m;
+            fx.m[seg & 1][wg][row] = m;
             mbar_arrive(bar(fx.l_bar[seg & 1]));
             if (lane == 0) mbar_arrive(bar(fx.seg_done[seg & 1]));
             done();
@@ -979,6 +937,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             uint64_t acc2[CW / 2];
 #pragma unroll
             for (int c = 0; c < CW / 2; ++c) acc2[c] = two(0.0f, 0.0f);
+            float top = -INFINITY, f0 = 1.0f, f1 = 1.0f;       // the larger reference; 2^(reference - top) of both
             for (int k = 0; k < nt; ++k, ++i) {
                 constexpr int OB = F::kOB;
                 const int ob = i % OB;
@@ -986,11 +945,20 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                 tc::tc_fence_after();
                 if (active) {
                     // (written before the probabilities, on which the product waited)
-                    if (k > 0 && *reinterpret_cast<volatile uint32_t *>(&fx.moved[i & 3][w4])) {
-                        const uint64_t f = two(fx.alpha[i & 3][row], fx.alpha[i & 3][row]), z = two(-0.0f, -0.0f);
+                    if (*reinterpret_cast<volatile uint32_t *>(&fx.moved[i & 3][w4])) {
+                        const float m = fx.ref[i & 3][row];
+                        if (__any_sync(~0u, m > top)) {
+                            const float up = fmaxf(m, top), f = weight(top, up);
+                            const uint64_t f2 = two(f, f), z = two(-0.0f, -0.0f);
 #pragma unroll
-                        for (int c = 0; c < CW / 2; ++c) acc2[c] = fma2(acc2[c], f, z);
+                            for (int c = 0; c < CW / 2; ++c) acc2[c] = fma2(acc2[c], f2, z);
+                            f0 *= f;
+                            f1 *= f;
+                            top = up;
+                        }
+                        (i & 1 ? f1 : f0) = weight(m, top);
                     }
+                    const uint64_t f = i & 1 ? two(f1, f1) : two(f0, f0);
 #pragma unroll
                     for (int c = 0; c < CW; c += 16) {
                         uint32_t v[16];
@@ -998,7 +966,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                         tmem_wait_ld(v);
 #pragma unroll
                         for (int e = 0; e < 16; e += 2)
-                            acc2[(c + e) / 2] = add2(acc2[(c + e) / 2], two(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
+                            acc2[(c + e) / 2] = fma2(two(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), f, acc2[(c + e) / 2]);
                     }
                     const int t0 = (sg.tile0 + k) * kTile, ctx = sg.ctx;
                     if (t0 + kTile > ctx) {
@@ -1008,9 +976,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                             const uint32_t bad = *reinterpret_cast<volatile uint32_t *>(&fx.bad[i & 7][w]);
                             if (!bad) continue;
                             // (by the block that has the position)
-                            const uint32_t mine = cap == kRows ? ~0u : (w & 1) != w4 >> 1 ? 0u : cap == 64 ? ~0u
-                                                                     : w4 & 1 ? 0xffff0000u : 0xffffu;
-                            for (uint32_t x = bad & mine & seen_word(anc, ly.words, t0 + 32 * w, ctx, sg.L); x; x &= x - 1) {
+                            if (w * 32 / cap != row / cap) continue;
+                            for (uint32_t x = bad & seen_word(anc, ly.words, t0 + 32 * w, ctx, sg.L); x; x &= x - 1) {
                                 const int t = t0 + 32 * w + __ffs(x) - 1;
                                 const int pg = a.table[(size_t)g->s * a.maxp + t / a.P];
                                 const C *v = reinterpret_cast<const C *>(a.v_pages) +
@@ -1037,14 +1004,20 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                 acc[2 * c] = v.x;
                 acc[2 * c + 1] = v.y;
             }
-            const float (*lp)[kRows] = fx.l[seg & 1];
-            const float *mp = fx.m[seg & 1];
+            const float (*lp)[kRows] = fx.l[seg & 1], (*mp)[kRows] = fx.m[seg & 1];
+            // reference and sum of a row of a block, of both warpgroups' tiles
+            auto of_row = [&](int x, float &l) {
+                const float m = fmaxf(mp[0][x], mp[1][x]);
+                l = lp[0][x] * weight(mp[0][x], m) + lp[1][x] * weight(mp[1][x], m);
+                return m;
+            };
             const int node = (sg.r0 + r) / G, h = sg.r0 + r - node * G;
             T *o = out + ((long)(sg.first + node) * a.NH + sg.kvh * G + h) * D + half * CW;
             const int part = sg.part;
             const size_t at = ((size_t)blockIdx.x * 2 + max(part, 0)) * kRows + r;
-            float m = mp[r], l = lp[0][r] + lp[1][r];
+            float m, l;
             if constexpr (cap == kRows) {
+                m = of_row(r, l);
                 if (r < sg.rows) {
                     if (part < 0) {
                         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -1061,14 +1034,16 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                 // the blocks of a row are added; each of its threads has a share of the values
                 constexpr int nb = kRows / cap, share = CW / nb;
                 const int mine = row / cap;
+                m = -INFINITY;
 #pragma unroll
-                for (int b = 1; b < nb; ++b) m = fmaxf(m, mp[b * cap + r]);
+                for (int b = 0; b < nb; ++b) m = fmaxf(m, fmaxf(mp[0][b * cap + r], mp[1][b * cap + r]));
                 l = 0.0f;
                 for (int b = 0; b < nb; ++b) {
-                    const float mb = mp[b * cap + r];
-                    l += (lp[0][b * cap + r] + lp[1][b * cap + r]) * (mb == m ? 1.0f : ex2(mb - m));
+                    float lb;
+                    const float mb = of_row(b * cap + r, lb);
+                    l += lb * weight(mb, m);
                 }
-                const float f = mp[row] == m ? 1.0f : ex2(mp[row] - m), inv = l == 0.0f ? 0.0f : 1.0f / l;
+                const float f = weight(top, m), inv = l == 0.0f ? 0.0f : 1.0f / l;
                 auto meet = [&] {
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar(fx.block_bar[half]));
