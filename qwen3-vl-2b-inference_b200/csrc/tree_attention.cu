@@ -93,6 +93,13 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
 }
 #define QVL_R8(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7])
 #define QVL_V8(r, o) "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7])
+__device__ __forceinline__ void tmem_ld32(uint32_t t, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : QVL_R8(r, 0), QVL_R8(r, 8), QVL_R8(r, 16), QVL_R8(r, 24)
+        : "r"(t));
+}
 __device__ __forceinline__ void tmem_st8(uint32_t t, const uint32_t (&r)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::QVL_V8(r, 0), "r"(t) : "memory");
 }
@@ -103,6 +110,9 @@ __device__ __forceinline__ void tmem_ld8(uint32_t t, uint32_t (&r)[8]) {
 #define QVL_RW8(r, o) "+r"(r[o]), "+r"(r[o + 1]), "+r"(r[o + 2]), "+r"(r[o + 3]), "+r"(r[o + 4]), "+r"(r[o + 5]), "+r"(r[o + 6]), "+r"(r[o + 7])
 __device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" : QVL_RW8(r, 0), QVL_RW8(r, 8)::"memory");
+}
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : QVL_RW8(r, 0), QVL_RW8(r, 8), QVL_RW8(r, 16), QVL_RW8(r, 24)::"memory");
 }
 __device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[8], uint32_t (&q)[8]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" : QVL_RW8(r, 0), QVL_RW8(q, 0)::"memory");
@@ -243,7 +253,7 @@ struct Segment {
 // What the joining launch knows of a partial segment.
 struct Part {
     int first, kvh, r0, rows;      // rows 0: nothing
-    int starts, ends;              // holds the pair's first / last tile
+    int behind, pad;               // the CTAs after this one that have parts of the pair too
 };
 
 template <typename T, int D>
@@ -285,12 +295,12 @@ constexpr uint32_t kTmO = 256, kTmQ = 384, kTmCols = 512;
 
 __host__ __device__ constexpr size_t part_floats(int D) { return (size_t)kRows * D; }
 __host__ __device__ constexpr size_t part_bytes(int D) {
-    return (size_t)kSMs * 2 * (part_floats(D) * sizeof(float) + kRows * sizeof(float2) + sizeof(Part));
+    return (size_t)kSMs * (2 * (part_floats(D) * sizeof(float) + kRows * sizeof(float2)) + sizeof(Part));
 }
 struct Workspace {
     float *acc;         // [CTA][2][row][D]
     float2 *ml;         // [CTA][2][row]: maximum, sum
-    Part *part;         // [CTA][2]
+    Part *part;         // [CTA]: the pair that begins in its last segment and goes on behind it
 };
 __device__ __forceinline__ Workspace workspace_of(void *p, int D) {
     Workspace w;
@@ -300,25 +310,6 @@ __device__ __forceinline__ Workspace workspace_of(void *p, int D) {
     return w;
 }
 
-template <typename T, int E>
-__device__ __forceinline__ void load_e(const T *p, float (&x)[E]) {
-    if constexpr (sizeof(T) * E == 16) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(p);
-        const T *t = reinterpret_cast<const T *>(&v);
-#pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = to_f32(t[e]);
-    } else if constexpr (sizeof(T) * E == 8) {
-        const uint2 v = *reinterpret_cast<const uint2 *>(p);
-        const T *t = reinterpret_cast<const T *>(&v);
-#pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = to_f32(t[e]);
-    } else {
-        const uint32_t v = *reinterpret_cast<const uint32_t *>(p);
-        const T *t = reinterpret_cast<const T *>(&v);
-#pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = to_f32(t[e]);
-    }
-}
 // Half of a query row from the K ring's slots (rows of 128 bytes, 128-byte swizzle) into
 // tensor memory (columns of two 16-bit values, hi and then lo) by the thread of the row,
 // and the row's score factor.  False where a wait gave up.
@@ -577,7 +568,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
         }
         Request rq{};
         if (left > 0) rq = request_of(a, s);
-        if (lane < 2) ws.part[blockIdx.x * 2 + lane].rows = 0;
+        if (lane == 0) ws.part[blockIdx.x].rows = 0;
         __syncwarp();
         // lane l: box l / (D / 64) of the tile's 64-value half l % (D / 64)
         const int lanes = (kTile >> ly.box_log2) * (D / 64);
@@ -590,6 +581,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
         asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(once));
         while (ok) {
             Segment g{};
+            long pair_end = 0;                                     // where the pair's units end, of all
             while (left > 0) {
                 while (off >= rq.units(a.NKV, begin)) {
                     off -= rq.units(a.NKV, begin);
@@ -614,8 +606,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                 g.n = rq.n;
                 const bool starts = g.tile0 == 0, ends = g.tile0 + g.nt == rq.tiles;
                 g.part = starts && ends ? -1 : starts ? 1 : 0;
-                if (g.part >= 0 && lane == 0)
-                    ws.part[blockIdx.x * 2 + g.part] = {g.first, g.kvh, g.r0, g.rows, starts, ends};
+                pair_end = hi - left + (len - u1);
                 break;
             }
             g.nt = max(g.nt, 0);
@@ -674,6 +665,13 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                 if (lane < lanes)
                     tma_load_once(tc::smem_u32(v_s + vt.slot * F::kSlot + to), &tm_v, half * 64, y, bar(fx.v_full[vt.slot]), once);
                 vt.step(ly.nv);
+            }
+            if (g.part == 1 && lane == 0) {
+                // the CTA that has the pair's last unit
+                const long x = pair_end - 1, y = x - more * (each + 1);
+                const long last = total < 1l << 31 ? (y < 0 ? (uint32_t)x / (uint32_t)(each + 1) : more + (uint32_t)y / (uint32_t)each)
+                                                   : (y < 0 ? x / (each + 1) : more + y / each);
+                ws.part[blockIdx.x] = {g.first, g.kvh, g.r0, g.rows, (int)(last - me), 0};
             }
         }
         // after a wait that gave up: loads in flight land before the CTA ends
@@ -812,26 +810,29 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                     const uint64_t cs2 = two(cs, cs);
                     float mm = m == -INFINITY ? 0.0f : kPBias - m;
                     uint64_t ls = two(0.0f, 0.0f);
-                    // 16 scores of chunk c; the high and low halves of their p take the 16 columns
-                    // that they leave
-                    auto part = [&](int c, uint32_t (&v)[16]) {
+                    // 32 positions at a time, enough of them to keep the pipes busy: their scores, and
+                    // then the high and low halves of their p in the same columns, 16 by 16
+                    auto part = [&](int c) {
+                        uint32_t v[32];
+                        tmem_ld32(sb + c * 16, v);
+                        tmem_wait_ld(v);
                         if (!plain) {
                             // what the row sees of them
                             const uint32_t *anc = anc_s + ((seg & 1) * a.max_nodes + min((sg.r0 + r) / G, sg.n - 1)) * ly.words;
-                            const bool box = (there >> ((c * 16 >> ly.box_log2) * (D / 64))) & 1u;
-                            const uint32_t see = box ? seen_word(anc, ly.words, t0 + (c >> 1) * 32, ctx, sg.L) >> (c & 1) * 16 : 0u;
+                            const uint32_t lo = (there >> ((c * 16 >> ly.box_log2) * (D / 64))) & 1u;
+                            const uint32_t hi = (there >> ((c * 16 + 16 >> ly.box_log2) * (D / 64))) & 1u;
+                            const uint32_t see = seen_word(anc, ly.words, t0 + c * 16, ctx, sg.L) &
+                                                 ((lo ? 0xffffu : 0u) | (hi ? 0xffff0000u : 0u));
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) v[e] = (see >> e) & 1u ? v[e] : 0xff800000u;
+                            for (int e = 0; e < 32; ++e) v[e] = (see >> e) & 1u ? v[e] : 0xff800000u;
                         }
-                        float top = max3(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]));
-                        float top2 = max3(__uint_as_float(v[3]), __uint_as_float(v[4]), __uint_as_float(v[5]));
+                        float t4[4];
 #pragma unroll
-                        for (int e = 6; e < 14; e += 4) {
-                            top = max3(top, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
-                            top2 = max3(top2, __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
-                        }
-                        top = max3(top, __uint_as_float(v[14]), __uint_as_float(v[15]));
-                        const float mt = fmaxf(top, top2) * cs;
+                        for (int e = 0; e < 4; ++e) t4[e] = fmaxf(__uint_as_float(v[e]), __uint_as_float(v[28 + e]));
+#pragma unroll
+                        for (int e = 4; e < 28; e += 2)
+                            t4[e / 2 % 4] = max3(t4[e / 2 % 4], __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+                        const float mt = fmaxf(max3(t4[0], t4[1], t4[2]), t4[3]) * cs;
                         if (__any_sync(~0u, mt > m + 7.0f && r < sg.rows)) {
                             // a new reference, a whole power of two; what the tile has under the old one is
                             // taken down
@@ -862,28 +863,22 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                             }
                         }
                         const uint64_t mm2 = two(mm, mm);
-                        uint32_t hi[8], lo[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const float2 x = parts(fma2(two(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), cs2, mm2));
-                            const float pa = ex2(x.x), pb = ex2(x.y);
-                            ls = add2(ls, two(pa, pb));
-                            split2<C>(pa, pb, hi[e], lo[e]);
+                        for (int b = 0; b < 2; ++b) {
+                            uint32_t hi[8], lo[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const float2 x = parts(fma2(two(__uint_as_float(v[b * 16 + 2 * e]), __uint_as_float(v[b * 16 + 2 * e + 1])), cs2, mm2));
+                                const float pa = ex2(x.x), pb = ex2(x.y);
+                                ls = add2(ls, two(pa, pb));
+                                split2<C>(pa, pb, hi[e], lo[e]);
+                            }
+                            tmem_st8(sb + (c + b) * 16, hi);
+                            tmem_st8(sb + (c + b) * 16 + 8, lo);
                         }
-                        tmem_st8(sb + c * 16, hi);
-                        tmem_st8(sb + c * 16 + 8, lo);
                     };
-                    uint32_t ra[16], rb[16];
-                    tc::tmem_ld16(sb + c0 * 16, ra);
 #pragma unroll 1
-                    for (int c = c0; c < c0 + nc; c += 2) {
-                        tmem_wait_ld(ra);
-                        tc::tmem_ld16(sb + c * 16 + 16, rb);
-                        part(c, ra);
-                        tmem_wait_ld(rb);
-                        if (c + 2 < c0 + nc) tc::tmem_ld16(sb + c * 16 + 32, ra);
-                        part(c + 1, rb);
-                    }
+                    for (int c = c0; c < c0 + nc; c += 2) part(c);
                     if constexpr (cap != kRows) {
                         // the other blocks' positions
                         const uint32_t none[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -1133,49 +1128,64 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
 }
 
 // Joins the parts of the pairs that more than one CTA worked on: weights
-// 2^(m_part - max m).  grid (CTAs, rows / 8): block (c, y) has the pair whose
-// first part is CTA c's last segment; one warp a row.
+// 2^(m_part - max m).  grid (CTAs, rows / 16): block (c, y) has the pair whose
+// first part is CTA c's last segment; 16 lanes a row, and four parts' reads on
+// their way at a time (latency is all that counts here).
+constexpr int kJoinRows = 16;
 template <typename T, int D>
-__global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ TreeArgs a, int ctas) {
+__global__ void __launch_bounds__(16 * kJoinRows) tree_join_kernel(const __grid_constant__ TreeArgs a) {
     pdl_launch_dependents();
     pdl_wait();
     const Workspace ws = workspace_of(a.workspace, D);
-    const int lane = threadIdx.x & 31, row = blockIdx.y * 8 + (threadIdx.x >> 5), c0 = blockIdx.x;
-    const Part p = ws.part[c0 * 2 + 1];
+    const int col = threadIdx.x & 15, row = blockIdx.y * kJoinRows + (threadIdx.x >> 4), c0 = blockIdx.x;
+    const Part p = ws.part[c0];
     if (row >= p.rows) return;
-    // the parts: this CTA's last segment and the first ones of the CTAs behind it
-    int behind = 0;
-    for (int c = c0 + 1; c < ctas; c += 32) {
-        const Part q = c + lane < ctas ? ws.part[(c + lane) * 2] : Part{};
-        const uint32_t e = __ballot_sync(~0u, q.rows == 0 || q.ends);
-        if (e) {
-            behind = c - c0 + __ffs(e) - 1;
-            break;
-        }
-    }
-    auto at = [&](int k) { return ((size_t)(c0 + k) * 2 + (k == 0)) * kRows + row; };
-    float m = -INFINITY;
-    for (int k = lane; k <= behind; k += 32) m = fmaxf(m, ws.ml[at(k)].x);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-    constexpr int E = D / 32;
-    float acc[E], l = 0.0f;
+    constexpr int E = D / 16, U = 4;
+    float acc[E], m = -INFINITY, l = 0.0f;
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-#pragma unroll 4
-    for (int k = 0; k <= behind; ++k) {
-        const float2 st = ws.ml[at(k)];
-        float v[E];
-        load_e<float, E>(ws.acc + at(k) * D + lane * E, v);
-        const float f = st.x == m ? 1.0f : ex2(st.x - m);
-        l = fmaf(st.y, f, l);
+#pragma unroll 1
+    for (int k = 0; k <= p.behind; k += U) {
+        float2 st[U];
+        float4 v[U][E / 4];
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = fmaf(v[e], f, acc[e]);
+        for (int u = 0; u < U; ++u) {
+            st[u] = make_float2(-INFINITY, 0.0f);
+#pragma unroll
+            for (int e = 0; e < E / 4; ++e) v[u][e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (k + u > p.behind) continue;
+            const size_t at = ((size_t)(c0 + k + u) * 2 + (k + u == 0)) * kRows + row;
+            st[u] = ws.ml[at];
+#pragma unroll
+            for (int e = 0; e < E / 4; ++e) v[u][e] = *reinterpret_cast<const float4 *>(ws.acc + at * D + e * 64 + col * 4);
+        }
+        float up = m;
+#pragma unroll
+        for (int u = 0; u < U; ++u) up = fmaxf(up, st[u].x);
+        const float f = weight(m, up);
+        m = up;
+        l *= f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] *= f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float w = weight(st[u].x, m);
+            l = fmaf(st[u].y, w, l);
+#pragma unroll
+            for (int e = 0; e < E / 4; ++e) {
+                acc[4 * e] = fmaf(v[u][e].x, w, acc[4 * e]);
+                acc[4 * e + 1] = fmaf(v[u][e].y, w, acc[4 * e + 1]);
+                acc[4 * e + 2] = fmaf(v[u][e].z, w, acc[4 * e + 2]);
+                acc[4 * e + 3] = fmaf(v[u][e].w, w, acc[4 * e + 3]);
+            }
+        }
     }
     const int G = a.NH / a.NKV, node = (p.r0 + row) / G, h = p.r0 + row - node * G;
-    T *o = reinterpret_cast<T *>(a.out) + ((long)(p.first + node) * a.NH + p.kvh * G + h) * D + lane * E;
+    T *o = reinterpret_cast<T *>(a.out) + ((long)(p.first + node) * a.NH + p.kvh * G + h) * D + col * 4;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = from_f32<T>(l == 0.0f ? 0.0f : acc[e] / l);
+    for (int e = 0; e < E / 4; ++e)
+        store4(o + e * 64, make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]), l == 0.0f, inv);
 }
 
 // ---------------------------------------------------------------- host side
@@ -1282,10 +1292,10 @@ cudaError_t launch_cap(const TreeArgs &a, cudaStream_t st) {
     cfg.numAttrs = 1;
     e = cudaLaunchKernelEx(&cfg, kern, mk, mv, mq, a, ly);
     if (e != cudaSuccess || ctas == 1) return e;
-    cfg.gridDim = dim3(ctas, (unsigned)((std::min(qrows, (long)kRows) + 7) / 8));
-    cfg.blockDim = dim3(256);
+    cfg.gridDim = dim3(ctas, (unsigned)((std::min(qrows, (long)kRows) + kJoinRows - 1) / kJoinRows));
+    cfg.blockDim = dim3(16 * kJoinRows);
     cfg.dynamicSmemBytes = 0;
-    return cudaLaunchKernelEx(&cfg, tree_join_kernel<T, D>, a, ctas);
+    return cudaLaunchKernelEx(&cfg, tree_join_kernel<T, D>, a);
 }
 // Rows of a request that has max_nodes: up to 32 or 64 go in blocks.
 template <typename T, typename C, int D>
