@@ -256,11 +256,14 @@ struct Part {
     int behind, pad;               // the CTAs after this one that have parts of the pair too
 };
 
-template <typename T, int D>
+template <typename T, int D, int CAP>
 struct Conf {
     static constexpr bool kSplitQ = std::is_same<T, float>::value;
     static constexpr int kQHalves = kSplitQ ? 2 : 1;
     static constexpr int kSlot = kTile * D * 2;
+    // The queries come in boxes of CAP rows of 128 bytes, as many as fit to a slot
+    static constexpr int kQBox = CAP * 128, kQBoxes = D * (int)sizeof(T) / 128;
+    static constexpr int kQPer = kQBoxes < kSlot / kQBox ? kQBoxes : kSlot / kQBox, kQSlots = kQBoxes / kQPer;
     static constexpr int kMaxRing = 4;
     static constexpr int kOB = D == 64 ? 2 : 1;             // buffers of O
 };
@@ -313,17 +316,17 @@ __device__ __forceinline__ Workspace workspace_of(void *p, int D) {
 // Half of a query row from the K ring's slots (rows of 128 bytes, 128-byte swizzle) into
 // tensor memory (columns of two 16-bit values, hi and then lo) by the thread of the row,
 // and the row's score factor.  False where a wait gave up.
-template <typename T, typename C, int D>
-__device__ __forceinline__ bool stage_queries(const TreeArgs &a, Fixed &fx, const unsigned char *const (&slot)[2], float *cs_s,
-                                              uint32_t tq, int half, int row, int cap, int turn) {
-    using F = Conf<T, D>;
+template <typename T, typename C, int D, int CAP>
+__device__ __forceinline__ bool stage_queries(const TreeArgs &a, Fixed &fx, const unsigned char *const (&slot)[Conf<T, D, CAP>::kQSlots], float *cs_s,
+                                              uint32_t tq, int half, int row, int turn) {
+    using F = Conf<T, D, CAP>;
     constexpr int H = D / 2, V = 16 / sizeof(T);             // values of 16 bytes
-    const int lane = threadIdx.x & 31, src = row & (cap - 1);
+    const int lane = threadIdx.x & 31, src = row & (CAP - 1);
     const float qmul = a.scale * kLog2e;
     // values [c, c + V) of the half
     auto load = [&](int c, float (&x)[V]) {
         const int byte = (half * H + c) * (int)sizeof(T), chunk = byte >> 7;
-        const unsigned char *p = (chunk < F::kSlot / 16384 ? slot[0] : slot[1]) + chunk % (F::kSlot / 16384) * 16384;
+        const unsigned char *p = (chunk < F::kQPer ? slot[0] : slot[F::kQSlots - 1]) + chunk % F::kQPer * F::kQBox;
         const uint4 v = *reinterpret_cast<const uint4 *>(p + src * 128 + ((((byte >> 4) & 7) ^ (src & 7)) << 4));
         const T *t = reinterpret_cast<const T *>(&v);
 #pragma unroll
@@ -442,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                const __grid_constant__ CUtensorMap tm_q,
                const __grid_constant__ TreeArgs a, const __grid_constant__ Layout ly) {
-    using F = Conf<T, D>;
+    using F = Conf<T, D, CAP>;
     // (addresses in it are constants, which keeps them out of the registers)
     extern __shared__ __align__(1024) unsigned char smem[];
     Fixed &fx = *reinterpret_cast<Fixed *>(smem);
@@ -518,16 +521,25 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
     if (warp == kTmaWarp) {
         // ---- segments, pages and loads ----
         // this CTA's stretch of all units: [lo, hi), found among the requests 32 at a time
-        long tiles = 0, pairs = 0;
-        for (int x = lane; x < a.S; x += 32) {
-            const Request r = request_of(a, x);
-            tiles += (long)r.tiles * r.row_tiles * a.NKV;
-            pairs += (long)r.row_tiles * a.NKV;
-        }
+        // (sums over the requests up to each lane's; of up to 32 requests they stay)
+        Request mine{};
+        long tiles = 0, pairs = 0, tiles_to = 0, pairs_to = 0;
+        auto sums = [&](int base) {
+            mine = Request{};
+            if (base + lane < a.S) mine = request_of(a, base + lane);
+            pairs_to = mine.row_tiles * (long)a.NKV;
+            tiles_to = pairs_to * mine.tiles;
 #pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            tiles += __shfl_xor_sync(~0u, tiles, o);
-            pairs += __shfl_xor_sync(~0u, pairs, o);
+            for (int o = 1; o < 32; o <<= 1) {
+                const long t = __shfl_up_sync(~0u, tiles_to, o), p = __shfl_up_sync(~0u, pairs_to, o);
+                tiles_to += lane >= o ? t : 0;
+                pairs_to += lane >= o ? p : 0;
+            }
+        };
+        for (int base = 0; base < a.S; base += 32) {
+            sums(base);
+            tiles += __shfl_sync(~0u, tiles_to, 31);
+            pairs += __shfl_sync(~0u, pairs_to, 31);
         }
         // What a pair costs beside its tiles, in tiles: about four where blocks have to be
         // added and tiles are quick, one otherwise (32 requests of up to 16 nodes over 4096:
@@ -549,25 +561,26 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
         const long lo = min(each * me + min(me, more), total), hi = min(lo + each + (me < more ? 1 : 0), total);
         int s = 0;
         long off = lo, left = ok ? hi - lo : 0;
+        Request rq{};
         for (int base = 0; left > 0; base += 32) {
-            long inc = base + lane < a.S ? request_of(a, base + lane).units(a.NKV, begin) : 0;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long up = __shfl_up_sync(~0u, inc, o);
-                if (lane >= o) inc += up;
-            }
+            if (a.S > 32) sums(base);
+            const long inc = tiles_to + pairs_to * begin;
             const uint32_t past = __ballot_sync(~0u, inc > off);
             if (past) {
                 const int at = __ffs(past) - 1;
                 const long before = __shfl_sync(~0u, inc, max(at - 1, 0));
                 s = base + at;
                 off -= at ? before : 0;
+                rq.first = __shfl_sync(~0u, mine.first, at);
+                rq.n = __shfl_sync(~0u, mine.n, at);
+                rq.ctx = __shfl_sync(~0u, mine.ctx, at);
+                rq.L = __shfl_sync(~0u, mine.L, at);
+                rq.tiles = __shfl_sync(~0u, mine.tiles, at);
+                rq.row_tiles = __shfl_sync(~0u, mine.row_tiles, at);
                 break;
             }
             off -= __shfl_sync(~0u, inc, 31);
         }
-        Request rq{};
-        if (left > 0) rq = request_of(a, s);
         if (lane == 0) ws.part[blockIdx.x].rows = 0;
         __syncwarp();
         // lane l: box l / (D / 64) of the tile's 64-value half l % (D / 64)
@@ -618,14 +631,13 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             }
             ++seg;
             if (g.nt == 0) break;
-            for (int h = 0; h < F::kQHalves; ++h, ++loads, kt.step(ly.nk)) {
-                constexpr int per = F::kSlot / 16384;               // boxes of 128 bytes a row
+            for (int h = 0; h < F::kQSlots; ++h, ++loads, kt.step(ly.nk)) {
                 if (loads >= ly.nk && !(ok = warp_wait(bar(fx.k_empty[kt.slot]), kt.parity ^ 1))) break;
-                if (lane == 0) tc::mbar_expect_tx(bar(fx.k_full[kt.slot]), per * ly.q_rows * 128);
+                if (lane == 0) tc::mbar_expect_tx(bar(fx.k_full[kt.slot]), F::kQPer * ly.q_rows * 128);
                 __syncwarp();
-                if (lane < per)
-                    tma_load_3d(tc::smem_u32(k_s + kt.slot * F::kSlot + lane * 16384), &tm_q,
-                                (h * per + lane) * (128 / (int)sizeof(T)), g.kvh * G, g.first + g.r0 / G, bar(fx.k_full[kt.slot]));
+                if (lane < F::kQPer)
+                    tma_load_3d(tc::smem_u32(k_s + kt.slot * F::kSlot + lane * F::kQBox), &tm_q,
+                                (h * F::kQPer + lane) * (128 / (int)sizeof(T)), g.kvh * G, g.first + g.r0 / G, bar(fx.k_full[kt.slot]));
             }
             if (!ok) break;
             // rows of the cache that 32 boxes start at (those of several tiles), one a lane, a
@@ -691,7 +703,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             while (ok && wait(fx.seg_full[seg & 3], (seg >> 2) & 1)) {
                 const int nt = *reinterpret_cast<volatile int *>(&fx.seg[seg & 3].nt);
                 if (nt == 0 || !wait(fx.q_full, seg & 1)) break;
-                for (int h = 0; h < F::kQHalves; ++h, kt.step(ly.nk)) mbar_arrive(bar(fx.k_empty[kt.slot]));
+                for (int h = 0; h < F::kQSlots; ++h, kt.step(ly.nk)) mbar_arrive(bar(fx.k_empty[kt.slot]));
                 for (int k = 0; k < nt; ++k, ++i) {
                     const int b = i & 1;
                     if (i >= 2 && !wait(fx.s_free[b], ((i >> 1) - 1) & 1)) break;
@@ -770,13 +782,13 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             if (!(ok = warp_wait(bar(fx.seg_full[n & 3]), (n >> 2) & 1))) return;
             if (fx.seg[n & 3].nt == 0) return;
             if (n > 0 && !(ok = warp_wait(bar(fx.q_empty), (n - 1) & 1))) return;
-            const unsigned char *slot[2];
-            for (int h = 0; h < F::kQHalves; ++h, qt.step(ly.nk)) {
+            const unsigned char *slot[F::kQSlots];
+            for (int h = 0; h < F::kQSlots; ++h, qt.step(ly.nk)) {
                 if (!(ok = warp_wait(bar(fx.k_full[qt.slot]), qt.parity))) return;
                 slot[h] = k_s + qt.slot * F::kSlot;
             }
             tc::tc_fence_after();
-            if ((ok = stage_queries<T, C, D>(a, fx, slot, fx.cs[n & 1], tr + kTmQ, wg, row, CAP, n))) mbar_arrive(bar(fx.q_full));
+            if ((ok = stage_queries<T, C, D, CAP>(a, fx, slot, fx.cs[n & 1], tr + kTmQ, wg, row, n))) mbar_arrive(bar(fx.q_full));
         };
         if (ok) queries(0);
         while (ok && next(g)) {
@@ -1220,7 +1232,7 @@ bool map_cache(CUtensorMap *m, const void *base, uint64_t rows, int D, int box, 
 
 // The queries as [rows][heads][values]; a box is 128 bytes of each head of a key
 // head's group, of as many rows as a tile takes.
-bool map_queries(CUtensorMap *m, const TreeArgs &a, size_t bytes) {
+bool map_queries(CUtensorMap *m, const TreeArgs &a, size_t bytes, int q_rows) {
     const EncodeTiled enc = encode_fn();
     if (!enc) return false;
     const int G = a.NH / a.NKV;
@@ -1228,7 +1240,7 @@ bool map_queries(CUtensorMap *m, const TreeArgs &a, size_t bytes) {
     // (of one row, the distance to the next is never used, but has to be one)
     const cuuint64_t row = (cuuint64_t)(a.T > 1 ? a.q_stride : (long)a.NH * a.D) * bytes;
     cuuint64_t strides[2] = {(cuuint64_t)a.D * bytes, row};
-    cuuint32_t bx[3] = {(cuuint32_t)(128 / bytes), (cuuint32_t)G, (cuuint32_t)(kRows / G)};
+    cuuint32_t bx[3] = {(cuuint32_t)(128 / bytes), (cuuint32_t)G, (cuuint32_t)(q_rows / G)};
     cuuint32_t es[3] = {1, 1, 1};
     const CUtensorMapDataType t = bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                   : a.dtype == QVL_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
@@ -1238,7 +1250,7 @@ bool map_queries(CUtensorMap *m, const TreeArgs &a, size_t bytes) {
 
 template <typename T, int D, int CAP>
 Layout layout_for(const TreeArgs &a) {
-    using F = Conf<T, D>;
+    using F = Conf<T, D, CAP>;
     Layout ly{};
     ly.words = (a.max_nodes + 31) / 32;
     ly.box_log2 = 4;
@@ -1246,7 +1258,7 @@ Layout layout_for(const TreeArgs &a) {
     ly.box = 1 << ly.box_log2;
     ly.all = (1u << ((kTile >> ly.box_log2) * (D / 64))) - 1u;
     const int G = a.NH / a.NKV;
-    ly.q_rows = kRows / G * G;
+    ly.q_rows = CAP / G * G;
     ly.anc_bytes = (2 * a.max_nodes * ly.words * 4 + 15) & ~15;
     // (3 + 3 slots where there is room measure as 2 + 2 do)
     const int rest = (((int)sizeof(Fixed) + 1023) & ~1023) + ly.anc_bytes + (CAP < kRows ? 2 * kRows * (D / 2 + 4) * 4 : 0);
@@ -1264,7 +1276,7 @@ cudaError_t launch_cap(const TreeArgs &a, cudaStream_t st) {
     const uint64_t rows = (uint64_t)a.num_pages * a.NKV * a.P;
     const bool bf = a.kv_dtype == QVL_DTYPE_BF16;
     if (!map_cache(&mk, a.k_pages, rows, D, ly.box, bf) || !map_cache(&mv, a.v_pages, rows, D, ly.box, bf) ||
-        !map_queries(&mq, a, sizeof(T)))
+        !map_queries(&mq, a, sizeof(T), ly.q_rows))
         return cudaErrorInvalidValue;
     // no more CTAs than there can be units
     const long qrows = (long)a.max_nodes * (a.NH / a.NKV);
