@@ -20,8 +20,7 @@
 //
 // Warps of a CTA:
 //   TMA      cuts the stretch into segments, finds the pages, fills a ring of slots for K
-//            and one for V (a slot: 128 positions, 128-byte swizzle); a segment's Q goes
-//            through the K ring ahead of its keys
+//            and one for V (a slot: 128 positions, 128-byte swizzle), and loads a segment's Q
 //   MMA      S = Q K^T [128 rows, 128 positions], O = P V [128 rows, D], a thread each, so
 //            that one has its next product ready while the other's is under way.  Q, S, P (over S) and O in tensor memory, so that shared memory, whose
 //            bandwidth the products would need most of otherwise, is read for K and V alone
@@ -261,9 +260,9 @@ struct Conf {
     static constexpr bool kSplitQ = std::is_same<T, float>::value;
     static constexpr int kQHalves = kSplitQ ? 2 : 1;
     static constexpr int kSlot = kTile * D * 2;
-    // The queries come in boxes of CAP rows of 128 bytes, as many as fit to a slot
-    static constexpr int kQBox = CAP * 128, kQBoxes = D * (int)sizeof(T) / 128;
-    static constexpr int kQPer = kQBoxes < kSlot / kQBox ? kQBoxes : kSlot / kQBox, kQSlots = kQBoxes / kQPer;
+    static constexpr int kQBox = CAP * 128, kQBoxes = D * (int)sizeof(T) / 128;      // queries: boxes of 128 bytes a row
+    static constexpr int kPitch = D / 2 * (CAP == 64 ? 1 : 2) / 2 + 4;  // floats of a row that a block hands to the others
+    static constexpr int kBlocks = CAP < kRows ? 2 * kRows * kPitch * 4 : 0;
     static constexpr int kMaxRing = 4;
     static constexpr int kOB = D == 64 ? 2 : 1;             // buffers of O
 };
@@ -285,7 +284,7 @@ struct Fixed {
     float m[2][2][kRows];           // references, by segment and warpgroup
     float qmax[2][kRows];           // maxima of a query row's halves
     Segment seg[4];
-    uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], s_free[2], p_ready[2], o_full[2], o_empty[2], q_full,
+    uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], s_free[2], p_ready[2], o_full[2], o_empty[2], q_load, q_full,
         q_empty, anc_full[2], seg_full[4], seg_empty[4], l_bar[2], seg_done[2], qmax_bar, block_bar[2], fix_ask, fix_done;
     uint32_t valid[8];              // boxes of a tile that exist, by tile
     uint32_t bad[8][4];             // positions with values held back, by tile
@@ -313,11 +312,11 @@ __device__ __forceinline__ Workspace workspace_of(void *p, int D) {
     return w;
 }
 
-// Half of a query row from the K ring's slots (rows of 128 bytes, 128-byte swizzle) into
+// Half of a query row from shared memory (rows of 128 bytes, 128-byte swizzle) into
 // tensor memory (columns of two 16-bit values, hi and then lo) by the thread of the row,
 // and the row's score factor.  False where a wait gave up.
 template <typename T, typename C, int D, int CAP>
-__device__ __forceinline__ bool stage_queries(const TreeArgs &a, Fixed &fx, const unsigned char *const (&slot)[Conf<T, D, CAP>::kQSlots], float *cs_s,
+__device__ __forceinline__ bool stage_queries(const TreeArgs &a, Fixed &fx, const unsigned char *q_s, float *cs_s,
                                               uint32_t tq, int half, int row, int turn) {
     using F = Conf<T, D, CAP>;
     constexpr int H = D / 2, V = 16 / sizeof(T);             // values of 16 bytes
@@ -326,7 +325,7 @@ __device__ __forceinline__ bool stage_queries(const TreeArgs &a, Fixed &fx, cons
     // values [c, c + V) of the half
     auto load = [&](int c, float (&x)[V]) {
         const int byte = (half * H + c) * (int)sizeof(T), chunk = byte >> 7;
-        const unsigned char *p = (chunk < F::kQPer ? slot[0] : slot[F::kQSlots - 1]) + chunk % F::kQPer * F::kQBox;
+        const unsigned char *p = q_s + chunk * F::kQBox;
         const uint4 v = *reinterpret_cast<const uint4 *>(p + src * 128 + ((((byte >> 4) & 7) ^ (src & 7)) << 4));
         const T *t = reinterpret_cast<const T *>(&v);
 #pragma unroll
@@ -452,10 +451,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
     constexpr int kHead = ((int)sizeof(Fixed) + 1023) & ~1023;
     unsigned char *k_s = smem + kHead;                              // slots of K, of V
     unsigned char *v_s = k_s + ly.nk * F::kSlot;
-    uint32_t *anc_s = reinterpret_cast<uint32_t *>(v_s + ly.nv * F::kSlot);     // [2][node][words], by segment
+    unsigned char *q_s = v_s + ly.nv * F::kSlot;                    // a segment's queries
+    uint32_t *anc_s = reinterpret_cast<uint32_t *>(q_s + F::kQBoxes * F::kQBox);    // [2][node][words], by segment
     // the blocks' sums, to be added: [half of D][row][pitch]
-    constexpr int kPitch = D / 2 + 4;
-    float *blocks_s = reinterpret_cast<float *>(v_s + ly.nv * F::kSlot + ly.anc_bytes);
+    float *blocks_s = reinterpret_cast<float *>(q_s + F::kQBoxes * F::kQBox + ly.anc_bytes);
     auto bar = [](uint64_t &b) { return tc::smem_u32(&b); };
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -480,6 +479,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             tc::mbar_init(bar(fx.l_bar[i]), 256);
             tc::mbar_init(bar(fx.seg_done[i]), 16);
         }
+        tc::mbar_init(bar(fx.q_load), 1);
         tc::mbar_init(bar(fx.q_full), 256);
         tc::mbar_init(bar(fx.q_empty), 1);
         tc::mbar_init(bar(fx.qmax_bar), 8);
@@ -589,7 +589,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
         const int oob = (int)(a.num_pages * a.NKV * a.P);          // past the last row: zeros
         const int to = half * (kTile * 128) + bx * ly.box * 128;
         Turn kt, vt;
-        int loads = 0;                                             // slots of the K ring filled
+        int keys = 0;                                              // loads of K so far
+        int queries = 0;                                           // and of queries
         uint64_t once;
         asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(once));
         while (ok) {
@@ -631,15 +632,14 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             }
             ++seg;
             if (g.nt == 0) break;
-            for (int h = 0; h < F::kQSlots; ++h, ++loads, kt.step(ly.nk)) {
-                if (loads >= ly.nk && !(ok = warp_wait(bar(fx.k_empty[kt.slot]), kt.parity ^ 1))) break;
-                if (lane == 0) tc::mbar_expect_tx(bar(fx.k_full[kt.slot]), F::kQPer * ly.q_rows * 128);
-                __syncwarp();
-                if (lane < F::kQPer)
-                    tma_load_3d(tc::smem_u32(k_s + kt.slot * F::kSlot + lane * F::kQBox), &tm_q,
-                                (h * F::kQPer + lane) * (128 / (int)sizeof(T)), g.kvh * G, g.first + g.r0 / G, bar(fx.k_full[kt.slot]));
-            }
-            if (!ok) break;
+            // (the place is free when the queries before are in tensor memory)
+            if (seg > 1 && !(ok = warp_wait(bar(fx.q_full), seg & 1))) break;
+            if (lane == 0) tc::mbar_expect_tx(bar(fx.q_load), F::kQBoxes * ly.q_rows * 128);
+            __syncwarp();
+            if (lane < F::kQBoxes)
+                tma_load_3d(tc::smem_u32(q_s + lane * F::kQBox), &tm_q, lane * (128 / (int)sizeof(T)), g.kvh * G,
+                            g.first + g.r0 / G, bar(fx.q_load));
+            ++queries;
             // rows of the cache that 32 boxes start at (those of several tiles), one a lane, a
             // group ahead: behind the loads of K and V an answer takes microseconds
             const int nb = kTile >> ly.box_log2, group = 32 / nb;
@@ -659,7 +659,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                 int y = __shfl_sync(~0u, rows_now, (k % group * nb + bx) & 31);
                 if (lane >= lanes) y = oob;
                 const uint32_t there = __ballot_sync(~0u, y != oob);
-                if (loads >= ly.nk && !(ok = warp_wait(bar(fx.k_empty[kt.slot]), kt.parity ^ 1))) break;
+                if (i >= ly.nk && !(ok = warp_wait(bar(fx.k_empty[kt.slot]), kt.parity ^ 1))) break;
                 if (lane == 0) {
                     // (keys are loaded at most nk + 2 tiles ahead of the softmax
                     // that reads this)
@@ -670,7 +670,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                 if (lane < lanes)
                     tma_load_once(tc::smem_u32(k_s + kt.slot * F::kSlot + to), &tm_k, half * 64, y, bar(fx.k_full[kt.slot]), once);
                 kt.step(ly.nk);
-                ++loads;
+                ++keys;
                 if (i >= ly.nv && !(ok = warp_wait(bar(fx.v_empty[vt.slot]), vt.parity ^ 1))) break;
                 if (lane == 0) tc::mbar_expect_tx(bar(fx.v_full[vt.slot]), F::kSlot);
                 __syncwarp();
@@ -689,7 +689,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
         // after a wait that gave up: loads in flight land before the CTA ends
         // (each slot's last load; a slot never filled has nothing in flight)
         if (!ok) {
-            for (int n = 0; n < min(loads, ly.nk); ++n) tc::mbar_wait(bar(fx.k_full[n]), (((loads - 1 - n) / ly.nk) & 1), nullptr);
+            if (queries > 0) tc::mbar_wait(bar(fx.q_load), (queries - 1) & 1, nullptr);
+            for (int n = 0; n < min(keys, ly.nk); ++n) tc::mbar_wait(bar(fx.k_full[n]), (((keys - 1 - n) / ly.nk) & 1), nullptr);
             for (int n = 0; n < min(i, ly.nv); ++n) tc::mbar_wait(bar(fx.v_full[n]), (((i - 1 - n) / ly.nv) & 1), nullptr);
         }
     } else if (warp == kScoreWarp) {
@@ -703,7 +704,6 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             while (ok && wait(fx.seg_full[seg & 3], (seg >> 2) & 1)) {
                 const int nt = *reinterpret_cast<volatile int *>(&fx.seg[seg & 3].nt);
                 if (nt == 0 || !wait(fx.q_full, seg & 1)) break;
-                for (int h = 0; h < F::kQSlots; ++h, kt.step(ly.nk)) mbar_arrive(bar(fx.k_empty[kt.slot]));
                 for (int k = 0; k < nt; ++k, ++i) {
                     const int b = i & 1;
                     if (i >= 2 && !wait(fx.s_free[b], ((i >> 1) - 1) & 1)) break;
@@ -777,18 +777,13 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
         const uint32_t tr = tmem + ((uint32_t)(w4 * 32) << 16), sb = tr + wg * kTile;
         const Segment *g;
         // the queries of segment n, after the products with those before them
-        Turn qt;
         auto queries = [&](int n) {
             if (!(ok = warp_wait(bar(fx.seg_full[n & 3]), (n >> 2) & 1))) return;
             if (fx.seg[n & 3].nt == 0) return;
             if (n > 0 && !(ok = warp_wait(bar(fx.q_empty), (n - 1) & 1))) return;
-            const unsigned char *slot[F::kQSlots];
-            for (int h = 0; h < F::kQSlots; ++h, qt.step(ly.nk)) {
-                if (!(ok = warp_wait(bar(fx.k_full[qt.slot]), qt.parity))) return;
-                slot[h] = k_s + qt.slot * F::kSlot;
-            }
+            if (!(ok = warp_wait(bar(fx.q_load), n & 1))) return;
             tc::tc_fence_after();
-            if ((ok = stage_queries<T, C, D, CAP>(a, fx, slot, fx.cs[n & 1], tr + kTmQ, wg, row, n))) mbar_arrive(bar(fx.q_full));
+            if ((ok = stage_queries<T, C, D, CAP>(a, fx, q_s, fx.cs[n & 1], tr + kTmQ, wg, row, n))) mbar_arrive(bar(fx.q_full));
         };
         if (ok) queries(0);
         while (ok && next(g)) {
@@ -799,16 +794,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             const int r = row & (cap - 1);          // the row, in its block
             const bool active = (w4 * 32 & (cap - 1)) < sg.rows;
             const int c0 = row / cap * nc;          // the block's first chunk
-            const bool last = ((i + nt - 1) & 1) == wg;
             float m = -INFINITY, l = 0.0f;
             for (int k = 0; k < nt; ++k, ++i) {
-                qt.step(ly.nk);
-                // the next segment's queries as soon as this one's last scores are made, so
-                // that its first ones are made beside this one's last probabilities
-                if (k == nt - 1 && last) {
-                    queries(seg + 1);
-                    if (!ok) break;
-                }
                 if ((i & 1) != wg) continue;
                 if (!(ok = warp_wait(bar(fx.s_full[wg]), (i >> 1) & 1))) break;
                 tc::tc_fence_after();
@@ -909,7 +896,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                 tc::tc_fence_before();
                 mbar_arrive(bar(fx.p_ready[wg]));
             }
-            if (ok && !last) queries(seg + 1);
+            // (one warpgroup is through with the segment a tile before the other)
+            if (ok) queries(seg + 1);
             if (!ok || (seg > 1 && !(ok = warp_wait(bar(fx.seg_done[seg & 1]), ((seg >> 1) - 1) & 1)))) break;
             fx.l[seg & 1][wg][row] = l;
             fx.m[seg & 1][wg][row] = m;
@@ -1056,24 +1044,49 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                     if (lane == 0) mbar_arrive(bar(fx.block_bar[half]));
                     return ok = warp_wait(bar(fx.block_bar[half]), meets++ & 1);
                 };
-                float *mine_s = blocks_s + (half * kRows + row) * kPitch;
+                float *mine_s = blocks_s + (half * kRows + row) * F::kPitch;
                 if (!meet()) break;                 // (the segment before this one is read)
+                if constexpr (nb == 2) {
+                    // (each block hands over the other's share alone: there is room for no more)
 #pragma unroll
-                for (int c = 0; c < CW; c += 4)
-                    *reinterpret_cast<float4 *>(mine_s + c) = make_float4(acc[c] * f, acc[c + 1] * f, acc[c + 2] * f, acc[c + 3] * f);
+                    for (int c = 0; c < share; ++c) {
+                        const float keep = (mine ? acc[share + c] : acc[c]) * f;
+                        acc[share + c] = (mine ? acc[c] : acc[share + c]) * f;
+                        acc[c] = keep;
+                    }
+#pragma unroll
+                    for (int c = 0; c < share; c += 4)
+                        *reinterpret_cast<float4 *>(mine_s + c) = make_float4(acc[share + c], acc[share + c + 1], acc[share + c + 2], acc[share + c + 3]);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < CW; c += 4)
+                        *reinterpret_cast<float4 *>(mine_s + c) = make_float4(acc[c] * f, acc[c + 1] * f, acc[c + 2] * f, acc[c + 3] * f);
+                }
                 if (!meet()) break;
                 if (r < sg.rows) {
-                    const float *from = blocks_s + (half * kRows + r) * kPitch;
-#pragma unroll 1
-                    for (int c = mine * share; c < (mine + 1) * share; c += 4) {
-                        float4 v = *reinterpret_cast<const float4 *>(from + c);
-#pragma unroll
-                        for (int b = 1; b < nb; ++b) {
-                            const float4 w = *reinterpret_cast<const float4 *>(from + b * cap * kPitch + c);
-                            v = make_float4(v.x + w.x, v.y + w.y, v.z + w.z, v.w + w.w);
-                        }
+                    auto put = [&](int c, const float4 &v) {
                         if (part < 0) store4(o + c, v, l == 0.0f, inv);
                         else *reinterpret_cast<float4 *>(ws.acc + at * D + half * CW + c) = v;
+                    };
+                    const float *from = blocks_s + (half * kRows + r) * F::kPitch;
+                    if constexpr (nb == 2) {
+                        from += (mine ^ 1) * cap * F::kPitch;
+#pragma unroll
+                        for (int c = 0; c < share; c += 4) {
+                            const float4 w = *reinterpret_cast<const float4 *>(from + c);
+                            put(mine * share + c, make_float4(acc[c] + w.x, acc[c + 1] + w.y, acc[c + 2] + w.z, acc[c + 3] + w.w));
+                        }
+                    } else {
+#pragma unroll
+                        for (int c = mine * share; c < (mine + 1) * share; c += 4) {
+                            float4 v = *reinterpret_cast<const float4 *>(from + c);
+#pragma unroll
+                            for (int b = 1; b < nb; ++b) {
+                                const float4 w = *reinterpret_cast<const float4 *>(from + b * cap * F::kPitch + c);
+                                v = make_float4(v.x + w.x, v.y + w.y, v.z + w.z, v.w + w.w);
+                            }
+                            put(c, v);
+                        }
                     }
                 }
                 if (!ok) break;
@@ -1261,7 +1274,7 @@ Layout layout_for(const TreeArgs &a) {
     ly.q_rows = CAP / G * G;
     ly.anc_bytes = (2 * a.max_nodes * ly.words * 4 + 15) & ~15;
     // (3 + 3 slots where there is room measure as 2 + 2 do)
-    const int rest = (((int)sizeof(Fixed) + 1023) & ~1023) + ly.anc_bytes + (CAP < kRows ? 2 * kRows * (D / 2 + 4) * 4 : 0);
+    const int rest = (((int)sizeof(Fixed) + 1023) & ~1023) + ly.anc_bytes + F::kBlocks + F::kQBoxes * F::kQBox;
     const int slots = std::min(2 * F::kMaxRing, (227 * 1024 - rest) / F::kSlot);
     ly.nk = slots / 2;
     ly.nv = slots - ly.nk;
