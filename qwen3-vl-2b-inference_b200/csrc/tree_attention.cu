@@ -61,7 +61,10 @@ namespace {
 constexpr int kTile = 128;              // positions per tile
 constexpr int kRows = 128;              // query rows per tile
 constexpr int kSMs = 148;
-constexpr int kThreads = 20 * 32;       // 96 registers each
+// 96 registers each at launch, 61440 in all; the last four warps hand 32 of each of their
+// threads to the softmax's and the sums': 512 * 104 + 128 * 64 = 61440
+constexpr int kThreads = 20 * 32;
+constexpr int kMoreRegs = 104, kRestRegs = 64;
 constexpr int kSumWarp = 8, kTmaWarp = 16, kScoreWarp = 17, kOutWarp = 18;          // the fixer is the last one
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kPBias = 8.0f;          // p is held times 2^8: its low half stays normal
@@ -136,6 +139,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 // 2^(m - top) of what was held under the reference m <= top, which may be -inf both.
 __device__ __forceinline__ float weight(float m, float top) { return m == top ? 1.0f : ex2(m - top); }
+template <int N> __device__ __forceinline__ void regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 // A whole warp's wait: false for all lanes where one gave up.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
     return __all_sync(~0u, tc::mbar_wait(bar, parity, &g_tree_timeout));
@@ -519,6 +524,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
     };
 
     if (warp == kTmaWarp) {
+        regs_less<kRestRegs>();
         // ---- segments, pages and loads ----
         // this CTA's stretch of all units: [lo, hi), found among the requests 32 at a time
         // (sums over the requests up to each lane's; of up to 32 requests they stay)
@@ -694,6 +700,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             for (int n = 0; n < min(i, ly.nv); ++n) tc::mbar_wait(bar(fx.v_full[n]), (((i - 1 - n) / ly.nv) & 1), nullptr);
         }
     } else if (warp == kScoreWarp) {
+        regs_less<kRestRegs>();
         // ---- scores.  Low halves first: what they add up to is small, and exact beside
         // the roundings of the high halves' sums ----
         if (lane == 0) {
@@ -728,6 +735,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             }
         }
     } else if (warp == kOutWarp) {
+        regs_less<kRestRegs>();
         // ---- outputs ----
         if (lane == 0) {
             constexpr uint32_t id = idesc_16<C>(D, true);
@@ -772,6 +780,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             }
         }
     } else if (warp < kSumWarp) {
+        regs_more<kMoreRegs>();
         // ---- softmax: thread = row, the tiles of this warpgroup's parity ----
         const int wg = warp >> 2, w4 = warp & 3, row = tid & 127;
         const uint32_t tr = tmem + ((uint32_t)(w4 * 32) << 16), sb = tr + wg * kTile;
@@ -906,6 +915,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             done();
         }
     } else if (warp < kTmaWarp) {
+        regs_more<kMoreRegs>();
         // ---- output sums: thread = row, half of the head's values ----
         constexpr int CW = D / 2;
         const int half = (warp - kSumWarp) >> 2, w4 = warp & 3, row = tid & 127;
@@ -1097,6 +1107,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             done();
         }
     } else {
+        regs_less<kRestRegs>();
         // ---- values of tiles that hold drafted tokens or end the context: rows past
         // the end are zeroed; of the drafted ones, which some rows do not see,
         // what is not finite would reach every row through 0 * v: it is taken out
