@@ -269,7 +269,13 @@ struct Conf {
     static constexpr int kPitch = D / 2 * (CAP == 64 ? 1 : 2) / 2 + 4;  // floats of a row that a block hands to the others
     static constexpr int kBlocks = CAP < kRows ? 2 * kRows * kPitch * 4 : 0;
     static constexpr int kMaxRing = 4;
-    static constexpr int kOB = D == 64 ? 2 : 1;             // buffers of O
+    // Buffers of scores.  With three a warpgroup finds its next tile's scores made when it is through
+    // with a tile; with two they wait for its probabilities' product (12 requests of
+    // 132 rows over 6000 positions, D 64: 38 and 42 us).  At D 128 there is no room for a third.
+    static constexpr int kNS = D == 64 ? 3 : 2;
+    // tensor memory columns: scores and probabilities (128 each), O, Q
+    static constexpr uint32_t kTmO = kNS * kTile, kTmQ = kTmO + D;
+    static_assert(kTmQ + kQHalves * D / 2 <= 512, "");
 };
 // Shared memory of a launch: what an SM has goes to the rings.
 struct Layout {
@@ -289,7 +295,7 @@ struct Fixed {
     float m[2][2][kRows];           // references, by segment and warpgroup
     float qmax[2][kRows];           // maxima of a query row's halves
     Segment seg[4];
-    uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], s_free[2], p_ready[2], o_full[2], o_empty[2], q_load, q_full,
+    uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[3], s_free[3], p_ready[3], o_full, o_empty, q_load, q_full,
         q_empty, anc_full[2], seg_full[4], seg_empty[4], l_bar[2], seg_done[2], qmax_bar, block_bar[2], fix_ask, fix_done;
     uint32_t valid[8];              // boxes of a tile that exist, by tile
     uint32_t bad[8][4];             // positions with values held back, by tile
@@ -297,8 +303,7 @@ struct Fixed {
     uint32_t tmem;
     int off;
 };
-// Tensor memory columns: S/P (128 each, two), O (D: one buffer of 128 or two of 64), Q
-constexpr uint32_t kTmO = 256, kTmQ = 384, kTmCols = 512;
+constexpr uint32_t kTmCols = 512;       // of tensor memory: all
 
 __host__ __device__ constexpr size_t part_floats(int D) { return (size_t)kRows * D; }
 __host__ __device__ constexpr size_t part_bytes(int D) {
@@ -474,16 +479,18 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             tc::mbar_init(bar(fx.seg_full[i]), 1);
             tc::mbar_init(bar(fx.seg_empty[i]), 19);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < F::kNS; ++i) {
             tc::mbar_init(bar(fx.s_full[i]), 1);
             tc::mbar_init(bar(fx.s_free[i]), 1);
             tc::mbar_init(bar(fx.p_ready[i]), 128);
-            tc::mbar_init(bar(fx.o_full[i]), 1);
-            tc::mbar_init(bar(fx.o_empty[i]), 256);
+        }
+        for (int i = 0; i < 2; ++i) {
             tc::mbar_init(bar(fx.anc_full[i]), 1);
             tc::mbar_init(bar(fx.l_bar[i]), 256);
             tc::mbar_init(bar(fx.seg_done[i]), 16);
         }
+        tc::mbar_init(bar(fx.o_full), 1);
+        tc::mbar_init(bar(fx.o_empty), 256);
         tc::mbar_init(bar(fx.q_load), 1);
         tc::mbar_init(bar(fx.q_full), 256);
         tc::mbar_init(bar(fx.q_empty), 1);
@@ -551,7 +558,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
         // added and tiles are quick, one otherwise (32 requests of up to 16 nodes over 4096:
         // 95 us with 0, 93 with 1, 85 with 2, 81 with 4; 12 of 132 rows over 6000: 55, 54,
         // 55, 57).  Where there are fewer tiles than CTAs, each tile gets its own.
-        const int begin = tiles > gridDim.x ? (CAP < kRows ? 4 : 1) : 0;
+        const int begin = tiles > gridDim.x ? (CAP < kRows ? 4 : 2) : 0;
         const long total = tiles + pairs * begin;
         // (fewer units than CTAs: the last CTAs have none, so that a pair's parts
         // are in consecutive CTAs)
@@ -712,8 +719,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                 const int nt = *reinterpret_cast<volatile int *>(&fx.seg[seg & 3].nt);
                 if (nt == 0 || !wait(fx.q_full, seg & 1)) break;
                 for (int k = 0; k < nt; ++k, ++i) {
-                    const int b = i & 1;
-                    if (i >= 2 && !wait(fx.s_free[b], ((i >> 1) - 1) & 1)) break;
+                    const int b = i % F::kNS;
+                    if (i >= F::kNS && !wait(fx.s_free[b], (i / F::kNS - 1) & 1)) break;
                     if (!wait(fx.k_full[kt.slot], kt.parity)) break;
                     tc::tc_fence_after();
                     const uint64_t kb = kd + (uint32_t)(kt.slot * (F::kSlot >> 4));
@@ -722,7 +729,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                     for (int l = F::kQHalves - 1; l >= 0; --l)
 #pragma unroll
                         for (int c = 0; c < D / 16; ++c)
-                            mma_ts(d, tmem + kTmQ + l * (D / 2) + c * 8, kb + ((c >> 2) * (kTile * 8) + (c & 3) * 2), id,
+                            mma_ts(d, tmem + F::kTmQ + l * (D / 2) + c * 8, kb + ((c >> 2) * (kTile * 8) + (c & 3) * 2), id,
                                    l < F::kQHalves - 1 || c ? 1u : 0u);
                     tc::tc_commit(bar(fx.s_full[b]));
                     tc::tc_commit(bar(fx.k_empty[kt.slot]));
@@ -739,7 +746,6 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
         // ---- outputs ----
         if (lane == 0) {
             constexpr uint32_t id = idesc_16<C>(D, true);
-            constexpr int OB = F::kOB;
             const uint64_t vd = sdesc_mn_sw128(tc::smem_u32(v_s), kTile * 128);
             Turn vt;
             auto wait = [&](uint64_t &b, uint32_t parity) { return ok = tc::mbar_wait(bar(b), parity, &g_tree_timeout); };
@@ -749,27 +755,27 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                 const int nt = sg.nt, plain = max(0, sg.ctx / kTile - sg.tile0);      // tiles before the drafted ones
                 if (nt == 0) break;
                 for (int k = 0; k < nt; ++k, ++i) {
-                    const int b = i & 1, ob = i % OB;
+                    const int b = i % F::kNS;
                     const bool tail = k >= plain;
                     // (the fixer is told one tile ahead: the slot of the tile's V then has its
                     // turn, and it waits for the load itself)
                     if (k == 0 && tail) mbar_arrive(bar(fx.fix_ask));
                     const bool ask = k + 1 < nt && k + 1 >= plain;
                     if (ask && !tail) mbar_arrive(bar(fx.fix_ask));
-                    if (i >= OB && !wait(fx.o_empty[ob], (i / OB - 1) & 1)) break;
+                    if (i >= 1 && !wait(fx.o_empty, (i - 1) & 1)) break;
                     if (!wait(fx.v_full[vt.slot], vt.parity)) break;
                     if (tail && !wait(fx.fix_done, fixes++ & 1)) break;
                     if (ask && tail) mbar_arrive(bar(fx.fix_ask));
-                    if (!wait(fx.p_ready[b], (i >> 1) & 1)) break;
+                    if (!wait(fx.p_ready[b], (i / F::kNS) & 1)) break;
                     tc::tc_fence_after();
                     const uint64_t vb = vd + (uint32_t)(vt.slot * (F::kSlot >> 4));
-                    const uint32_t pb = tmem + b * kTile, d = tmem + kTmO + ob * 64;
+                    const uint32_t pb = tmem + b * kTile, d = tmem + F::kTmO;
 #pragma unroll
                     for (int l = 1; l >= 0; --l)
 #pragma unroll
                         for (int c = 0; c < kTile / 16; ++c)
                             mma_ts(d, pb + c * 16 + l * 8, vb + c * (2048 >> 4), id, l == 0 || c ? 1u : 0u);
-                    tc::tc_commit(bar(fx.o_full[ob]));
+                    tc::tc_commit(bar(fx.o_full));
                     tc::tc_commit(bar(fx.s_free[b]));
                     tc::tc_commit(bar(fx.v_empty[vt.slot]));
                     vt.step(ly.nv);
@@ -783,7 +789,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
         regs_more<kMoreRegs>();
         // ---- softmax: thread = row, the tiles of this warpgroup's parity ----
         const int wg = warp >> 2, w4 = warp & 3, row = tid & 127;
-        const uint32_t tr = tmem + ((uint32_t)(w4 * 32) << 16), sb = tr + wg * kTile;
+        const uint32_t tr = tmem + ((uint32_t)(w4 * 32) << 16);
         const Segment *g;
         // the queries of segment n, after the products with those before them
         auto queries = [&](int n) {
@@ -792,7 +798,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             if (n > 0 && !(ok = warp_wait(bar(fx.q_empty), (n - 1) & 1))) return;
             if (!(ok = warp_wait(bar(fx.q_load), n & 1))) return;
             tc::tc_fence_after();
-            if ((ok = stage_queries<T, C, D, CAP>(a, fx, q_s, fx.cs[n & 1], tr + kTmQ, wg, row, n))) mbar_arrive(bar(fx.q_full));
+            if ((ok = stage_queries<T, C, D, CAP>(a, fx, q_s, fx.cs[n & 1], tr + F::kTmQ, wg, row, n))) mbar_arrive(bar(fx.q_full));
         };
         if (ok) queries(0);
         while (ok && next(g)) {
@@ -806,7 +812,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             float m = -INFINITY, l = 0.0f;
             for (int k = 0; k < nt; ++k, ++i) {
                 if ((i & 1) != wg) continue;
-                if (!(ok = warp_wait(bar(fx.s_full[wg]), (i >> 1) & 1))) break;
+                const int b = i % F::kNS;
+                const uint32_t sb = tr + b * kTile;
+                if (!(ok = warp_wait(bar(fx.s_full[b]), (i / F::kNS) & 1))) break;
                 tc::tc_fence_after();
                 const int t0 = (sg.tile0 + k) * kTile, ctx = sg.ctx;
                 const uint32_t there = *reinterpret_cast<volatile uint32_t *>(&fx.valid[i & 7]);
@@ -903,7 +911,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                 if (moved) fx.ref[i & 3][row] = m;
                 if (lane == 0) fx.moved[i & 3][w4] = moved;
                 tc::tc_fence_before();
-                mbar_arrive(bar(fx.p_ready[wg]));
+                mbar_arrive(bar(fx.p_ready[b]));
             }
             // (one warpgroup is through with the segment a tile before the other)
             if (ok) queries(seg + 1);
@@ -919,7 +927,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
         // ---- output sums: thread = row, half of the head's values ----
         constexpr int CW = D / 2;
         const int half = (warp - kSumWarp) >> 2, w4 = warp & 3, row = tid & 127;
-        const uint32_t to = tmem + ((uint32_t)(w4 * 32) << 16) + kTmO + half * CW;
+        const uint32_t to = tmem + ((uint32_t)(w4 * 32) << 16) + F::kTmO + half * CW;
         T *out = reinterpret_cast<T *>(a.out);
         // rows that no node owns get zeros
         for (int s = blockIdx.x; s < a.S; s += gridDim.x) {
@@ -944,9 +952,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             for (int c = 0; c < CW / 2; ++c) acc2[c] = two(0.0f, 0.0f);
             float top = -INFINITY, f0 = 1.0f, f1 = 1.0f;       // the larger reference; 2^(reference - top) of both
             for (int k = 0; k < nt; ++k, ++i) {
-                constexpr int OB = F::kOB;
-                const int ob = i % OB;
-                if (!(ok = warp_wait(bar(fx.o_full[ob]), (i / OB) & 1))) break;
+                if (!(ok = warp_wait(bar(fx.o_full), i & 1))) break;
                 tc::tc_fence_after();
                 if (active) {
                     // (written before the probabilities, on which the product waited)
@@ -967,7 +973,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
 #pragma unroll
                     for (int c = 0; c < CW; c += 16) {
                         uint32_t v[16];
-                        tc::tmem_ld16(to + ob * 64 + c, v);
+                        tc::tmem_ld16(to + c, v);
                         tmem_wait_ld(v);
 #pragma unroll
                         for (int e = 0; e < 16; e += 2)
@@ -999,7 +1005,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                     }
                 }
                 tc::tc_fence_before();
-                mbar_arrive(bar(fx.o_empty[ob]));
+                mbar_arrive(bar(fx.o_empty));
             }
             if (!ok || !(ok = warp_wait(bar(fx.l_bar[seg & 1]), (seg >> 1) & 1))) break;
             float acc[CW];
