@@ -954,6 +954,12 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             for (int k = 0; k < nt; ++k, ++i) {
                 if (!(ok = warp_wait(bar(fx.o_full), i & 1))) break;
                 tc::tc_fence_after();
+                // O is free for the next product as soon as it is in registers
+                auto read = [&] {
+                    tc::tc_fence_before();
+                    mbar_arrive(bar(fx.o_empty));
+                };
+                if (!active) read();
                 if (active) {
                     // (written before the probabilities, on which the product waited)
                     if (*reinterpret_cast<volatile uint32_t *>(&fx.moved[i & 3][w4])) {
@@ -970,13 +976,16 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                         (i & 1 ? f1 : f0) = weight(m, top);
                     }
                     const uint64_t f = i & 1 ? two(f1, f1) : two(f0, f0);
+                    constexpr int step = D == 64 ? 32 : 16;         // (registers allow no more at D 128)
 #pragma unroll
-                    for (int c = 0; c < CW; c += 16) {
-                        uint32_t v[16];
-                        tc::tmem_ld16(to + c, v);
+                    for (int c = 0; c < CW; c += step) {
+                        uint32_t v[step];
+                        if constexpr (step == 32) tmem_ld32(to + c, v);
+                        else tc::tmem_ld16(to + c, v);
                         tmem_wait_ld(v);
+                        if (c + step == CW) read();
 #pragma unroll
-                        for (int e = 0; e < 16; e += 2)
+                        for (int e = 0; e < step; e += 2)
                             acc2[(c + e) / 2] = fma2(two(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), f, acc2[(c + e) / 2]);
                     }
                     const int t0 = (sg.tile0 + k) * kTile, ctx = sg.ctx;
@@ -1004,8 +1013,6 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                         __syncwarp();
                     }
                 }
-                tc::tc_fence_before();
-                mbar_arrive(bar(fx.o_empty));
             }
             if (!ok || !(ok = warp_wait(bar(fx.l_bar[seg & 1]), (seg >> 1) & 1))) break;
             float acc[CW];
