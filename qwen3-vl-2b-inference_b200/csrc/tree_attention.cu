@@ -22,21 +22,21 @@
 //   TMA      cuts the stretch into segments, finds the pages, fills a ring of slots for K
 //            and one for V (a slot: 128 positions, 128-byte swizzle), and loads a segment's Q
 //   MMA      S = Q K^T [128 rows, 128 positions], O = P V [128 rows, D], a thread each, so
-//            that one has its next product ready while the other's is under way.  Q, S, P (over S) and O in tensor memory, so that shared memory, whose
-//            bandwidth the products would need most of otherwise, is read for K and V alone
+//            that one has its next product ready while the other's is under way.  Q, S, P
+//            (over S) and O in tensor memory, so that shared memory, whose bandwidth the
+//            products would need most of otherwise, is read for K and V alone
 //   softmax  two warpgroups, every other tile each, so that one's waits pass beside the
 //            other's work; thread = row.  A warpgroup's reference of a row (p = 2^(score -
 //            reference)) is left as it is until a score passes it by 2^7, which p held times
 //            2^8 in fp16 allows: almost no tile rescales anything, and scores are
-//            read once.  Between segments they bring the next one's Q to tensor memory
+//            read once.  Between segments they bring the next one's Q to tensor memory.
 //            A tile of at most 32 (64) rows is there four times (twice) over, in as many
 //            blocks of the 128 rows: each block takes its share of the positions and
 //            has p = 0 elsewhere, so that all warps have work, and the blocks are
 //            added at the end like parts of a context
 //   sums     two warpgroups (half of D each) add each tile's O to fp32 registers, times what
-//            its warpgroup's reference is below the largest: the
-//            tensor cores do not round their sums to nearest, so no chain of them is
-//            longer than a tile
+//            its warpgroup's reference is below the largest: the tensor cores do not round
+//            their sums to nearest, so no chain of them is longer than a tile
 //   fixer    the nodes' ancestors as bits, and values of the drafted tile that some
 //            row does not see: 0 * NaN
 // fp32 queries are split q = hi + lo (fp16 each, after a power of two per row
@@ -44,6 +44,22 @@
 // 22 bits in all (bf16: 16): the products of 16-bit values are exact in the tensor
 // cores, so fp32 outputs keep fp32 accuracy and 16-bit ones are rounded once.
 // 16-bit queries are exact as they are.
+//
+// Measured (16 query and 8 key heads of 128, fp16 cache, keys and values read once: 5 TB/s
+// and 4.3 TB/s of the 6.5 that a copy reaches): 16 requests of 64 nodes over up to 32768
+// positions, fp16, 247 us; 32 of 16 nodes over up to 4096, fp32, 73 us, of which
+// tiles take what memory does, and a segment's beginning and end the rest.  In a long
+// row of such calls the board's power limit, not a pipe, sets the time (315 and 92 us, the
+// SMs at 1.4 and 1.5 GHz of 1.97): the products of the low halves are a tenth of it, and
+// those of the 32-row tile's other blocks, which no one reads, a fifth.  12 requests of
+// 132 rows over up to 6000, bf16, heads of 64: 38 us, the softmax's 3400 cycles for a
+// tile of 128 x 128.  One token over 452 positions 13.6 us, 27 nodes over 2011 20 us: latency,
+// the kernel's beginning (5 us: finding the stretch, queries to tensor memory), one tile, and the
+// join (5 us).
+// Tried and not kept: 16 scores a step (4000 cycles a tile for 3000), 64 with the largest
+// found first; scores a step ahead in registers (spills: 318 us for 268);
+// 16-bit queries as an operand from shared memory, with a third buffer of scores at D 128 (no
+// difference); rings of 3 + 3 slots (none).
 //
 // Every wait is bounded (2 s); one that gives up sets this kernel's timeout word,
 // and while it is set the kernel computes nothing (qvl_tc_timeout_status).
@@ -555,9 +571,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             pairs += __shfl_sync(~0u, pairs_to, 31);
         }
         // What a pair costs beside its tiles, in tiles: about four where blocks have to be
-        // added and tiles are quick, one otherwise (32 requests of up to 16 nodes over 4096:
-        // 95 us with 0, 93 with 1, 85 with 2, 81 with 4; 12 of 132 rows over 6000: 55, 54,
-        // 55, 57).  Where there are fewer tiles than CTAs, each tile gets its own.
+        // added and tiles are quick, two otherwise (32 requests of up to 16 nodes over 4096: 82
+        // us with 1, 78 with 2, 79 with 3, 76 with 4, 77 with 6; 16 of 128 rows over 32768 and 12 of
+        // 132 over 6000: 269 and 43.7 with 0, 267 and 42.6 with 1, 265 and 42.7 with 2,
+        // 264 and 43.0 with 3).  Where there are fewer tiles than CTAs, each tile gets its own.
         const int begin = tiles > gridDim.x ? (CAP < kRows ? 4 : 2) : 0;
         const long total = tiles + pairs * begin;
         // (fewer units than CTAs: the last CTAs have none, so that a pair's parts
@@ -674,8 +691,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                 const uint32_t there = __ballot_sync(~0u, y != oob);
                 if (i >= ly.nk && !(ok = warp_wait(bar(fx.k_empty[kt.slot]), kt.parity ^ 1))) break;
                 if (lane == 0) {
-                    // (keys are loaded at most nk + 2 tiles ahead of the softmax
-                    // that reads this)
+                    // (keys are loaded at most nk + 2 tiles, six, ahead of the softmax that
+                    // reads this)
                     fx.valid[i & 7] = there;
                     tc::mbar_expect_tx(bar(fx.k_full[kt.slot]), F::kSlot);
                 }

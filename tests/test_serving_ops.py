@@ -736,3 +736,13 @@ def test_python_refusals(qvl, cuda):
               dict(out=torch.empty_like(m[0], dtype=F16)), dict(positions=i32(m[7])[:0])):
         with pytest.raises(E):
             qvl.qknorm_mrope_kv_append(**args(**o))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("D,nodes", [(64, [150, 3]), (128, [70, 129]), (128, [20, 9])])
+def test_tree_attention_signs_of_the_scale(qvl, cuda, dtype, D, nodes):
+    """A negative scale, and none at all, for tiles of many rows and of few."""
+    c = tree_case(qvl, [333, 700], nodes, 4, 2, D, 32, dtype, seed=D + nodes[0])
+    for scale in (-0.07, 0.0):
+        check_tree(qvl, c, scale=scale)
