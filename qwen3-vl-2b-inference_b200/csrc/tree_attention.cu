@@ -50,8 +50,8 @@
 // positions, fp16, 247 us; 32 of 16 nodes over up to 4096, fp32, 73 us, of which
 // tiles take what memory does, and a segment's beginning and end the rest.  In a long
 // row of such calls the board's power limit, not a pipe, sets the time (315 and 92 us, the
-// SMs at 1.4 and 1.5 GHz of 1.97): the products of the low halves are a tenth of it, and
-// those of the 32-row tile's other blocks, which no one reads, a fifth.  12 requests of
+// SMs at 1.4 and 1.5 GHz of 1.97): the products of p's low halves are a tenth of it, and
+// at 32 rows a fifth goes to the scores' products, of which each block uses a quarter.  12 requests of
 // 132 rows over up to 6000, bf16, heads of 64: 38 us, the softmax's 3400 cycles for a
 // tile of 128 x 128.  One token over 452 positions 13.6 us, 27 nodes over 2011 20 us: latency,
 // the kernel's beginning (5 us: finding the stretch, queries to tensor memory), one tile, and the
