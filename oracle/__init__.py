@@ -52,7 +52,7 @@ _I = ctypes.c_int
 def build(ref: bool = True) -> None:
     """Compile the restatement, and the reference library when its sources exist."""
     subprocess.run(["make", "-C", HERE, "-s", "all"], check=True)
-    if ref and REF_SRC and os.path.isdir(REF_SRC):
+    if ref and REF_SRC and os.path.isfile(os.path.join(REF_SRC, "matmul", "src", "cpu_wrapper.cpp")):
         subprocess.run(["make", "-C", HERE, "-s", "-j8", "ref", f"REF={REF_SRC}"], check=True)
 
 
