@@ -14,8 +14,9 @@
 // them 77 us (4.0 TB/s; 66 us without: one exponential a logit and its conversions take
 // the issue slots at two bytes a logit); 27 rows of fp32 with 20 of them 13.3 us.
 //
-// Sums: a thread's exponentials are taken against a maximum that moves only when a
-// logit passes it by 44, so that almost no load rescales anything.
+// Sums: a thread's exponentials are taken against a reference that moves only when a
+// logit passes it by 8, so that almost no load rescales anything; an exponent of up
+// to 8 is rounded by 8 u, u = 2^-24, which is what its exponential is then off by.
 //
 // Candidates: the pass leaves each thread with the largest of its logits.  A thread whose
 // maximum is passed by k others has nothing among the alternatives; the logits of the
@@ -39,6 +40,7 @@ constexpr int kCand = 1024;
 constexpr int kMaxCluster = 8;
 constexpr int kShare = 128;             // candidates that a slice may hand on unranked
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kFar = 8.0f;
 
 // Value and index as one number, larger where the alternative comes first: by value, then
 // by lower index (both zeros are one value).
@@ -122,7 +124,7 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 }
 // N logits (even); `top` is the largest of them.
 template <int N> __device__ __forceinline__ void take(Stats &t, const float (&x)[N], float top) {
-    if (top > t.m + 44.0f || t.z == 0.0f) t = rebase(t, top == -INFINITY ? 0.0f : top);
+    if (top > t.m + kFar || t.z == 0.0f) t = rebase(t, top == -INFINITY ? 0.0f : top);
     uint64_t z = two(t.z, 0.0f), s = two(t.s, 0.0f);
     const uint64_t m = two(-t.m, -t.m), l = two(kLog2e, kLog2e);
 #pragma unroll

@@ -746,3 +746,41 @@ def test_tree_attention_signs_of_the_scale(qvl, cuda, dtype, D, nodes):
     c = tree_case(qvl, [333, 700], nodes, 4, 2, D, 32, dtype, seed=D + nodes[0])
     for scale in (-0.07, 0.0):
         check_tree(qvl, c, scale=scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,NH,NKV,D,dtype,cache,weights,fused", [
+    (1500, 16, 8, 128, F32, F16, "int8", False), (2100, 5, 1, 64, BF16, BF16, F32, True), (1301, 24, 4, 256, F32, F16, F16, False),
+    (700, 64, 8, 128, F16, F16, None, True)])
+def test_mrope_append_many_tokens(qvl, cuda, T, NH, NKV, D, dtype, cache, weights, fused):
+    """Several tokens to a CTA, among them some without a slot or with a position outside the
+    table; heads in several parts."""
+    case = list(mrope_case(qvl, T, NH, NKV, D, dtype, cache, weights, fused, seed=T))
+    slots, pos = case[6].copy(), case[7].copy()
+    r = np.random.default_rng(T)
+    slots[r.random(T) < 0.1] = -1
+    pos[r.integers(0, 3, 60), r.integers(0, T, 60)] = 300
+    pos[0, -1], pos[2, 0] = -1, 10 ** 9
+    case[6], case[7] = slots, pos
+    check_mrope(qvl, case)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,V,k", [(300, 3001, 7), (700, 513, 64), (1200, 40, 0), (150, 9000, 3)])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_token_logprobs_many_rows(qvl, cuda, T, V, k, dtype):
+    """More rows than there are places for CTAs at a time, and the sizes around that."""
+    g = torch.Generator(device="cuda").manual_seed(T + V)
+    x = (torch.randn((T, V), generator=g, device="cuda") * 4).to(dtype)
+    x[torch.rand((T, V), generator=g, device="cuda") < 0.02] = -float("inf")
+    x[::17] = 1.5                        # rows of one value: more ties than there is room for candidates
+    check_logprobs(qvl, x, torch.arange(T, device="cuda").remainder(V).int(), k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [2, 9, 700])
+def test_token_logprobs_rising_logits(qvl, cuda, V):
+    """Every logit far above those before it, up to 40 at a time: the largest's log-probability is nearly 0."""
+    steps = torch.linspace(0.5, 40, 300, device="cuda")[:, None] * torch.arange(V, device="cuda").remainder(9)
+    for x in (steps, steps.flip(1), steps - 150, steps - steps.amax(1, keepdim=True)):
+        check_logprobs(qvl, x.contiguous(), torch.full((300,), V - 1, dtype=torch.int32, device="cuda"), min(V, 12))
