@@ -590,6 +590,7 @@ def attention_q16(q, kv: PagedKV, seq_ids, positions, max_ctx, out, q_out, q_out
 # time counts: checks are a few attribute reads, and the arguments cross the C ABI as
 # one buffer of 64-bit words.
 _FLOAT_DTYPES = {torch.float32: DTYPE_FP32, torch.float16: DTYPE_FP16, torch.bfloat16: DTYPE_BF16}
+_F32, _I32, _I8 = torch.float32, torch.int32, torch.int8
 _PLAN, _ROPE, _TREE, _LOGPROBS = range(4)
 _WORDS = (struct.Struct("<17q"), struct.Struct("<26qd2q"), struct.Struct("<15qd5q"), struct.Struct("<12q"))
 _serving = None
@@ -633,6 +634,8 @@ def _heads(t: torch.Tensor, T: int, H: int, D: int, what: str):
     contiguous; rows may lie apart."""
     if t.shape != (T, H, D) or not t.is_cuda:
         raise QvlError(f"{what}: expected a CUDA tensor {(T, H, D)}, got {tuple(t.shape)}")
+    if t.is_contiguous():
+        return t.data_ptr(), H * D
     st = t.stride()
     if (st[2] != 1 and D != 1) or (st[1] != D and H != 1):
         raise QvlError(f"{what}: each token's values must be contiguous")
@@ -700,9 +703,11 @@ def _norm_weight(w, D, what):
         return 0, 0, DTYPE_FP32, 0
     if isinstance(w, tuple):
         w, s, group = w
-        if w.dtype is not torch.int8 or s.dtype is not torch.float32 or w.numel() != D or s.numel() * group != D:
+        if w.dtype is not _I8 or s.dtype is not _F32 or w.numel() != D or s.numel() * group != D:
             raise QvlError(f"{what}: expected int8 [{D}] with fp32 scales [{D} / group]")
-        return _addr(w, what), _addr(s, what), DTYPE_INT8, group
+        if not (w.is_cuda and w.is_contiguous() and s.is_cuda and s.is_contiguous()):
+            raise QvlError(f"{what}: expected contiguous CUDA tensors")
+        return w.data_ptr(), s.data_ptr(), DTYPE_INT8, group
     if w.numel() != D:
         raise QvlError(f"{what}: expected {D} weights")
     return _addr(w, what), 0, _dtype(w), 0
@@ -719,21 +724,27 @@ def qknorm_mrope_kv_append(q, k, v, kv: PagedKV, slots, positions, axes, rope_co
     None, a float weight [D] or (int8 weight, fp32 scales, group).  Returns the
     normed, rotated queries (out, or a new tensor; out may be q)."""
     d = kv.dims
-    T, NH, NKV, D, kp, vp = q.shape[0], d.num_heads, d.num_kv_heads, d.head_dim, kv.k, kv.v
-    dt = q.dtype
-    if k.dtype is not dt or v.dtype is not dt or vp.dtype is not kp.dtype:
+    NH, NKV, D, kp, vp = d.num_heads, d.num_kv_heads, d.head_dim, kv.k, kv.v
+    dt, ct, shape = q.dtype, kp.dtype, q.shape
+    T = shape[0]
+    if k.dtype is not dt or v.dtype is not dt or vp.dtype is not ct:
         raise QvlError("q, k and v must have one type, and so must the cache's two halves")
     if out is None:
-        out = torch.empty(q.shape, dtype=dt, device=q.device)
-    elif out.dtype is not dt or out.shape != q.shape:
+        out = torch.empty(shape, dtype=dt, device=q.device)
+    elif out.dtype is not dt or out.shape != shape:
         raise QvlError("out must have q's shape and type")
     at = positions.shape
     if len(at) != 2 or at[1] != T:
         raise QvlError(f"positions: expected [axes, {T}], got {tuple(at)}")
     table = (d.max_pos, D // 2)
-    if rope_cos.shape != table or rope_sin.shape != table or rope_cos.dtype is not torch.float32 or \
-            rope_sin.dtype is not torch.float32:
+    if rope_cos.shape != table or rope_sin.shape != table or rope_cos.dtype is not _F32 or rope_sin.dtype is not _F32:
         raise QvlError(f"rope tables: expected fp32 {table}")
+    if slots.dtype is not _I32 or positions.dtype is not _I32 or axes.dtype is not _I32 or slots.numel() != T or \
+            axes.numel() != D // 2:
+        raise QvlError(f"slots, positions, axes: expected int32 [{T}], [axes, {T}], [{D // 2}]")
+    for t in (out, kp, vp, slots, positions, axes, rope_cos, rope_sin):
+        if not (t.is_cuda and t.is_contiguous()):
+            raise QvlError("out, the pages, slots, positions, axes and the rope tables must be contiguous CUDA tensors")
     qw, qs, wd, g = _norm_weight(q_norm, D, "q_norm")
     kw, ks, wd2, g2 = _norm_weight(k_norm, D, "k_norm")
     if wd != wd2 or g != g2:
@@ -741,10 +752,9 @@ def qknorm_mrope_kv_append(q, k, v, kv: PagedKV, slots, positions, axes, rope_co
     qa, q_st = _heads(q, T, NH, D, "q")
     ka, k_st = _heads(k, T, NKV, D, "k")
     va, v_st = _heads(v, T, NKV, D, "v")
-    _call(_ROPE, "qknorm_mrope_kv_append", qa, ka, va, _dtype(q), q_st, k_st, v_st, _addr(out, "out"), _addr(kp, "k pages"),
-          _addr(vp, "v pages"), _dtype(kp), kp.shape[0], _i32(slots, T, "slots"), _i32(positions, None, "positions"), T,
-          at[0], _i32(axes, D // 2, "axes"), T, _addr(rope_cos, "rope_cos"), _addr(rope_sin, "rope_sin"), qw, qs, kw, ks, wd,
-          g, eps, ctypes.addressof(d), _raw_stream(stream))
+    _call(_ROPE, "qknorm_mrope_kv_append", qa, ka, va, _dtype(q), q_st, k_st, v_st, out.data_ptr(), kp.data_ptr(),
+          vp.data_ptr(), _dtype(kp), kp.shape[0], slots.data_ptr(), positions.data_ptr(), T, at[0], axes.data_ptr(), T,
+          rope_cos.data_ptr(), rope_sin.data_ptr(), qw, qs, kw, ks, wd, g, eps, ctypes.addressof(d), _raw_stream(stream))
     return out
 
 
