@@ -41,6 +41,7 @@ constexpr int kMaxCluster = 8;
 constexpr int kShare = 128;             // candidates that a slice may hand on unranked
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kFar = 8.0f;
+constexpr float kGone = 1000.0f;        // an exponential from this far below is 0
 
 // Value and index as one number, larger where the alternative comes first: by value, then
 // by lower index (both zeros are one value).
@@ -83,7 +84,9 @@ struct Stats {
 };
 __device__ __forceinline__ Stats rebase(const Stats &a, float m) {
     if (a.z == 0.0f || a.m == m) return {m, a.z, a.s};
-    const float d = a.m - m, f = ex2(d * kLog2e);
+    // (from lowest values, as masks write them, the way is so far that z d would pass the type's
+    // range: where f is 0 already, any d will do)
+    const float d = fmaxf(a.m - m, -kGone), f = ex2(d * kLog2e);
     return {m, a.z * f, (a.s + a.z * d) * f};
 }
 __device__ __forceinline__ Stats warp_join(const Stats &t) {
@@ -133,7 +136,7 @@ template <int N> __device__ __forceinline__ void take(Stats &t, const float (&x)
         const float2 y = parts(mul2(d, l)), w = parts(d);
         const uint64_t p = two(ex2(y.x), ex2(y.y));
         z = add2(z, p);                     // (NaN stays in it)
-        s = fma2(p, two(fmaxf(w.x, -1000.0f), fmaxf(w.y, -1000.0f)), s);     // a masked logit: 0, not 0 * inf
+        s = fma2(p, two(fmaxf(w.x, -kGone), fmaxf(w.y, -kGone)), s);     // a masked logit: 0, not 0 * inf
     }
     t.z = parts(z).x + parts(z).y;
     t.s = parts(s).x + parts(s).y;

@@ -784,3 +784,35 @@ def test_token_logprobs_rising_logits(qvl, cuda, V):
     steps = torch.linspace(0.5, 40, 300, device="cuda")[:, None] * torch.arange(V, device="cuda").remainder(9)
     for x in (steps, steps.flip(1), steps - 150, steps - steps.amax(1, keepdim=True)):
         check_logprobs(qvl, x.contiguous(), torch.full((300,), V - 1, dtype=torch.int32, device="cuda"), min(V, 12))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,V", [(4, 4001), (2, 151936), (400, 4001)])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_token_logprobs_lowest_values(qvl, cuda, T, V, dtype):
+    """Logits of the type's lowest value, as masks write them, and others that are as far from the
+    row's largest: finite, without weight, and of no influence on the sums."""
+    g = torch.Generator(device="cuda").manual_seed(V + T)
+    x = (torch.randn((T, V), generator=g, device="cuda") * 3).to(dtype)
+    low = torch.finfo(dtype).min
+    far = torch.tensor(-1e38 if dtype != F16 else -5e4).to(dtype)
+    keep = torch.zeros((6, V), dtype=torch.bool, device="cuda")
+    keep[0, V // 3:] = True                         # a masked prefix
+    keep[1, ::701] = True                           # all but a few, one at most to a load
+    keep[2, :V // 4] = True                         # whole slices and threads of nothing else
+    keep[3, V - 1] = True                           # one logit alone
+    keep[4] = torch.rand(V, generator=g, device="cuda") < 0.5
+    keep[5, :] = True
+    keep[5, 0] = False
+    tok = torch.arange(T, device="cuda").remainder(V).int()
+    for turn in range(0, 6, min(T, 6)):
+        m = keep[(torch.arange(T, device="cuda") + turn) % 6]
+        for masked in (torch.full_like(x, low), torch.full_like(x, float(far)), torch.where(x > 0, low, far).to(dtype)):
+            got = check_logprobs(qvl, torch.where(m, x, masked), tok, 5)
+            assert bool(torch.isfinite(got.entropy).all())
+        # the largest logit further above than the type holds (its own token: the others' log-probabilities
+        # are no fp32 numbers)
+        if dtype != F16:
+            y = torch.where(m, x, torch.full_like(x, low))
+            y[:, V // 2] = 3e38
+            assert not bool(check_logprobs(qvl, y, torch.full_like(tok, V // 2), 1).entropy.any())
