@@ -729,6 +729,9 @@ def qknorm_mrope_kv_append(q, k, v, kv: PagedKV, slots, positions, axes, rope_co
     T = shape[0]
     if k.dtype is not dt or v.dtype is not dt or vp.dtype is not ct:
         raise QvlError("q, k and v must have one type, and so must the cache's two halves")
+    pages = kp.shape
+    if len(pages) != 4 or pages != vp.shape or pages[1:] != (NKV, d.page_size, D):
+        raise QvlError(f"the cache's halves: expected [pages, {NKV}, {d.page_size}, {D}], both of one size")
     if out is None:
         out = torch.empty(shape, dtype=dt, device=q.device)
     elif out.dtype is not dt or out.shape != shape:
@@ -753,7 +756,7 @@ def qknorm_mrope_kv_append(q, k, v, kv: PagedKV, slots, positions, axes, rope_co
     ka, k_st = _heads(k, T, NKV, D, "k")
     va, v_st = _heads(v, T, NKV, D, "v")
     _call(_ROPE, "qknorm_mrope_kv_append", qa, ka, va, _dtype(q), q_st, k_st, v_st, out.data_ptr(), kp.data_ptr(),
-          vp.data_ptr(), _dtype(kp), kp.shape[0], slots.data_ptr(), positions.data_ptr(), T, at[0], axes.data_ptr(), T,
+          vp.data_ptr(), _dtype(kp), pages[0], slots.data_ptr(), positions.data_ptr(), T, at[0], axes.data_ptr(), T,
           rope_cos.data_ptr(), rope_sin.data_ptr(), qw, qs, kw, ks, wd, g, eps, ctypes.addressof(d), _raw_stream(stream))
     return out
 
@@ -773,9 +776,11 @@ def tree_attention(q, kv: PagedKV, ctx_lens, starts, parents, max_ctx, max_nodes
     over an fp16 cache, bf16 over bf16; rows that see nothing get zeros."""
     d = kv.dims
     T, D, kp, vp, table = q.shape[0], d.head_dim, kv.k, kv.v, kv.page_table
-    S = ctx_lens.numel()
-    if table.shape[0] < S or vp.dtype is not kp.dtype:
-        raise QvlError("the page table has fewer rows than there are requests, or the cache has two types")
+    S, shape, pages = ctx_lens.numel(), table.shape, kp.shape
+    if len(shape) != 2 or shape[0] < S or shape[1] != d.max_pages_per_seq:
+        raise QvlError(f"page_table: expected {S} rows of {d.max_pages_per_seq} pages, got {tuple(shape)}")
+    if len(pages) != 4 or pages != vp.shape or pages[1:] != (d.num_kv_heads, d.page_size, D) or vp.dtype is not kp.dtype:
+        raise QvlError(f"the cache's halves: expected [pages, {d.num_kv_heads}, {d.page_size}, {D}], of one size and type")
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     elif out.dtype is not q.dtype or out.shape != q.shape:
@@ -785,7 +790,7 @@ def tree_attention(q, kv: PagedKV, ctx_lens, starts, parents, max_ctx, max_nodes
         nbytes = _tree_bytes[D] = load_library().qvl_tree_attention_workspace_bytes(1, 1, 1, 1, ctypes.byref(d))
     ws = _ws(workspace, q.device).get(nbytes)
     qa, q_st = _heads(q, T, d.num_heads, D, "q")
-    _call(_TREE, "tree_attention", qa, _dtype(q), q_st, _addr(kp, "k pages"), _addr(vp, "v pages"), _dtype(kp), kp.shape[0],
+    _call(_TREE, "tree_attention", qa, _dtype(q), q_st, _addr(kp, "k pages"), _addr(vp, "v pages"), _dtype(kp), pages[0],
           _i32(table, None, "page_table"), _i32(ctx_lens, S, "ctx_lens"), _i32(starts, S + 1, "starts"),
           _i32(parents, T, "parents"), S, T, max_ctx, max_nodes, D ** -0.5 if scale is None else scale, _addr(out, "out"),
           ctypes.addressof(d), ws.data_ptr(), ws.numel(), _raw_stream(stream))

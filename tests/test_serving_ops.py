@@ -816,3 +816,36 @@ def test_token_logprobs_lowest_values(qvl, cuda, T, V, dtype):
             y = torch.where(m, x, torch.full_like(x, low))
             y[:, V // 2] = 3e38
             assert not bool(check_logprobs(qvl, y, torch.full_like(tok, V // 2), 1).entropy.any())
+
+
+@pytest.mark.gpu
+def test_caches_and_page_tables_of_another_shape_are_refused(qvl, cuda):
+    """What the cache's description says has to be what its tensors are: the kernels go by the former."""
+    import types
+    E = qvl.QvlError
+    c = tree_case(qvl, [20], [4], 4, 2, 128, 16, F32, seed=1)
+    a = (i32([20]), i32([0, 4]), i32([-1, 0, 0, 1]))
+    kv = c["kv"]
+    shape = list(kv.k.shape)
+
+    def other(**o):
+        return types.SimpleNamespace(**{**dict(k=kv.k, v=kv.v, page_table=kv.page_table, dims=kv.dims,
+                                               page_size=kv.page_size), **o})
+
+    pages = [torch.zeros([n + (i == j) * by for j, n in enumerate(shape)], dtype=kv.k.dtype, device="cuda")
+             for i, by in ((0, -1), (1, -1), (2, -1), (3, -64))] + [torch.zeros(shape[:3], dtype=kv.k.dtype, device="cuda")]
+    m = mrope_case(qvl, 5, 4, 2, 128, F32, F16, F32, False, 1)
+    rope = (i32(m[6]), i32(m[7]), m[8], m[9], m[10])
+    for i, x in enumerate(pages):
+        for o in (dict(v=x), dict(k=x)) + ((dict(k=x, v=x),) if i else ()):      # (fewer pages in both are a cache)
+            with pytest.raises(E):
+                qvl.tree_attention(c["q"], other(**o), *a, 24, 4)
+            with pytest.raises(E):
+                qvl.qknorm_mrope_kv_append(m[0], m[1], m[2], other(dims=m[3].dims, **o), *rope, m[11][0], m[11][1])
+    t = kv.page_table
+    for x in (t[:, :1].contiguous(), torch.cat([t, t], 1), t[0], t[:0]):
+        with pytest.raises(E):
+            qvl.tree_attention(c["q"], other(page_table=x), *a, 24, 4)
+        with pytest.raises(E):
+            qvl.tree_attention(c["q"], qvl.PagedKV(1, 2 * 16, 4, 2, 128, 16, k=kv.k, v=kv.v, page_table=x), *a, 24, 4)
+    assert bool(torch.isfinite(qvl.tree_attention(c["q"], other(), *a, 24, 4)).all())
