@@ -43,6 +43,10 @@
 // that keeps both in fp16's normal range) and all probabilities p = hi + lo,
 // 22 bits in all (bf16: 16): the products of 16-bit values are exact in the tensor
 // cores, so fp32 outputs keep fp32 accuracy and 16-bit ones are rounded once.
+// Infinities and NaN of keys and values that a row sees: 0 * inf and inf - inf of the halves, and of the
+// other blocks' zeros, make NaN where the definition has an infinity or nothing at all.  They leave a sum
+// that is not finite, for which a row's sums are tested; such outputs are computed
+// once more in plain fp32 (fix_row), after the products or in the joining launch.
 // A p below 2^-22 of its reference is held to 2^-33 of that (fp16's smallest step, times
 // 2^-8), which no sum with a p near 1 in it can show.
 // 16-bit queries are exact as they are.
@@ -155,6 +159,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 // 2^(m - top) of what was held under the reference m <= top, which may be -inf both.
 __device__ __forceinline__ float weight(float m, float top) { return m == top ? 1.0f : ex2(m - top); }
 template <int N> __device__ __forceinline__ void regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -267,6 +272,11 @@ __device__ __forceinline__ Request request_of(const TreeArgs &a, int s) {
     r.row_tiles = (r.n + per - 1) / per;
     return r;
 }
+// Where a CTA's stretch is being cut: request, units into it, and units to go.
+struct Cut {
+    int s, begin;
+    long off, left;
+};
 // A range of the tiles of one pair.  part: -1 whole pair; otherwise the place in
 // the CTA's half of the workspace.
 struct Segment {
@@ -275,8 +285,40 @@ struct Segment {
 // What the joining launch knows of a partial segment.
 struct Part {
     int first, kvh, r0, rows;      // rows 0: nothing
-    int behind, pad;               // the CTAs after this one that have parts of the pair too
+    int behind, s;                 // the CTAs after this one that have parts of the pair too; its request
 };
+// The next segment of a stretch (false at its end), and the pair's units behind it.
+__device__ __forceinline__ bool next_segment(const TreeArgs &a, int q_rows, Cut &c, Request &rq, Segment &g, int &behind) {
+    while (c.left > 0) {
+        while (c.off >= rq.units(a.NKV, c.begin)) {
+            c.off -= rq.units(a.NKV, c.begin);
+            rq = request_of(a, ++c.s);
+        }
+        // key head, then tile of rows, then the units of the pair
+        const int len = rq.tiles + c.begin;
+        const int pair = c.off < 1l << 31 ? (int)((uint32_t)c.off / (uint32_t)len) : (int)(c.off / len);
+        const int u0 = (int)(c.off - (long)pair * len), u1 = (int)min((long)u0 + c.left, (long)len);
+        c.off += u1 - u0;
+        c.left -= u1 - u0;
+        g.tile0 = max(u0 - c.begin, 0);
+        g.nt = max(u1 - c.begin, 0) - g.tile0;
+        if (g.nt <= 0) continue;                           // ended before the pair's first tile
+        g.s = c.s;
+        g.kvh = pair / rq.row_tiles;
+        g.r0 = (pair - g.kvh * rq.row_tiles) * q_rows;
+        g.rows = min(q_rows, rq.n * (a.NH / a.NKV) - g.r0);
+        g.ctx = rq.ctx;
+        g.L = rq.L;
+        g.first = rq.first;
+        g.n = rq.n;
+        const bool starts = g.tile0 == 0, ends = g.tile0 + g.nt == rq.tiles;
+        g.part = starts && ends ? -1 : starts ? 1 : 0;
+        behind = len - u1;
+        return true;
+    }
+    g.nt = 0;
+    return false;
+}
 
 template <typename T, int D, int CAP>
 struct Conf {
@@ -313,6 +355,8 @@ struct Fixed {
     float m[2][2][kRows];           // references, by segment and warpgroup
     float qmax[2][kRows];           // maxima of a query row's halves
     Segment seg[4];
+    Cut cut;                        // the whole stretch
+    int again;                      // some output of a whole pair is not finite
     uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[3], s_free[3], p_ready[3], o_full, o_empty, q_load, q_full,
         q_empty, anc_full[2], seg_full[4], seg_empty[4], l_bar[2], seg_done[2], qmax_bar, block_bar[2], fix_ask, fix_done;
     uint32_t valid[8];              // boxes of a tile that exist, by tile
@@ -438,6 +482,82 @@ __device__ __forceinline__ uint32_t seen_word(const uint32_t *anc, int words, in
     }
     return L - t0 < 32 ? m & ((1u << (L - t0)) - 1u) : m;
 }
+// Outputs of one row (node, head h of the key head's group) that are not finite, by a warp and by
+// definition in fp32: of a score that is NaN or inf, NaN; a score of -inf has no weight, every other one a
+// weight above 0 (it may meet an infinite value), and a row without weights is 0.  A plain loop: 32
+// positions at a time, a lane each for their scores.  Outputs that are finite stay as they are.
+template <typename T, typename C, int D>
+__device__ __forceinline__ void fix_row(const TreeArgs &a, int s, int ctx, int L, int first, int kvh, int node, int h, int lane) {
+    constexpr int E = D / 32;
+    const long at = (((long)first + node) * a.NH + (long)kvh * (a.NH / a.NKV) + h) * D;
+    T *out = reinterpret_cast<T *>(a.out) + at + lane * E;
+    const T *q = reinterpret_cast<const T *>(a.q) + ((long)first + node) * a.q_stride + ((long)kvh * (a.NH / a.NKV) + h) * D;
+    bool odd = false;
+#pragma unroll
+    for (int e = 0; e < E; ++e) odd |= !finite(to_f32(out[e]));
+    if (!__any_sync(~0u, odd)) return;
+    // the node and its ancestors: lane l has nodes 32 l to 32 l + 31
+    uint32_t mine = 0;
+    for (int j = node; j >= 0;) {
+        if (lane == (j >> 5)) mine |= 1u << (j & 31);
+        const int p = a.parents[first + j];
+        j = p < j ? p : -1;
+    }
+    // row of the cache that holds position t, or -1: not seen, or on no page
+    auto row_of = [&](int t) -> long {
+        const int j = t - ctx;
+        const uint32_t w = __shfl_sync(~0u, mine, max(j, 0) >> 5);
+        if (t >= L || (j >= 0 && !((w >> (j & 31)) & 1u))) return -1;
+        const int pg = a.table[(size_t)s * a.maxp + t / a.P];
+        return pg >= 0 && pg < a.num_pages ? ((long)pg * a.NKV + kvh) * a.P + t % a.P : -1;
+    };
+    const C *kp = reinterpret_cast<const C *>(a.k_pages), *vp = reinterpret_cast<const C *>(a.v_pages);
+    auto score = [&](long r) {
+        if (r < 0) return -INFINITY;
+        float x = 0.0f;
+#pragma unroll 4
+        for (int c = 0; c < D; c += 2) {
+            const float2 k = unpack2<C>(*reinterpret_cast<const uint32_t *>(kp + r * D + c));
+            x = fmaf(to_f32(q[c + 1]) * a.scale, k.y, fmaf(to_f32(q[c]) * a.scale, k.x, x));
+        }
+        return x;
+    };
+    float m = -INFINITY, l = 0.0f, acc[E];
+    bool none = false;                          // a score of inf or NaN
+    for (int t = 0; t < L; t += 32) {
+        const float x = score(row_of(t + lane));
+        none |= !(x < INFINITY);
+        m = fmaxf(m, x);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    none = __any_sync(~0u, none);
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+    for (int t = 0; t < L && !none; t += 32) {
+        const long r = row_of(t + lane);
+        const float x = score(r), p = x > -INFINITY ? fmaxf(expf(x - m), 1.175494351e-38f) : 0.0f;
+        l += p;
+        for (uint32_t use = __ballot_sync(~0u, p > 0.0f); use; use &= use - 1) {
+            const int u = __ffs(use) - 1;
+            const float w = __shfl_sync(~0u, p, u);
+            const C *v = vp + __shfl_sync(~0u, r, u) * D + lane * E;
+#pragma unroll
+            for (int e = 0; e < E; e += 2) {
+                const float2 y = unpack2<C>(*reinterpret_cast<const uint32_t *>(v + e));
+                acc[e] = fmaf(w, y.x, acc[e]);
+                acc[e + 1] = fmaf(w, y.y, acc[e + 1]);
+            }
+        }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const float y = none ? NAN : l == 0.0f ? 0.0f : acc[e] / l;
+        if (!finite(to_f32(out[e]))) out[e] = from_f32<T>(y);
+    }
+}
 // A place in a ring of n slots: the slot, and the parity of its turn.
 struct Turn {
     int slot = 0;
@@ -527,7 +647,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
         tc::tmem_relinquish();
     }
     pdl_wait();
-    if (tid == 0) fx.off = *reinterpret_cast<volatile int *>(&g_tree_timeout);
+    if (tid == 0) {
+        fx.off = *reinterpret_cast<volatile int *>(&g_tree_timeout);
+        fx.again = 0;
+    }
 
     tc::tc_fence_before();
     __syncthreads();
@@ -592,9 +715,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
         }
         const long lo = min(each * me + min(me, more), total), hi = min(lo + each + (me < more ? 1 : 0), total);
         int s = 0;
-        long off = lo, left = ok ? hi - lo : 0;
+        long off = lo;
         Request rq{};
-        for (int base = 0; left > 0; base += 32) {
+        for (int base = 0; ok && hi > lo; base += 32) {
             if (a.S > 32) sums(base);
             const long inc = tiles_to + pairs_to * begin;
             const uint32_t past = __ballot_sync(~0u, inc > off);
@@ -613,7 +736,11 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             }
             off -= __shfl_sync(~0u, inc, 31);
         }
-        if (lane == 0) ws.part[blockIdx.x].rows = 0;
+        Cut cut{s, begin, off, ok ? hi - lo : 0};
+        if (lane == 0) {
+            ws.part[blockIdx.x].rows = 0;
+            fx.cut = cut;
+        }
         __syncwarp();
         // lane l: box l / (D / 64) of the tile's 64-value half l % (D / 64)
         const int lanes = (kTile >> ly.box_log2) * (D / 64);
@@ -627,35 +754,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
         asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(once));
         while (ok) {
             Segment g{};
-            long pair_end = 0;                                     // where the pair's units end, of all
-            while (left > 0) {
-                while (off >= rq.units(a.NKV, begin)) {
-                    off -= rq.units(a.NKV, begin);
-                    rq = request_of(a, ++s);
-                }
-                // key head, then tile of rows, then the units of the pair
-                const int len = rq.tiles + begin;
-                const int pair = off < 1l << 31 ? (int)((uint32_t)off / (uint32_t)len) : (int)(off / len);
-                const int u0 = (int)(off - (long)pair * len), u1 = (int)min((long)u0 + left, (long)len);
-                off += u1 - u0;
-                left -= u1 - u0;
-                g.tile0 = max(u0 - begin, 0);
-                g.nt = max(u1 - begin, 0) - g.tile0;
-                if (g.nt <= 0) continue;                           // ended before the pair's first tile
-                g.s = s;
-                g.kvh = pair / rq.row_tiles;
-                g.r0 = (pair - g.kvh * rq.row_tiles) * ly.q_rows;
-                g.rows = min(ly.q_rows, rq.n * G - g.r0);
-                g.ctx = rq.ctx;
-                g.L = rq.L;
-                g.first = rq.first;
-                g.n = rq.n;
-                const bool starts = g.tile0 == 0, ends = g.tile0 + g.nt == rq.tiles;
-                g.part = starts && ends ? -1 : starts ? 1 : 0;
-                pair_end = hi - left + (len - u1);
-                break;
-            }
-            g.nt = max(g.nt, 0);
+            int behind = 0;                                        // the pair's units after the segment
+            next_segment(a, ly.q_rows, cut, rq, g, behind);
             if (seg >= 4) ok = warp_wait(bar(fx.seg_empty[seg & 3]), ((seg >> 2) - 1) & 1);
             if (!ok) break;
             if (lane == 0) {
@@ -712,10 +812,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             }
             if (g.part == 1 && lane == 0) {
                 // the CTA that has the pair's last unit
-                const long x = pair_end - 1, y = x - more * (each + 1);
+                const long x = hi - cut.left + behind - 1, y = x - more * (each + 1);
                 const long last = total < 1l << 31 ? (y < 0 ? (uint32_t)x / (uint32_t)(each + 1) : more + (uint32_t)y / (uint32_t)each)
                                                    : (y < 0 ? x / (each + 1) : more + y / each);
-                ws.part[blockIdx.x] = {g.first, g.kvh, g.r0, g.rows, (int)(last - me), 0};
+                ws.part[blockIdx.x] = {g.first, g.kvh, g.r0, g.rows, (int)(last - me), g.s};
             }
         }
         // after a wait that gave up: loads in flight land before the CTA ends
@@ -1024,8 +1124,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
 #pragma unroll
                                 for (int c = 0; c < CW; c += 2) {
                                     const float2 y = unpack2<C>(*reinterpret_cast<const volatile uint32_t *>(v + c));
-                                    acc2[c / 2] = add2(acc2[c / 2], two(fabsf(y.x) <= 3.402823466e38f ? 0.0f : y.x,
-                                                                        fabsf(y.y) <= 3.402823466e38f ? 0.0f : y.y));
+                                    acc2[c / 2] = add2(acc2[c / 2], two(finite(y.x) ? 0.0f : y.x, finite(y.y) ? 0.0f : y.y));
                                 }
                             }
                         }
@@ -1052,14 +1151,18 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             T *o = out + ((long)(sg.first + node) * a.NH + sg.kvh * G + h) * D + half * CW;
             const int part = sg.part;
             const size_t at = ((size_t)blockIdx.x * 2 + max(part, 0)) * kRows + r;
-            float m, l;
+            float m, l, odd;        // odd: a sum of all that goes out, not finite where a part of it is not
             if constexpr (cap == kRows) {
                 m = of_row(r, l);
+                odd = l;
                 if (r < sg.rows) {
                     if (part < 0) {
                         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
                         for (int c = 0; c < CW; c += 8) store8(o + c, acc + c, l == 0.0f, inv);
+#pragma unroll
+                        for (int c = 0; c < CW; ++c) odd += acc[c];
+                        if (!finite(odd)) fx.again = 1;
                     } else {
 #pragma unroll
                         for (int c = 0; c < CW; c += 4)
@@ -1081,6 +1184,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                     l += lb * weight(mb, m);
                 }
                 const float f = weight(top, m), inv = l == 0.0f ? 0.0f : 1.0f / l;
+                odd = l;
                 auto meet = [&] {
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar(fx.block_bar[half]));
@@ -1107,6 +1211,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                 if (!meet()) break;
                 if (r < sg.rows) {
                     auto put = [&](int c, const float4 &v) {
+                        odd += (v.x + v.y) + (v.z + v.w);
                         if (part < 0) store4(o + c, v, l == 0.0f, inv);
                         else *reinterpret_cast<float4 *>(ws.acc + at * D + half * CW + c) = v;
                     };
@@ -1130,6 +1235,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                             put(c, v);
                         }
                     }
+                    if (!finite(odd)) fx.again = 1;
                 }
                 if (!ok) break;
             }
@@ -1137,6 +1243,19 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(fx.seg_done[seg & 1]));
             done();
+        }
+        // whole pairs' outputs that are not finite, when nobody waits for these warps any more
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (ok && *reinterpret_cast<volatile int *>(&fx.again)) {
+            Cut cut = fx.cut;
+            Request rq = request_of(a, cut.s);
+            Segment x{};
+            int behind;
+            while (next_segment(a, ly.q_rows, cut, rq, x, behind)) {
+                if (x.part >= 0) continue;
+                for (int y = warp - kSumWarp; y < x.rows; y += 8)
+                    fix_row<T, C, D>(a, x.s, x.ctx, x.L, x.first, x.kvh, (x.r0 + y) / G, (x.r0 + y) % G, lane);
+            }
         }
     } else {
         regs_less<kRestRegs>();
@@ -1200,20 +1319,21 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
 // first part is CTA c's last segment; 16 lanes a row, and four parts' reads on
 // their way at a time (latency is all that counts here).
 constexpr int kJoinRows = 16;
-template <typename T, int D>
+template <typename T, typename C, int D>
 __global__ void __launch_bounds__(16 * kJoinRows) tree_join_kernel(const __grid_constant__ TreeArgs a) {
     pdl_launch_dependents();
     pdl_wait();
     const Workspace ws = workspace_of(a.workspace, D);
     const int col = threadIdx.x & 15, row = blockIdx.y * kJoinRows + (threadIdx.x >> 4), c0 = blockIdx.x;
     const Part p = ws.part[c0];
-    if (row >= p.rows) return;
+    if ((row & ~1) >= p.rows) return;           // (whole warps, of two rows)
+    const bool in = row < p.rows;
     constexpr int E = D / 16, U = 4;
     float acc[E], m = -INFINITY, l = 0.0f;
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.0f;
 #pragma unroll 1
-    for (int k = 0; k <= p.behind; k += U) {
+    for (int k = 0; in && k <= p.behind; k += U) {
         float2 st[U];
         float4 v[U][E / 4];
 #pragma unroll
@@ -1251,9 +1371,22 @@ __global__ void __launch_bounds__(16 * kJoinRows) tree_join_kernel(const __grid_
     const int G = a.NH / a.NKV, node = (p.r0 + row) / G, h = p.r0 + row - node * G;
     T *o = reinterpret_cast<T *>(a.out) + ((long)(p.first + node) * a.NH + p.kvh * G + h) * D + col * 4;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    float odd = l;              // a sum of all, not finite where a part of it is not
+#pragma unroll
+    for (int e = 0; e < E; ++e) odd += acc[e];
 #pragma unroll
     for (int e = 0; e < E / 4; ++e)
-        store4(o + e * 64, make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]), l == 0.0f, inv);
+        if (in) store4(o + e * 64, make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]), l == 0.0f, inv);
+    uint32_t again = __ballot_sync(~0u, in && !finite(odd));
+    if (again) {
+        __syncwarp();
+        const Request rq = request_of(a, p.s);
+        for (int u = 0; u < 2; ++u, again >>= 16)
+            if (again & 0xffffu) {
+                const int y = p.r0 + (row & ~1) + u;
+                fix_row<T, C, D>(a, p.s, rq.ctx, rq.L, p.first, p.kvh, y / G, y % G, threadIdx.x & 31);
+            }
+    }
 }
 
 // ---------------------------------------------------------------- host side
@@ -1363,7 +1496,7 @@ cudaError_t launch_cap(const TreeArgs &a, cudaStream_t st) {
     cfg.gridDim = dim3(ctas, (unsigned)((std::min(qrows, (long)kRows) + kJoinRows - 1) / kJoinRows));
     cfg.blockDim = dim3(16 * kJoinRows);
     cfg.dynamicSmemBytes = 0;
-    return cudaLaunchKernelEx(&cfg, tree_join_kernel<T, D>, a);
+    return cudaLaunchKernelEx(&cfg, tree_join_kernel<T, C, D>, a);
 }
 // Rows of a request that has max_nodes: up to 32 or 64 go in blocks.
 template <typename T, typename C, int D>

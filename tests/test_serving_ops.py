@@ -849,3 +849,76 @@ def test_caches_and_page_tables_of_another_shape_are_refused(qvl, cuda):
         with pytest.raises(E):
             qvl.tree_attention(c["q"], qvl.PagedKV(1, 2 * 16, 4, 2, 128, 16, k=kv.k, v=kv.v, page_table=x), *a, 24, 4)
     assert bool(torch.isfinite(qvl.tree_attention(c["q"], other(), *a, 24, 4)).all())
+
+
+def tree_by_definition(c, scale, G):
+    """The rows of request 0 and the first key head's G heads in 64 bits, of finite and other values: a
+    position whose score is -inf has no weight, every other one a weight above 0, however far its score."""
+    ctx, n, kv = c["ctx"][0], c["nodes"][0], c["kv"]
+    t = torch.arange(ctx + n, device="cuda")
+    page = torch.as_tensor(np.asarray(c["table"])[0], device="cuda")[t // c["P"]]
+    K, V = kv.k[page, 0, t % c["P"]].double(), kv.v[page, 0, t % c["P"]].double()
+    seen = torch.ones((n, ctx + n), dtype=torch.bool, device="cuda")
+    seen[:, ctx:] = torch.from_numpy(ancestors(c["parents"][:n], n)).cuda()
+    out = []
+    for h in range(G):
+        x = (c["q"][:n, h].double()[:, None] * K[None]).sum(-1) * scale
+        x = torch.where(seen, x, -np.inf)
+        nan = torch.isnan(x).any(1) | (x == np.inf).any(1)
+        p = torch.exp(x - x.nan_to_num(0).amax(1, keepdim=True)).clamp_min(1e-300)
+        p = torch.where(x > -np.inf, p, 0.0)
+        y = torch.where((x > -np.inf)[:, :, None], p[:, :, None] * V[None], 0.0).sum(1) / p.sum(1, keepdim=True).clamp_min(1e-300)
+        out.append(torch.where(nan[:, None], np.nan, y))
+    return torch.stack(out, 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("G,D,nodes", [(2, 128, 1), (2, 64, 12), (4, 128, 16), (2, 128, 50), (4, 64, 40)])
+@pytest.mark.parametrize("ctx", [3, 90, 700])
+def test_tree_attention_infinities_that_are_seen(qvl, cuda, dtype, G, D, nodes, ctx):
+    """Infinite values and keys at cached positions, at drafted nodes and at both, in tiles of few rows and
+    of many, whole and in parts: outputs are what the definition says, infinite, NaN or finite."""
+    c = tree_case(qvl, [ctx, 5], [nodes, 2], 2 * G, 2, D, 32, dtype, seed=ctx + nodes, spread=6)
+    scale = D ** -0.5
+    clean = run_tree(qvl, c).clone()
+    base_k, base_v = c["kv"].k.clone(), c["kv"].v.clone()
+
+    def put(x, t, h, col, val):
+        x[int(c["table"][0][t // 32]), h, t % 32, col] = val
+
+    inf = float("inf")
+    last = ctx + nodes - 1
+    plants = [[("v", 0, 3, inf)], [("v", ctx - 1, 7, -inf)], [("v", 1, 3, inf), ("v", 2, 3, -inf), ("v", 1, 9, inf)],
+              [("v", last, D - 1, -inf), ("v", 2, 0, inf)], [("k", 1, 5, inf)], [("k", ctx - 1, 11, -inf)],
+              [("k", last, 2, inf)], [("k", 0, 2, inf), ("v", 0, 6, inf), ("v", ctx - 1, 6, 1.0)],
+              [("v", 2, 4, float("nan"))], [("k", 2, 4, float("nan"))]]
+    for plant in plants:
+        c["kv"].k.copy_(base_k)
+        c["kv"].v.copy_(base_v)
+        for which, t, col, val in plant:
+            put(c["kv"].k if which == "k" else c["kv"].v, t, 0, col, val)
+        got = run_tree(qvl, c)
+        assert torch.equal(got[:, G:], clean[:, G:])                    # the other key head
+        assert torch.equal(got[nodes:], clean[nodes:])                  # the other request
+        got, want = got[:nodes, :G], tree_by_definition(c, scale, G)
+        assert torch.equal(torch.isnan(got), torch.isnan(want)), plant
+        inf_at = torch.isinf(want)
+        assert torch.equal(got.double()[inf_at], want[inf_at]), plant
+        # what is finite: within the bound of finite inputs, here with |q k| and |v| of the finite ones at
+        # most (5.5 sqrt(D))^2 and 5.5
+        fin = torch.isfinite(want)
+        off = (D + 4) * 2 * U * scale * 30 * D
+        lim = (2 * off + 160 * 2 * U) * 5.5 + R[dtype] * want[fin].abs() * (1 + 2.0 ** -8) + 2.0 ** -24
+        assert bool(((got.double() - want).abs()[fin] <= lim).all()), plant
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_tree_attention_scores_of_minus_infinity_alone(qvl, cuda, dtype):
+    """A row whose every score is -inf has no weights, like one that sees nothing: zeros."""
+    c = tree_case(qvl, [4], [3], 2, 1, 64, 16, dtype, seed=3, chain=True)
+    c["q"][..., 0] = c["q"][..., 0].abs() + 1
+    c["kv"].k[int(c["table"][0][0]), 0, :7, 0] = -float("inf")
+    assert not run_tree(qvl, c).any()
+    assert not tree_by_definition(c, 0.125, 2).any()
