@@ -484,17 +484,21 @@ __device__ __forceinline__ uint32_t seen_word(const uint32_t *anc, int words, in
 }
 // Outputs of one row (node, head h of the key head's group) that are not finite, by a warp and by
 // definition in fp32: of a score that is NaN or inf, NaN; a score of -inf has no weight, every other one a
-// weight above 0 (it may meet an infinite value), and a row without weights is 0.  A plain loop: 32
-// positions at a time, a lane each for their scores.  Outputs that are finite stay as they are.
+// weight above 0 (it may meet an infinite value), and a row without weights is 0.  Outputs that are finite
+// stay as they are.  A lane has a position's score, 32 at a time.
+// Where some outputs are finite, the weights are: the others are infinite or NaN by the values
+// alone that are, which are looked for in their columns.  Measured: 16 requests of 64 nodes over 32768
+// positions, every page with a NaN among its values, 12.6 ms (each row anew, two bytes of a key at a time: 326
+// ms); 32 of 16 nodes over 4096, fp32, keys with -inf in them, half the rows anew, 9.1 ms.
 template <typename T, typename C, int D>
 __device__ __forceinline__ void fix_row(const TreeArgs &a, int s, int ctx, int L, int first, int kvh, int node, int h, int lane) {
-    constexpr int E = D / 32;
+    constexpr int E = D / 32, V = 16 / sizeof(T);
     const long at = (((long)first + node) * a.NH + (long)kvh * (a.NH / a.NKV) + h) * D;
     T *out = reinterpret_cast<T *>(a.out) + at + lane * E;
     const T *q = reinterpret_cast<const T *>(a.q) + ((long)first + node) * a.q_stride + ((long)kvh * (a.NH / a.NKV) + h) * D;
-    bool odd = false;
+    uint32_t odd = 0;                           // of this lane's outputs
 #pragma unroll
-    for (int e = 0; e < E; ++e) odd |= !finite(to_f32(out[e]));
+    for (int e = 0; e < E; ++e) odd |= finite(to_f32(out[e])) ? 0u : 1u << e;
     if (!__any_sync(~0u, odd)) return;
     // the node and its ancestors: lane l has nodes 32 l to 32 l + 31
     uint32_t mine = 0;
@@ -508,43 +512,73 @@ __device__ __forceinline__ void fix_row(const TreeArgs &a, int s, int ctx, int L
         const int j = t - ctx;
         const uint32_t w = __shfl_sync(~0u, mine, max(j, 0) >> 5);
         if (t >= L || (j >= 0 && !((w >> (j & 31)) & 1u))) return -1;
-        const int pg = a.table[(size_t)s * a.maxp + t / a.P];
-        return pg >= 0 && pg < a.num_pages ? ((long)pg * a.NKV + kvh) * a.P + t % a.P : -1;
+        const int c = t / a.P, pg = a.table[(size_t)s * a.maxp + c];
+        return pg >= 0 && pg < a.num_pages ? ((long)pg * a.NKV + kvh) * a.P + (t - c * a.P) : -1;
     };
     const C *kp = reinterpret_cast<const C *>(a.k_pages), *vp = reinterpret_cast<const C *>(a.v_pages);
     auto score = [&](long r) {
         if (r < 0) return -INFINITY;
         float x = 0.0f;
 #pragma unroll 4
-        for (int c = 0; c < D; c += 2) {
-            const float2 k = unpack2<C>(*reinterpret_cast<const uint32_t *>(kp + r * D + c));
-            x = fmaf(to_f32(q[c + 1]) * a.scale, k.y, fmaf(to_f32(q[c]) * a.scale, k.x, x));
+        for (int c = 0; c < D; c += V) {
+            const uint4 qv = *reinterpret_cast<const uint4 *>(q + c);
+            uint32_t k[V / 2];
+            if constexpr (V == 8) *reinterpret_cast<uint4 *>(k) = *reinterpret_cast<const uint4 *>(kp + r * D + c);
+            else *reinterpret_cast<uint2 *>(k) = *reinterpret_cast<const uint2 *>(kp + r * D + c);
+#pragma unroll
+            for (int e = 0; e < V; e += 2) {
+                const T *y = reinterpret_cast<const T *>(&qv) + e;
+                const float2 w = unpack2<C>(k[e / 2]);
+                x = fmaf(to_f32(y[1]) * a.scale, w.y, fmaf(to_f32(y[0]) * a.scale, w.x, x));
+            }
         }
         return x;
     };
+    bool whole = !__any_sync(~0u, odd != (1u << E) - 1u);
+    for (int col = 0; col < D && !whole; ++col) {
+        if (!((__shfl_sync(~0u, odd, col / E) >> (col % E)) & 1u)) continue;
+        uint32_t kinds = 0;                     // 1: inf, 2: -inf, 4: NaN
+        for (int t = 0; t < L; t += 128) {
+            long r[4];
+            float v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) r[u] = row_of(t + u * 32 + lane);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[u] = r[u] < 0 ? 0.0f : to_f32(vp[r[u] * D + col]);
+#pragma unroll 1
+            for (int u = 0; u < 4; ++u) {
+                const float x = u == 0 ? v[0] : u == 1 ? v[1] : u == 2 ? v[2] : v[3];
+                if (finite(x)) continue;
+                if (score(u == 0 ? r[0] : u == 1 ? r[1] : u == 2 ? r[2] : r[3]) > -INFINITY) kinds |= x > 0.0f ? 1u : x < 0.0f ? 2u : 4u;
+            }
+        }
+        kinds = __reduce_or_sync(~0u, kinds);
+        whole = kinds == 0;                     // (those found have no weight)
+        if (!whole && lane == col / E) out[col % E] = from_f32<T>(kinds == 1 ? INFINITY : kinds == 2 ? -INFINITY : NAN);
+    }
+    if (!whole) return;
     float m = -INFINITY, l = 0.0f, acc[E];
     bool none = false;                          // a score of inf or NaN
-    for (int t = 0; t < L; t += 32) {
+    for (int t = 0; t < L && !none; t += 32) {
         const float x = score(row_of(t + lane));
-        none |= !(x < INFINITY);
+        none = __any_sync(~0u, !(x < INFINITY));
         m = fmaxf(m, x);
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-    none = __any_sync(~0u, none);
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.0f;
     for (int t = 0; t < L && !none; t += 32) {
         const long r = row_of(t + lane);
         const float x = score(r), p = x > -INFINITY ? fmaxf(expf(x - m), 1.175494351e-38f) : 0.0f;
         l += p;
-        for (uint32_t use = __ballot_sync(~0u, p > 0.0f); use; use &= use - 1) {
-            const int u = __ffs(use) - 1;
+#pragma unroll 8
+        for (int u = 0; u < 32; ++u) {
             const float w = __shfl_sync(~0u, p, u);
             const C *v = vp + __shfl_sync(~0u, r, u) * D + lane * E;
 #pragma unroll
             for (int e = 0; e < E; e += 2) {
-                const float2 y = unpack2<C>(*reinterpret_cast<const uint32_t *>(v + e));
+                const float2 y = unpack2<C>(w > 0.0f ? *reinterpret_cast<const uint32_t *>(v + e) : 0u);
                 acc[e] = fmaf(w, y.x, acc[e]);
                 acc[e + 1] = fmaf(w, y.y, acc[e + 1]);
             }
