@@ -27,8 +27,8 @@
 //            products would need most of otherwise, is read for K and V alone
 //   softmax  two warpgroups, every other tile each, so that one's waits pass beside the
 //            other's work; thread = row.  A warpgroup's reference of a row (p = 2^(score -
-//            reference)) is left as it is until a score passes it by 2^7, which p held times
-//            2^8 in fp16 allows: almost no tile rescales anything, and scores are
+//            reference)) is left as it is until a score passes it by 2^5 (2^7 over bf16), which the way
+//            p is held allows: almost no tile rescales anything, and scores are
 //            read once.  Between segments they bring the next one's Q to tensor memory.
 //            A tile of at most 32 (64) rows is there four times (twice) over, in as many
 //            blocks of the 128 rows: each block takes its share of the positions and
@@ -40,15 +40,13 @@
 //   fixer    the nodes' ancestors as bits, and values of the drafted tile that some
 //            row does not see: 0 * NaN
 // fp32 queries are split q = hi + lo (fp16 each, after a power of two per row
-// that keeps both in fp16's normal range) and all probabilities p = hi + lo,
-// 22 bits in all (bf16: 16): the products of 16-bit values are exact in the tensor
+// that keeps both in fp16's normal range), 22 bits in all, and all probabilities p = hi + lo, 23 bits
+// (bf16: 17; Held): the products of 16-bit values are exact in the tensor
 // cores, so fp32 outputs keep fp32 accuracy and 16-bit ones are rounded once.
 // Infinities and NaN of keys and values that a row sees: 0 * inf and inf - inf of the halves, and of the
 // other blocks' zeros, make NaN where the definition has an infinity or nothing at all.  They leave a sum
 // that is not finite, for which a row's sums are tested; such outputs are computed
 // once more in plain fp32 (fix_row), after the products or in the joining launch.
-// A p below 2^-22 of its reference is held to 2^-33 of that (fp16's smallest step, times
-// 2^-8), which no sum with a p near 1 in it can show.
 // 16-bit queries are exact as they are.
 //
 // Measured (16 query and 8 key heads of 128, fp16 cache, keys and values read once: 5 TB/s
@@ -89,7 +87,25 @@ constexpr int kThreads = 20 * 32;
 constexpr int kMoreRegs = 104, kRestRegs = 64;
 constexpr int kSumWarp = 8, kTmaWarp = 16, kScoreWarp = 17, kOutWarp = 18;          // the fixer is the last one
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kPBias = 8.0f;          // p is held times 2^8: its low half stays normal
+// Probabilities over an fp16 cache.  A reference moves when a score passes it by more than 2^kRise, and p is
+// held times 2^(15 - kRise), so that it fits fp16; the low halves times 2^11 more, which their product
+// takes back (the accumulator goes down by 2^11 before the high halves' product is added).  p is
+// then off by 2^-23 of itself, or by 2^(kRise - 51) of its reference where fp16's smallest step
+// is more: where the largest p meets a value of 0, and the others 2^-29 of it are the output, by
+// 2^-17.  kRise 5: 16 requests of 64 nodes over 32768 positions 274 us (7: 274, 3: 293, 1: 397), with scores five
+// times as far apart 418 (7: 402, 3: 440).
+template <typename C> struct Held;
+template <> struct Held<__half> {
+    static constexpr float kRise = 5.0f, kBias = 15.0f - kRise;
+    static constexpr int kLow = 11;
+    static constexpr float kLowUp = 2048.0f, kLowDown = 1.0f / 2048.0f;
+};
+// Over a bf16 cache: fp32's exponents, 2^-17 of itself.
+template <> struct Held<__nv_bfloat16> {
+    static constexpr float kRise = 7.0f, kBias = 8.0f;
+    static constexpr int kLow = 0;
+    static constexpr float kLowUp = 1.0f, kLowDown = 1.0f;
+};
 
 // ---- tensor core helpers ----
 // kind::f16, fp32 sums; B with the contraction index as its slow one if `b_mn`.
@@ -113,6 +129,15 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
         "setp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
         "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+// The same onto 2^-N of what is there.
+template <int N> __device__ __forceinline__ void mma_ts_down(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, 1, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p, %4;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "n"(N)
         : "memory");
 }
 #define QVL_R8(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7])
@@ -208,14 +233,14 @@ template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
 template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
     return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
 }
-// A pair as hi + lo, 16 bits each: hi is cut off, not rounded, so that what is
-// left needs no conversion back.
+// A pair as hi + 2^-kLow lo, 16 bits each: hi rounded, what is left of it exact before its own rounding.
 template <typename C> __device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t &lo) {
-    constexpr uint32_t m = std::is_same<C, __half>::value ? 0xffffe000u : 0xffff0000u;
-    const float ha = __uint_as_float(__float_as_uint(a) & m), hb = __uint_as_float(__float_as_uint(b) & m);
-    if constexpr (std::is_same<C, __half>::value) hi = pack2<C>(ha, hb);
-    else hi = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
-    const float2 l = parts(add2(two(a, b), two(-ha, -hb)));
+    constexpr float up = Held<C>::kLowUp;
+    hi = pack2<C>(a, b);
+    const float2 h = unpack2<C>(hi);
+    float2 l;
+    if constexpr (up == 1.0f) l = parts(add2(two(a, b), two(-h.x, -h.y)));
+    else l = parts(fma2(two(h.x, h.y), two(-up, -up), fma2(two(a, b), two(up, up), two(-0.0f, -0.0f))));
     lo = pack2<C>(l.x, l.y);
 }
 // Both halves of a packed pair are finite; the pair with those that are not set to 0.
@@ -926,8 +951,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
 #pragma unroll
                     for (int l = 1; l >= 0; --l)
 #pragma unroll
-                        for (int c = 0; c < kTile / 16; ++c)
-                            mma_ts(d, pb + c * 16 + l * 8, vb + c * (2048 >> 4), id, l == 0 || c ? 1u : 0u);
+                        for (int c = 0; c < kTile / 16; ++c) {
+                            if (l == 0 && c == 0) mma_ts_down<Held<C>::kLow>(d, pb, vb, id);
+                            else mma_ts(d, pb + c * 16 + l * 8, vb + c * (2048 >> 4), id, l == 0 || c ? 1u : 0u);
+                        }
                     tc::tc_commit(bar(fx.o_full));
                     tc::tc_commit(bar(fx.s_free[b]));
                     tc::tc_commit(bar(fx.v_empty[vt.slot]));
@@ -977,7 +1004,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                 if (active) {
                     const float cs = fx.cs[seg & 1][row];
                     const uint64_t cs2 = two(cs, cs);
-                    float mm = m == -INFINITY ? 0.0f : kPBias - m;
+                    float mm = m == -INFINITY ? 0.0f : Held<C>::kBias - m;
                     uint64_t ls = two(0.0f, 0.0f);
                     // 32 positions at a time, enough of them to keep the pipes busy: their scores, and
                     // then the high and low halves of their p in the same columns, 16 by 16
@@ -1002,16 +1029,16 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                         for (int e = 4; e < 28; e += 2)
                             t4[e / 2 % 4] = max3(t4[e / 2 % 4], __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
                         const float mt = fmaxf(max3(t4[0], t4[1], t4[2]), t4[3]) * cs;
-                        if (__any_sync(~0u, mt > m + 7.0f && r < sg.rows)) {
+                        if (__any_sync(~0u, mt > m + Held<C>::kRise && r < sg.rows)) {
                             // a new reference, a whole power of two; what the tile has under the old one is
                             // taken down
                             moved = true;
                             float f = 1.0f;
-                            if (mt > m + 7.0f && r < sg.rows) {
+                            if (mt > m + Held<C>::kRise && r < sg.rows) {
                                 const float up = ceilf(mt);
                                 f = ex2(m - up);
                                 m = up;
-                                mm = kPBias - m;
+                                mm = Held<C>::kBias - m;
                                 l *= f;
                                 ls = fma2(ls, two(f, f), two(-0.0f, -0.0f));
                             }
@@ -1025,7 +1052,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
 #pragma unroll
                                 for (int e = 0; e < 8; ++e) {
                                     const float2 h = unpack2<C>(hi[e]), w = unpack2<C>(lo[e]);
-                                    if (f != 1.0f) split2<C>((h.x + w.x) * f, (h.y + w.y) * f, hi[e], lo[e]);
+                                    constexpr float down = Held<C>::kLowDown;
+                                    if (f != 1.0f) split2<C>(fmaf(w.x, down, h.x) * f, fmaf(w.y, down, h.y) * f, hi[e], lo[e]);
                                 }
                                 tmem_st8(sb + x * 16, hi);
                                 tmem_st8(sb + x * 16 + 8, lo);

@@ -922,3 +922,26 @@ def test_tree_attention_scores_of_minus_infinity_alone(qvl, cuda, dtype):
     c["kv"].k[int(c["table"][0][0]), 0, :7, 0] = -float("inf")
     assert not run_tree(qvl, c).any()
     assert not tree_by_definition(c, 0.125, 2).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("D,nodes,ctx", [(128, 1, 40), (64, 20, 300), (128, 60, 300), (128, 5, 3000)])
+def test_tree_attention_small_weights_carry_the_output(qvl, cuda, dtype, D, nodes, ctx):
+    """One position that takes nearly all of every row's weight and whose value is 0, as an attention sink's
+    is: the output is made of weights 2^-17 to 2^-29 of that one, and as exact as any."""
+    for below in (12.0, 14.0, 17.0, 20.0):
+        c = tree_case(qvl, [ctx], [nodes], 4, 2, D, 32, dtype, seed=int(below), chain=True)
+        # scores of the sink: `below` + the others', which are random with a deviation of 1/4
+        c["q"].mul_(0.25)
+        c["q"][..., 0] = 4.0
+        page = int(c["table"][0][0])
+        t = torch.arange(ctx + nodes, device="cuda")
+        pg = torch.as_tensor(c["table"][0], device="cuda")[t // 32]
+        c["kv"].k[pg, :, t % 32, 0] = 0.0
+        c["kv"].k[page, :, 0, :] = 0.0
+        c["kv"].k[page, :, 0, 0] = below * D ** 0.5 / 4.0
+        # (values of a size at which fp16 outputs are normal numbers)
+        c["kv"].v[pg, :, t % 32, :] *= 8192.0
+        c["kv"].v[page, :, 0, :] = 0.0
+        check_tree(qvl, c)
