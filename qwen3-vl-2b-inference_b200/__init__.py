@@ -33,6 +33,7 @@ from __future__ import annotations
 import ctypes
 import os
 import struct
+import threading
 
 import numpy as np
 import torch
@@ -205,21 +206,41 @@ class Workspace:
 _default_ws: dict = {}
 
 
-def _ws(ws, device):
+def _scratch(ws, device, nbytes: int, stream) -> torch.Tensor:
+    """Scratch of a call on `stream`: the caller's Workspace, or one that only calls of this thread on
+    this stream share (calls on two streams, or the launches of two threads' calls, would
+    write each other's).  A call that is being captured gets memory of its graph."""
     if ws is not None:
-        return ws
-    key = torch.device(device).index
-    if key not in _default_ws:
-        _default_ws[key] = Workspace(device)
-    return _default_ws[key]
+        return ws.get(nbytes)
+    if device.type != "cuda":
+        raise QvlError("expected a CUDA tensor")
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return _scratch(None, device, nbytes, None)
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
+    key = (device.index, torch._C._cuda_getCurrentRawStream(device.index), threading.get_ident())
+    own = _default_ws.get(key)
+    if own is None:
+        own = _default_ws[key] = Workspace(device)
+    return own.get(nbytes)
+
+
+def _empty(shape, dtype, device, stream) -> torch.Tensor:
+    """An output of a call on `stream`, from that stream's memory: what the allocator takes from another
+    stream's may still be in use there."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
 
 
 # --------------------------------------------------------------------------- ops
 def quantize_rows(x: torch.Tensor, group_size: int, stream=None):
     """fp32 [M,K] -> (int16 [M,K], fp32 [M,K/g]); the reference's activation prologue."""
     M, K = x.shape
-    q = torch.empty((M, K), dtype=torch.int16, device=x.device)
-    s = torch.empty((M, K // group_size), dtype=torch.float32, device=x.device)
+    q = _empty((M, K), torch.int16, x.device, stream)
+    s = _empty((M, K // group_size), torch.float32, x.device, stream)
     _check(load_library().qvl_quantize_rows(_ptr(x), _ptr(q), _ptr(s), M, K, group_size,
                                             _stream(stream)), "quantize_rows")
     return q, s
@@ -234,11 +255,11 @@ def linear(A: torch.Tensor, B: torch.Tensor, B_scale: torch.Tensor, C: torch.Ten
     M, K = A.shape
     N = B.shape[0]
     if C is None:
-        C = torch.empty((M, N), dtype=torch.float32, device=A.device)
+        C = _empty((M, N), torch.float32, A.device, stream)
     g = group_size if group_quantized else K
     L = load_library()
     nbytes = L.qvl_linear_i8_workspace_bytes(M, K, g)
-    ws = _ws(workspace, A.device).get(nbytes)
+    ws = _scratch(workspace, A.device, nbytes, stream)
     _check(L.qvl_linear_i8(_ptr(A), _ptr(B), _ptr(B_scale), _ptr(C), M, N, K, int(group_quantized),
                            group_size, semantics, _ptr(ws), ws.numel(), _stream(stream)), "linear")
     return C
@@ -248,7 +269,7 @@ def linear_q16(q, q_scales, B, B_scale, group_size, C=None, semantics=SEM_REFERE
     M, K = q.shape
     N = B.shape[0]
     if C is None:
-        C = torch.empty((M, N), dtype=torch.float32, device=q.device)
+        C = _empty((M, N), torch.float32, q.device, stream)
     _check(load_library().qvl_linear_q16_i8(_ptr(q), _ptr(q_scales), _ptr(B), _ptr(B_scale), _ptr(C),
                                             M, N, K, group_size, semantics, _stream(stream)),
            "linear_q16")
@@ -267,9 +288,9 @@ def swiglu_mlp(x, w_gate, s_gate, w_up, s_up, w_down, s_down, group_size, out=No
     M, H = x.shape
     I = w_gate.shape[0]
     if out is None:
-        out = torch.empty((M, H), dtype=torch.float32, device=x.device)
+        out = _empty((M, H), torch.float32, x.device, stream)
     L = load_library()
-    ws = _ws(workspace, x.device).get(L.qvl_swiglu_mlp_workspace_bytes(M, H, I, group_size))
+    ws = _scratch(workspace, x.device, L.qvl_swiglu_mlp_workspace_bytes(M, H, I, group_size), stream)
     _check(L.qvl_swiglu_mlp_i8(_ptr(x), _ptr(w_gate), _ptr(s_gate), _ptr(w_up), _ptr(s_up),
                                _ptr(w_down), _ptr(s_down), _ptr(out), M, H, I, group_size, semantics,
                                _ptr(ws), ws.numel(), _stream(stream)), "swiglu_mlp")
@@ -313,9 +334,9 @@ def attention(q, kv: PagedKV, seq_ids, positions, max_ctx, out=None, workspace=N
     """out[nq, NH, D] = softmax(q k^T / sqrt(D)) v over positions [0, pos] of each query."""
     nq = q.shape[0]
     if out is None:
-        out = torch.empty_like(q)
+        out = _empty(q.shape, q.dtype, q.device, stream)
     L = load_library()
-    ws = _ws(workspace, q.device).get(L.qvl_attention_workspace_bytes(nq, max_ctx, ctypes.byref(kv.dims)))
+    ws = _scratch(workspace, q.device, L.qvl_attention_workspace_bytes(nq, max_ctx, ctypes.byref(kv.dims)), stream)
     _check(L.qvl_attention_decode(_ptr(q), kv.k.data_ptr(), kv.v.data_ptr(), _ptr(kv.page_table),
                                   _ptr(seq_ids), _ptr(positions), nq, max_ctx, _ptr(out),
                                   ctypes.byref(kv.dims), _ptr(ws), ws.numel(), _stream(stream)),
@@ -329,9 +350,9 @@ def attention_ordered(q, kv: PagedKV, seq_ids, positions, max_ctx, out=None, wor
     fp16-valued cache); sequential over the context, so slower."""
     nq = q.shape[0]
     if out is None:
-        out = torch.empty_like(q)
+        out = _empty(q.shape, q.dtype, q.device, stream)
     L = load_library()
-    ws = _ws(workspace, q.device).get(L.qvl_attention_ordered_workspace_bytes(nq, max_ctx, ctypes.byref(kv.dims)))
+    ws = _scratch(workspace, q.device, L.qvl_attention_ordered_workspace_bytes(nq, max_ctx, ctypes.byref(kv.dims)), stream)
     _check(L.qvl_attention_decode_ordered(_ptr(q), kv.k.data_ptr(), kv.v.data_ptr(), _ptr(kv.page_table),
                                           _ptr(seq_ids), _ptr(positions), nq, max_ctx, _ptr(out),
                                           ctypes.byref(kv.dims), _ptr(ws), ws.numel(), _stream(stream)),
@@ -346,9 +367,9 @@ def qknorm_rope_attention_ordered(q, k_new, v_new, kv: PagedKV, seq_ids, positio
     pass (q is left unrotated); every query a different sequence."""
     nq = q.shape[0]
     if out is None:
-        out = torch.empty_like(q)
+        out = _empty(q.shape, q.dtype, q.device, stream)
     L = load_library()
-    ws = _ws(workspace, q.device).get(L.qvl_attention_ordered_workspace_bytes(nq, max_ctx, ctypes.byref(kv.dims)))
+    ws = _scratch(workspace, q.device, L.qvl_attention_ordered_workspace_bytes(nq, max_ctx, ctypes.byref(kv.dims)), stream)
     _check(L.qvl_qknorm_rope_attention_decode_ordered(
         _ptr(q), _ptr(k_new), _ptr(v_new), kv.k.data_ptr(), kv.v.data_ptr(), _ptr(kv.page_table), _ptr(seq_ids),
         _ptr(positions), nq, max_ctx, _ptr(rope_cos), _ptr(rope_sin), _ptr(q_norm_w), _ptr(q_norm_s),
@@ -422,7 +443,7 @@ def greedy_decode(logits: torch.Tensor, out=None, stream=None) -> torch.Tensor:
     rows = logits.shape[0] if logits.dim() == 2 else 1
     n = logits.shape[-1]
     if out is None:
-        out = torch.empty(rows, dtype=torch.int32, device=logits.device)
+        out = _empty(rows, torch.int32, logits.device, stream)
     _check(load_library().qvl_argmax_rows(_ptr(logits), _ptr(out), rows, n, _stream(stream)),
            "greedy_decode")
     return out
@@ -577,7 +598,7 @@ def attention_q16(q, kv: PagedKV, seq_ids, positions, max_ctx, out, q_out, q_out
     """attention + per-row quantisation of its output (fused when single-launch)."""
     nq = q.shape[0]
     L = load_library()
-    ws = _ws(workspace, q.device).get(L.qvl_attention_workspace_bytes(nq, max_ctx, ctypes.byref(kv.dims)))
+    ws = _scratch(workspace, q.device, L.qvl_attention_workspace_bytes(nq, max_ctx, ctypes.byref(kv.dims)), stream)
     _check(L.qvl_attention_decode_q16(_ptr(q), kv.k.data_ptr(), kv.v.data_ptr(), _ptr(kv.page_table),
                                       _ptr(seq_ids), _ptr(positions), nq, max_ctx, _ptr(out), _ptr(q_out),
                                       _ptr(q_out_scales), _ptr(counter), ctypes.byref(kv.dims), _ptr(ws),
@@ -645,9 +666,9 @@ def _heads(t: torch.Tensor, T: int, H: int, D: int, what: str):
 class PagePlan:
     """What plan_pages writes: one int32 buffer with views of it."""
 
-    def __init__(self, n_seqs: int, max_tokens: int, device):
+    def __init__(self, n_seqs: int, max_tokens: int, device, stream=None):
         self.n_seqs, self.max_tokens = n_seqs, max_tokens
-        buf = self.buf = torch.empty(n_seqs + 3 + 3 * max_tokens, dtype=torch.int32, device=device)
+        buf = self.buf = _empty(n_seqs + 3 + 3 * max_tokens, torch.int32, device, stream)
         self.free_count, self.missing, self.starts = buf[0:1], buf[1:2], buf[2:n_seqs + 3]
         self.seq_ids, self.positions, self.slots = buf[n_seqs + 3:].view(3, max_tokens)
 
@@ -668,7 +689,7 @@ def plan_pages(old_lengths, new_lengths, page_table, free_pages, free_count, pag
     if len(shape) != 2 or shape[0] != S:
         raise QvlError(f"page_table: expected {S} rows, got {tuple(shape)}")
     if plan is None:
-        plan = PagePlan(S, max_tokens, old_lengths.device)
+        plan = PagePlan(S, max_tokens, old_lengths.device, stream)
     elif plan.n_seqs != S or plan.max_tokens != max_tokens:
         raise QvlError("plan was made for another number of requests or tokens")
     p = plan.buf.data_ptr()
@@ -733,7 +754,7 @@ def qknorm_mrope_kv_append(q, k, v, kv: PagedKV, slots, positions, axes, rope_co
     if len(pages) != 4 or pages != vp.shape or pages[1:] != (NKV, d.page_size, D):
         raise QvlError(f"the cache's halves: expected [pages, {NKV}, {d.page_size}, {D}], both of one size")
     if out is None:
-        out = torch.empty(shape, dtype=dt, device=q.device)
+        out = _empty(shape, dt, q.device, stream)
     elif out.dtype is not dt or out.shape != shape:
         raise QvlError("out must have q's shape and type")
     at = positions.shape
@@ -782,13 +803,13 @@ def tree_attention(q, kv: PagedKV, ctx_lens, starts, parents, max_ctx, max_nodes
     if len(pages) != 4 or pages != vp.shape or pages[1:] != (d.num_kv_heads, d.page_size, D) or vp.dtype is not kp.dtype:
         raise QvlError(f"the cache's halves: expected [pages, {d.num_kv_heads}, {d.page_size}, {D}], of one size and type")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = _empty(q.shape, q.dtype, q.device, stream)
     elif out.dtype is not q.dtype or out.shape != q.shape:
         raise QvlError("out must have q's shape and type")
     nbytes = _tree_bytes.get(D)          # the head's size alone decides
     if nbytes is None:
         nbytes = _tree_bytes[D] = load_library().qvl_tree_attention_workspace_bytes(1, 1, 1, 1, ctypes.byref(d))
-    ws = _ws(workspace, q.device).get(nbytes)
+    ws = _scratch(workspace, q.device, nbytes, stream)
     qa, q_st = _heads(q, T, d.num_heads, D, "q")
     _call(_TREE, "tree_attention", qa, _dtype(q), q_st, _addr(kp, "k pages"), _addr(vp, "v pages"), _dtype(kp), pages[0],
           _i32(table, None, "page_table"), _i32(ctx_lens, S, "ctx_lens"), _i32(starts, S + 1, "starts"),
@@ -800,11 +821,11 @@ def tree_attention(q, kv: PagedKV, ctx_lens, starts, parents, max_ctx, max_nodes
 class TokenLogprobs:
     """What token_logprobs writes: logprobs, entropy [T], top_ids, top_logprobs [T, k]."""
 
-    def __init__(self, rows: int, top_k: int, device):
+    def __init__(self, rows: int, top_k: int, device, stream=None):
         self.rows, self.top_k = rows, top_k
-        self.logprobs, self.entropy = torch.empty((2, rows), dtype=torch.float32, device=device)
-        self.top_ids = torch.empty((rows, top_k), dtype=torch.int32, device=device)
-        self.top_logprobs = torch.empty((rows, top_k), dtype=torch.float32, device=device)
+        self.logprobs, self.entropy = _empty((2, rows), torch.float32, device, stream)
+        self.top_ids = _empty((rows, top_k), torch.int32, device, stream)
+        self.top_logprobs = _empty((rows, top_k), torch.float32, device, stream)
 
 
 def token_logprobs(logits, tokens, top_k=0, out: TokenLogprobs | None = None, stream=None) -> TokenLogprobs:
@@ -815,7 +836,7 @@ def token_logprobs(logits, tokens, top_k=0, out: TokenLogprobs | None = None, st
     if not logits.is_cuda or (V > 1 and logits.stride(1) != 1):
         raise QvlError("logits: expected a CUDA tensor with contiguous rows")
     if out is None:
-        out = TokenLogprobs(T, top_k, logits.device)
+        out = TokenLogprobs(T, top_k, logits.device, stream)
     elif out.rows != T or out.top_k != top_k:
         raise QvlError("out was made for another number of rows or alternatives")
     _call(_LOGPROBS, "token_logprobs", logits.data_ptr(), _dtype(logits), logits.stride(0) if T > 1 else V,

@@ -945,3 +945,91 @@ def test_tree_attention_small_weights_carry_the_output(qvl, cuda, dtype, D, node
         c["kv"].v[pg, :, t % 32, :] *= 8192.0
         c["kv"].v[page, :, 0, :] = 0.0
         check_tree(qvl, c)
+
+
+@pytest.mark.gpu
+def test_default_scratch_of_streams_and_threads(qvl, cuda):
+    """Calls without a workspace on two streams at a time, and from two threads on one stream: each has
+    its own parts."""
+    import threading
+    cases = [tree_case(qvl, [ctx], [n], 8, 4, 128, 64, F32, seed=n) for ctx, n in ((9000, 40), (7000, 9))]
+    args = [(c["q"], c["kv"], i32(c["ctx"]), i32(c["starts"]), i32(c["parents"]), c["ctx"][0] + c["nodes"][0], c["nodes"][0])
+            for c in cases]
+    want = [qvl.tree_attention(*a, workspace=qvl.Workspace()) for a in args]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(40):
+        for i in range(2):
+            got[i].append(qvl.tree_attention(*args[i], stream=streams[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
+
+    def work(i):
+        got[i] = [qvl.tree_attention(*args[i]) for _ in range(40)]
+
+    got = [[], []]
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert len(got[i]) == 40 and all(torch.equal(g, want[i]) for g in got[i])
+
+
+@pytest.mark.gpu
+def test_captured_call_keeps_its_scratch(qvl, cuda):
+    """A graph that was captured without a workspace, replayed after other calls have asked for more
+    scratch and other tensors have taken what was given back."""
+    c = tree_case(qvl, [5000, 300], [20, 3], 8, 4, 128, 64, F32, seed=5)
+    a = (c["q"], c["kv"], i32(c["ctx"]), i32(c["starts"]), i32(c["parents"]), 5020, 20)
+    want = qvl.tree_attention(*a).clone()
+    out = torch.empty_like(want)
+    side, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(g, stream=side):
+        qvl.tree_attention(*a, out=out)
+    x, w = torch.randn((3000, 8192), device="cuda"), torch.ones((32, 8192), dtype=torch.int8, device="cuda")
+    for st in (None, side):
+        qvl.linear(x, w, torch.ones((32, 1), device="cuda"), group_quantized=False, stream=st)
+    torch.cuda.synchronize()
+    hold = [torch.full((1 << 18,), 7.0, device="cuda") for _ in range(200)]
+    out.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    assert all(bool((h == 7.0).all()) for h in hold)
+
+
+@pytest.mark.gpu
+def test_memory_comes_from_the_stream_of_the_call(qvl, cuda, monkeypatch):
+    """Outputs and scratch that a call on another stream allocates are that stream's: what is free on the
+    current one may still be in use there."""
+    side, made, real = torch.cuda.Stream(), [], torch.empty
+    c = tree_case(qvl, [20], [4], 4, 2, 128, 16, F32, seed=1)
+    a = (i32(c["ctx"]), i32(c["starts"]), i32(c["parents"]))
+    m = mrope_case(qvl, 30, 4, 2, 128, F32, F16, None, False, 1)
+    x, w, s = torch.randn((64, 256), device="cuda"), torch.ones((32, 256), dtype=torch.int8, device="cuda"), torch.ones((32, 1), device="cuda")
+    slots, pos, tok = i32(m[6]), i32(m[7]), torch.zeros(64, dtype=torch.int32, device="cuda")
+    plan = (i32([0]), i32([9]), i32([[-1]]), i32([0]), i32([1]))
+    side.wait_stream(torch.cuda.current_stream())
+
+    def recorded(*args, **kw):
+        made.append(torch.cuda.current_stream().cuda_stream)
+        return real(*args, **kw)
+
+    monkeypatch.setattr(torch, "empty", recorded)
+    for call in (lambda: qvl.tree_attention(c["q"], c["kv"], *a, 24, 4, stream=side),
+                 lambda: qvl.qknorm_mrope_kv_append(m[0], m[1], m[2], m[3], slots, pos, m[8], m[9], m[10], stream=side),
+                 lambda: qvl.token_logprobs(x, tok, 5, stream=side), lambda: qvl.plan_pages(*plan, 16, 40, stream=side),
+                 lambda: qvl.greedy_decode(x, stream=side), lambda: qvl.quantize_rows(x, 256, stream=side),
+                 lambda: qvl.linear(x, w, s, group_quantized=False, stream=side),
+                 lambda: qvl.attention(c["q"], c["kv"], tok[:4], tok[:4], 24, stream=side)):
+        made.clear()
+        call()
+        assert made and set(made) <= {side.cuda_stream}
+    torch.cuda.synchronize()
