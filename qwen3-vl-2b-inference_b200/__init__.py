@@ -806,9 +806,11 @@ def tree_attention(q, kv: PagedKV, ctx_lens, starts, parents, max_ctx, max_nodes
         out = _empty(q.shape, q.dtype, q.device, stream)
     elif out.dtype is not q.dtype or out.shape != q.shape:
         raise QvlError("out must have q's shape and type")
-    nbytes = _tree_bytes.get(D)          # the head's size alone decides
+    nbytes = _tree_bytes.get(D)          # the head's size alone decides, of dimensions that are not refused (0)
     if nbytes is None:
-        nbytes = _tree_bytes[D] = load_library().qvl_tree_attention_workspace_bytes(1, 1, 1, 1, ctypes.byref(d))
+        nbytes = load_library().qvl_tree_attention_workspace_bytes(1, 1, 1, 1, ctypes.byref(d))
+        if nbytes:
+            _tree_bytes[D] = nbytes
     ws = _scratch(workspace, q.device, nbytes, stream)
     qa, q_st = _heads(q, T, d.num_heads, D, "q")
     _call(_TREE, "tree_attention", qa, _dtype(q), q_st, _addr(kp, "k pages"), _addr(vp, "v pages"), _dtype(kp), pages[0],

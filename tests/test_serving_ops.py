@@ -1033,3 +1033,17 @@ def test_memory_comes_from_the_stream_of_the_call(qvl, cuda, monkeypatch):
         call()
         assert made and set(made) <= {side.cuda_stream}
     torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,P,NH", [(128, 8, 4), (64, 24, 4), (128, 16, 3)])
+def test_tree_attention_after_a_refused_call(qvl, cuda, monkeypatch, D, P, NH):
+    """What the library refuses says nothing about the scratch of later calls."""
+    import qvl_b200
+    monkeypatch.setattr(qvl_b200, "_tree_bytes", {})
+    c = tree_case(qvl, [20], [4], 4, 2, D, 16, F32, seed=1)
+    a = (i32(c["ctx"]), i32(c["starts"]), i32(c["parents"]), 24, 4)
+    with pytest.raises(qvl.QvlError):
+        qvl.tree_attention(torch.zeros((4, NH, D), device="cuda"), qvl.PagedKV(1, 48, NH, 2, D, P), *a,
+                           workspace=qvl.Workspace())
+    check_tree(qvl, c, workspace=qvl.Workspace())
