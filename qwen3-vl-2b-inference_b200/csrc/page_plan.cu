@@ -26,6 +26,7 @@
 // another in every CTA and a search per token; 16 with two and three CTAs on an SM, the
 // sums formed in each).
 #include <algorithm>
+#include <atomic>
 #include "serving.cuh"
 
 namespace qvl {
@@ -220,10 +221,19 @@ __global__ void __launch_bounds__(kThreads) plan_pages_kernel(PlanArgs a) {
 
 cudaError_t launch_plan_pages(const PlanArgs &args, cudaStream_t st) {
     PlanArgs a = args;
-    const size_t smem = (size_t)3 * (a.S + 1) * sizeof(int);
+    const auto smem_of = [](int S) { return (size_t)3 * (S + 1) * sizeof(int); };
+    const size_t smem = smem_of(a.S);
     if (smem > 40 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(plan_pages_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        // what the most requests need, whatever these do: another thread's launch goes by it too
+        static std::atomic<uint64_t> allowed{0};        // devices that have it
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
         if (e != cudaSuccess) return e;
+        if (dev >= 64 || !((allowed.load(std::memory_order_relaxed) >> dev) & 1)) {
+            e = cudaFuncSetAttribute(plan_pages_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_of(kPlanMaxSeqs));
+            if (e != cudaSuccess) return e;
+            if (dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
+        }
     }
     a.inv_p = ~0ull / (unsigned)a.P + ((a.P & (a.P - 1)) == 0) + 1;
     // a CTA an SM; the pages that may change hands are about a request's last one and a page

@@ -1047,3 +1047,30 @@ def test_tree_attention_after_a_refused_call(qvl, cuda, monkeypatch, D, P, NH):
         qvl.tree_attention(torch.zeros((4, NH, D), device="cuda"), qvl.PagedKV(1, 48, NH, 2, D, P), *a,
                            workspace=qvl.Workspace())
     check_tree(qvl, c, workspace=qvl.Workspace())
+
+
+@pytest.mark.gpu
+def test_plan_pages_of_different_sizes_from_two_threads(qvl, cuda):
+    """Plans of many and of fewer requests at once: what one launch needs of shared memory does not
+    take away the other's."""
+    import threading
+    args, errors = [], []
+    for S in (16384, 3600):
+        z = torch.zeros(S, dtype=torch.int32, device="cuda")
+        args.append((z, z, torch.full((S, 1), -1, dtype=torch.int32, device="cuda"), i32([0]), i32([0]), 16, 0, qvl.PagePlan(S, 0, "cuda")))
+
+    def work(a):
+        stream = torch.cuda.Stream()
+        try:
+            for _ in range(20000):
+                qvl.plan_pages(*a, stream=stream)
+        except qvl.QvlError as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(a,)) for a in args]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors
