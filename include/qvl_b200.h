@@ -456,7 +456,7 @@ const uint64_t *qvl_text_decode_trace(const void *workspace);
  * at or past the old pages of growing requests, free_pages at or past
  * *free_count, and free_count_out is a word of its own.  A caller that finds
  * missing > 0 plans again from the same lengths and the same free_count with
- * smaller new_lengths.  n_seqs <= 16384; fewer than 2^31 tokens in all. */
+ * smaller new_lengths.  n_seqs <= 16384; max_tokens < 2^31 - 2^18; fewer than 2^31 tokens in all. */
 int qvl_plan_pages(const int32_t *old_lengths, const int32_t *new_lengths, size_t n_seqs, int32_t *page_table,
                    int page_size, int max_pages_per_seq, int32_t *free_pages, const int32_t *free_count,
                    size_t capacity, int32_t *free_count_out, int32_t *missing, int32_t *starts, int32_t *seq_ids,

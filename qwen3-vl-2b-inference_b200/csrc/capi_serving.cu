@@ -35,7 +35,8 @@ int qvl_plan_pages(const int32_t *old_lengths, const int32_t *new_lengths, size_
         !starts || (max_tokens && (!seq_ids || !positions || !slots)))
         return QVL_ERR_INVALID;
     if (n_seqs == 0 || page_size <= 0 || max_pages_per_seq <= 0 || free_count == free_count_out) return QVL_ERR_INVALID;
-    if (capacity > (size_t)INT32_MAX || max_tokens > (size_t)INT32_MAX - 4096) return QVL_ERR_INVALID;
+    // (the kernel's stretches of tokens end up to 4704 * 32 past the last one)
+    if (capacity > (size_t)INT32_MAX || max_tokens > (size_t)INT32_MAX - (1u << 18)) return QVL_ERR_INVALID;
     const void *p[] = {old_lengths, new_lengths, page_table, free_pages, free_count, free_count_out,
                        missing,     starts,      seq_ids,    positions,  slots};
     for (const void *x : p)

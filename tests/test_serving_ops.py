@@ -1074,3 +1074,11 @@ def test_plan_pages_of_different_sizes_from_two_threads(qvl, cuda):
         t.join()
     torch.cuda.synchronize()
     assert not errors
+
+
+def test_plan_pages_refuses_more_tokens_than_its_indexes_hold():
+    """A warp's stretch of tokens ends up to 150,000 past the last one, in 32 bits."""
+    L = import_qvl().load_library()
+    f = 4096                                     # aligned, never dereferenced
+    for n in (2 ** 31 - 1 - 4096, 2 ** 31 - 150_000, 2 ** 31 - 2 ** 18, 2 ** 31, 2 ** 40):
+        assert L.qvl_plan_pages(f, f, 4, f, 16, 4, f, f, 8, f + 4, f, f, f, f, f, n, None) == 1, n
