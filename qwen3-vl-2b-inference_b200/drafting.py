@@ -84,7 +84,9 @@ class TreeDecoder:
     """Requests 0 .. max_requests - 1 over one pool of num_pages cache pages per layer.
 
     max_tokens: nodes of all requests in one pass.  sections: rotary frequencies per position axis
-    (D / 2 in all), None for text positions alone."""
+    (D / 2 in all), None for text positions alone.  A token without positions of its own is at
+    its request's largest position so far plus 1, on all axes (a node of a tree at its depth past that),
+    which after an image is less than the number of tokens."""
 
     def __init__(self, weights: TextWeights, max_requests: int, max_ctx: int, num_pages: int, max_tokens: int = 512,
                  page_size: int = 64, sections=None, device="cuda"):
@@ -102,6 +104,7 @@ class TreeDecoder:
         self.free_pages = torch.arange(num_pages - 1, -1, -1, dtype=torch.int32, device=dev)
         self.free_count = torch.full((1,), num_pages, dtype=torch.int32, device=dev)
         self.lengths = [0] * max_requests
+        self.next_pos = [0] * max_requests          # each request's largest position so far plus 1
         sections = (D // 2,) if sections is None else sections
         self.axes, self.n_axes = mrope_axes(sections, device=dev), len(sections)
         cos, sin = rope_table(max_ctx, D, cfg.rope_theta)
@@ -167,8 +170,9 @@ class TreeDecoder:
     def _pass(self, trees, rows, top_k, positions):
         """All nodes of `trees` {request: (tokens, parents)} through the model; log-probabilities of
         the greedy choices at the nodes `rows` (of all, packed in request order).  Leaves the
-        drafts' keys and values in the cache.  (greedy ids, TokenLogprobs, plan, lengths)"""
-        tokens, parents, pos, counts = [], [], [], [0] * self.S
+        drafts' keys and values in the cache.  (greedy ids, TokenLogprobs, plan, lengths on the
+        device and the host, positions by request)"""
+        tokens, parents, pos, counts = [], [], {}, [0] * self.S
         for s in sorted(trees):
             if not 0 <= s < self.S:
                 raise QvlError(f"no request {s}")
@@ -181,23 +185,24 @@ class TreeDecoder:
                 raise QvlError(f"request {s}: {self.lengths[s]} + {len(toks)} tokens pass the context of {self.max_ctx}")
             own = positions.get(s) if positions else None
             if own is None:
-                own = [[self.lengths[s] + d for d in depth]] * self.n_axes
+                own = [[self.next_pos[s] + d for d in depth]] * self.n_axes
             elif np.shape(own) != (self.n_axes, len(toks)):
                 raise QvlError(f"positions of request {s}: expected [{self.n_axes}, {len(toks)}]")
-            pos.append(np.asarray(own, np.int32))
+            pos[s] = np.asarray(own, np.int32)
         T = len(tokens)
         if not 1 <= T <= self.max_tokens:
             raise QvlError(f"a pass takes 1 to {self.max_tokens} tokens, got {T}")
         after = [n + c for n, c in zip(self.lengths, counts)]
         # one upload: tokens, parents, positions, lengths before and after
-        host = np.concatenate([tokens, parents, np.concatenate(pos, 1).reshape(-1), self.lengths, after]).astype(np.int32)
+        host = np.concatenate([tokens, parents, np.concatenate(list(pos.values()), 1).reshape(-1), self.lengths,
+                               after]).astype(np.int32)
         up = torch.from_numpy(host).to(self.device)
-        tok, par, pos, old, new = torch.split(up, [T, T, self.n_axes * T, self.S, self.S])
+        tok, par, dpos, old, new = torch.split(up, [T, T, self.n_axes * T, self.S, self.S])
         plan = self._plan(old, new, self.free_count, T, "grow")
         x = self.x[:T]
         t, cfg = self.w.t, self.cfg
         embedding_lookup_i8(t["embed"], t["embed_s"], tok, x)
-        self._layers(x, T, plan, pos.view(self.n_axes, T), old, par, max(after), max(counts))
+        self._layers(x, T, plan, dpos.view(self.n_axes, T), old, par, max(after), max(counts))
         if rows is not None:
             x = x[torch.tensor(rows, device=self.device)]
         R, H = x.shape
@@ -211,7 +216,7 @@ class TreeDecoder:
         if int(plan.missing.item()):
             # nothing is kept: the stack's old size and the old lengths still hold
             raise QvlError(f"the cache pool has no page for {int(plan.missing.item())} of the pass's tokens")
-        return greedy, scores, plan, new, after
+        return greedy, scores, plan, new, after, pos
 
     def _keep(self, plan, new, after, lengths) -> None:
         """The requests' lengths after a pass; pages past them go back to the pool."""
@@ -240,8 +245,10 @@ class TreeDecoder:
                     where[s] = np.asarray(positions[s])[:, at[s]:at[s] + n]
                 at[s] += n
                 ends.append(self.max_tokens - room - 1)
-            greedy, _, plan, new, after = self._pass(trees, ends, 0, where)
+            greedy, _, plan, new, after, pos = self._pass(trees, ends, 0, where)
             self._keep(plan, new, after, after)
+            for s, own in pos.items():
+                self.next_pos[s] = max(self.next_pos[s], int(own.max()) + 1)
             last.update(zip(sorted(trees), greedy.tolist()))
         return last
 
@@ -249,17 +256,18 @@ class TreeDecoder:
         """One pass over drafted trees {request: (tokens, parents)}: node 0 is the request's last
         chosen token, not yet in the cache.  Returns {request: Accepted} and keeps
         the accepted nodes' keys and values."""
-        greedy, scores, plan, new, after = self._pass(trees, None, top_k, positions)
+        greedy, scores, plan, new, after, pos = self._pass(trees, None, top_k, positions)
         ids = greedy.tolist()
         lp, ent = scores.logprobs.cpu().numpy(), scores.entropy.cpu().numpy()
         top_ids, top_lp = scores.top_ids.cpu().numpy(), scores.top_logprobs.cpu().numpy()
-        got, lengths, moves, first = {}, list(after), [], 0
+        got, lengths, next_pos, moves, first = {}, list(after), list(self.next_pos), [], 0
         for s in sorted(trees):
             tokens, parents = trees[s]
             path = accepted_path(tokens, parents, ids[first:first + len(tokens)])
             rows = [first + p for p in path]
             got[s] = Accepted([ids[r] for r in rows], lp[rows], ent[rows], top_ids[rows], top_lp[rows])
             lengths[s] = self.lengths[s] + len(path)
+            next_pos[s] = max(next_pos[s], int(pos[s][:, path].max()) + 1)
             moves += [(r, first + i) for i, r in enumerate(rows) if r != first + i]
             first += len(tokens)
         if moves:
@@ -269,6 +277,7 @@ class TreeDecoder:
             for c in (self.k_all, self.v_all):
                 c[:, dst // P, :, dst % P] = c[:, src // P, :, src % P]
         self._keep(plan, new, after, lengths)
+        self.next_pos = next_pos
         return got
 
     def release(self, requests) -> None:
@@ -278,3 +287,4 @@ class TreeDecoder:
         plan = self._plan(old, new, self.free_count, 0, "shrink")
         self.free_count = plan.free_count.clone()
         self.lengths = lengths
+        self.next_pos = [p if n else 0 for p, n in zip(self.next_pos, lengths)]

@@ -225,3 +225,39 @@ def test_tree_decoder_refusals(qvl, cuda):
             call()
         t.release([0, 1])
     assert t.lengths == [0, 0] and int(t.free_count) == 2
+
+
+@pytest.mark.gpu
+def test_tokens_after_a_prompt_with_its_own_positions(qvl, cuda):
+    """After an image prompt the next position is the largest one so far plus 1, for a drafted tree as for
+    more of the prompt; the accepted path's depth counts, not the number of its nodes."""
+    D, F, cfg, w, one = _setup(qvl, cuda, seed=8)
+    prompt = [(3 * i + 1) % cfg.vocab for i in range(20)]
+    grid = np.stack([np.zeros(20), np.arange(20) // 5, np.arange(20) % 5]).astype(np.int32)      # largest: 4
+    a, b = (F.TreeDecoder(w, 2, 64, 4, max_tokens=64, sections=(24, 20, 20), device=cuda) for _ in range(2))
+    roots = [d.extend({1: prompt}, positions={1: grid})[1] for d in (a, b)]
+    assert roots[0] == roots[1]
+
+    def same(x, y):
+        assert x[1].tokens == y[1].tokens and torch.equal(a.logits, b.logits)
+        assert torch.equal(a.k_all, b.k_all) and torch.equal(a.v_all, b.v_all)
+
+    # a tree: root and two children side by side, a grandchild of the second
+    tree = ([roots[0], 5, 6, 7], [-1, 0, 0, 2])
+    same(a.verify({1: tree}), b.verify({1: tree}, positions={1: [[5, 6, 6, 7]] * 3}))
+    kept = a.lengths[1] - 20
+    # a chain whose first child is the model's own choice: two nodes at least are kept
+    root = a.verify({1: ([9], [-1])})[1].tokens
+    assert b.verify({1: ([9], [-1])}, positions={1: [[5 + kept]] * 3})[1].tokens == root
+    chain = ([root[0], 1], [-1, 0])
+    nxt = 5 + kept + 1
+    same(a.verify({1: chain}), b.verify({1: chain}, positions={1: [[nxt, nxt + 1]] * 3}))
+    nxt += a.lengths[1] - 20 - kept - 1
+    # more text after it, in an extend()
+    assert a.extend({1: [4, 5, 6]}) == b.extend({1: [4, 5, 6]}, positions={1: [list(range(nxt, nxt + 3))] * 3})
+    assert torch.equal(a.logits, b.logits) and torch.equal(a.k_all, b.k_all)
+    # a request that ended and another one in its place begin at 0
+    a.release([1])
+    c = F.TreeDecoder(w, 2, 64, 4, max_tokens=64, sections=(24, 20, 20), device=cuda)
+    assert a.extend({1: prompt[:7]}) == c.extend({1: prompt[:7]}, positions={1: np.tile(np.arange(7), (3, 1))})
+    assert torch.equal(a.logits, c.logits)
