@@ -188,7 +188,10 @@ class TreeDecoder:
                 own = [[self.next_pos[s] + d for d in depth]] * self.n_axes
             elif np.shape(own) != (self.n_axes, len(toks)):
                 raise QvlError(f"positions of request {s}: expected [{self.n_axes}, {len(toks)}]")
-            pos[s] = np.asarray(own, np.int32)
+            own = np.asarray(own)
+            if own.min() < 0 or own.max() >= self.max_ctx:
+                raise QvlError(f"request {s}: a position outside the rotary table's {self.max_ctx} rows")
+            pos[s] = own.astype(np.int32)
         T = len(tokens)
         if not 1 <= T <= self.max_tokens:
             raise QvlError(f"a pass takes 1 to {self.max_tokens} tokens, got {T}")

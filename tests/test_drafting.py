@@ -261,3 +261,23 @@ def test_tokens_after_a_prompt_with_its_own_positions(qvl, cuda):
     c = F.TreeDecoder(w, 2, 64, 4, max_tokens=64, sections=(24, 20, 20), device=cuda)
     assert a.extend({1: prompt[:7]}) == c.extend({1: prompt[:7]}, positions={1: np.tile(np.arange(7), (3, 1))})
     assert torch.equal(a.logits, c.logits)
+
+
+@pytest.mark.gpu
+def test_positions_outside_the_rotary_table_are_refused(qvl, cuda):
+    """The table has max_ctx rows; a token outside it would get no query and no place in the cache."""
+    D, F, cfg, w, one = _setup(qvl, cuda, seed=8)
+    t = F.TreeDecoder(w, 1, 64, 2, max_tokens=64, sections=(24, 20, 20), device=cuda)
+    good = np.tile(np.arange(5), (3, 1))
+    for axis, at, value in ((0, 4, 64), (2, 0, -1), (1, 2, 2 ** 31 - 1)):
+        bad = good.copy()
+        bad[axis, at] = value
+        with pytest.raises(qvl.QvlError):
+            t.extend({0: [1, 2, 3, 4, 5]}, positions={0: bad})
+        with pytest.raises(qvl.QvlError):
+            t.verify({0: ([1, 2, 3, 4, 5], [-1, 0, 1, 2, 3])}, positions={0: bad})
+    assert t.lengths == [0] and int(t.free_count) == 2
+    t.extend({0: [1, 2, 3, 4, 5]}, positions={0: good + 59})       # up to the table's last row
+    with pytest.raises(qvl.QvlError):
+        t.verify({0: ([1], [-1])})
+    assert t.lengths == [5]
