@@ -103,7 +103,7 @@ class TreeDecoder:
         self.kv = [PooledKV(self.k_all[l], self.v_all[l], self.page_table, dims) for l in range(cfg.layers)]
         self.free_pages = torch.arange(num_pages - 1, -1, -1, dtype=torch.int32, device=dev)
         self.free_count = torch.full((1,), num_pages, dtype=torch.int32, device=dev)
-        self.lengths = [0] * max_requests
+        self.num_pages, self.lengths = num_pages, [0] * max_requests
         self.next_pos = [0] * max_requests          # each request's largest position so far plus 1
         sections = (D // 2,) if sections is None else sections
         self.axes, self.n_axes = mrope_axes(sections, device=dev), len(sections)
@@ -122,6 +122,25 @@ class TreeDecoder:
         self.planes = Planes(T, max(H, I, cfg.heads * D), dev)
         self.ws = Workspace(dev)
         self._plans: dict = {}
+
+    def _own_positions(self, s: int, own, n: int) -> np.ndarray:
+        """Positions [axes, n] that request s is to have, checked."""
+        own = np.asarray(own)
+        if own.shape != (self.n_axes, n):
+            raise QvlError(f"positions of request {s}: expected [{self.n_axes}, {n}]")
+        if own.min() < 0 or own.max() >= self.max_ctx:
+            raise QvlError(f"request {s}: a position outside the rotary table's {self.max_ctx} rows")
+        return own.astype(np.int32)
+
+    def _check_room(self, after) -> None:
+        """The context and the pool have room for requests of these lengths.  (The pool is this decoder's
+        alone, so that its free pages follow from the lengths.)"""
+        for s, n in enumerate(after):
+            if n > self.max_ctx:
+                raise QvlError(f"request {s}: {n} tokens pass the context of {self.max_ctx}")
+        pages = sum(-(-n // self.page_size) for n in after)
+        if pages > self.num_pages:
+            raise QvlError(f"the cache pool has {self.num_pages} pages, and the requests would hold {pages}")
 
     def _plan(self, old, new, free_count, tokens: int, which: str) -> PagePlan:
         """Lengths old -> new; the pass's own plan and the one that gives pages back write
@@ -181,21 +200,15 @@ class TreeDecoder:
             tokens += toks
             parents += par
             counts[s] = len(toks)
-            if self.lengths[s] + len(toks) > self.max_ctx:
-                raise QvlError(f"request {s}: {self.lengths[s]} + {len(toks)} tokens pass the context of {self.max_ctx}")
             own = positions.get(s) if positions else None
             if own is None:
                 own = [[self.next_pos[s] + d for d in depth]] * self.n_axes
-            elif np.shape(own) != (self.n_axes, len(toks)):
-                raise QvlError(f"positions of request {s}: expected [{self.n_axes}, {len(toks)}]")
-            own = np.asarray(own)
-            if own.min() < 0 or own.max() >= self.max_ctx:
-                raise QvlError(f"request {s}: a position outside the rotary table's {self.max_ctx} rows")
-            pos[s] = own.astype(np.int32)
+            pos[s] = self._own_positions(s, own, len(toks))
         T = len(tokens)
         if not 1 <= T <= self.max_tokens:
             raise QvlError(f"a pass takes 1 to {self.max_tokens} tokens, got {T}")
         after = [n + c for n, c in zip(self.lengths, counts)]
+        self._check_room(after)
         # one upload: tokens, parents, positions, lengths before and after
         host = np.concatenate([tokens, parents, np.concatenate(list(pos.values()), 1).reshape(-1), self.lengths,
                                after]).astype(np.int32)
@@ -216,9 +229,6 @@ class TreeDecoder:
         self._product(qh, qs, ("embed",), None, [self.logits])
         greedy = greedy_decode(self.logits)
         scores = token_logprobs(self.logits, greedy, top_k)
-        if int(plan.missing.item()):
-            # nothing is kept: the stack's old size and the old lengths still hold
-            raise QvlError(f"the cache pool has no page for {int(plan.missing.item())} of the pass's tokens")
         return greedy, scores, plan, new, after, pos
 
     def _keep(self, plan, new, after, lengths) -> None:
@@ -232,10 +242,21 @@ class TreeDecoder:
     def extend(self, prompts: dict, positions: dict | None = None) -> dict:
         """Appends prompts {request: tokens} and returns {request: next greedy token}.  A pass
         takes up to 256 tokens of each request, a chain each; positions: {request: [axes,
-        len(prompt)]}."""
+        len(prompt)]}.  All of it is checked first: a call that is refused leaves the requests as they were."""
+        prompts = {s: list(map(int, p)) for s, p in prompts.items()}
+        positions, after = dict(positions or {}), list(self.lengths)
+        for s, p in prompts.items():
+            if not 0 <= s < self.S:
+                raise QvlError(f"no request {s}")
+            if not p:
+                raise QvlError("an empty prompt")
+            if min(p) < 0 or max(p) >= self.cfg.vocab:
+                raise QvlError("a token of a prompt lies outside the vocabulary")
+            after[s] += len(p)
+            text = [range(self.next_pos[s], self.next_pos[s] + len(p))] * self.n_axes
+            positions[s] = self._own_positions(s, positions.get(s, text), len(p))
+        self._check_room(after)
         at, last = {s: 0 for s in prompts}, {}
-        if any(len(p) == 0 for p in prompts.values()):
-            raise QvlError("an empty prompt")
         while any(at[s] < len(prompts[s]) for s in at):
             trees, where, ends, room = {}, {}, [], self.max_tokens
             for s in sorted(prompts):
@@ -243,9 +264,8 @@ class TreeDecoder:
                 if n <= 0:
                     continue
                 room -= n
-                trees[s] = (list(map(int, prompts[s][at[s]:at[s] + n])), list(range(-1, n - 1)))
-                if positions and s in positions:
-                    where[s] = np.asarray(positions[s])[:, at[s]:at[s] + n]
+                trees[s] = (prompts[s][at[s]:at[s] + n], list(range(-1, n - 1)))
+                where[s] = positions[s][:, at[s]:at[s] + n]
                 at[s] += n
                 ends.append(self.max_tokens - room - 1)
             greedy, _, plan, new, after, pos = self._pass(trees, ends, 0, where)

@@ -281,3 +281,32 @@ def test_positions_outside_the_rotary_table_are_refused(qvl, cuda):
     with pytest.raises(qvl.QvlError):
         t.verify({0: ([1], [-1])})
     assert t.lengths == [5]
+
+
+@pytest.mark.gpu
+def test_a_refused_prompt_leaves_nothing_behind(qvl, cuda):
+    """What is wrong with a prompt, or with one of several, in a chunk after the first as well: lengths and
+    pool are as they were, and the requests go on as if nothing had been asked."""
+    D, F, cfg, w, one = _setup(qvl, cuda, seed=8)
+    a, b = (F.TreeDecoder(w, 3, 256, 4, max_tokens=40, device=cuda) for _ in range(2))
+    assert a.extend({1: [5, 6, 7]}) == b.extend({1: [5, 6, 7]})
+    v = cfg.vocab
+    long = [1] * 50
+    for call in (lambda: a.extend({0: [1] * 257}), lambda: a.extend({1: [1] * 254}), lambda: a.extend({0: long + [v]}),
+                 lambda: a.extend({0: [1] * 45, 2: [1] * 30 + [-1]}), lambda: a.extend({0: long, 3: [1]}),
+                 lambda: a.extend({0: [1] * 60, 2: []}), lambda: a.extend({-1: [1], 0: [1]}),
+                 lambda: a.extend({0: long}, positions={0: [list(range(49))]}),
+                 lambda: a.extend({0: long}, positions={0: [list(range(50))] * 2}),
+                 lambda: a.extend({0: long}, positions={0: [list(range(49)) + [256]]}),
+                 # pages: the second chunk of one, and the second of two, find none
+                 lambda: a.extend({0: [1] * 193}), lambda: a.extend({0: [1] * 129, 2: [1] * 30}),
+                 lambda: a.verify({0: ([1] * 40, list(range(-1, 39))), 3: ([1], [-1])})):
+        with pytest.raises(qvl.QvlError):
+            call()
+        assert a.lengths == [0, 3, 0] and int(a.free_count) == 3
+    prompt = [(5 * i + 2) % v for i in range(70)]
+    assert a.extend({0: prompt, 1: [9]}) == b.extend({0: prompt, 1: [9]})
+    assert a.lengths == b.lengths == [70, 4, 0] and torch.equal(a.logits, b.logits)
+    tree = {0: ([3, 4], [-1, 0]), 1: ([8], [-1])}
+    x, y = a.verify(tree), b.verify(tree)
+    assert [x[s].tokens for s in x] == [y[s].tokens for s in y] and torch.equal(a.logits, b.logits)
