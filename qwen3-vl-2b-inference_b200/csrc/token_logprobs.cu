@@ -195,6 +195,8 @@ __global__ void __launch_bounds__(kThreads, kPerSM) token_logprobs_kernel(const 
     const int loads = (a.V - head) / N, tail = head + loads * N;
     const int per = (loads + C - 1) / C, lo = min(rank * per, loads), hi = min(lo + per, loads);
     const int loose = rank == 0 ? head + a.V - tail : 0;
+    // (ordinary loads: the launch begins before the one that writes the logits has ended, and the
+    // read-only path is for what nobody writes in a kernel's lifetime)
     const uint4 *xv = reinterpret_cast<const uint4 *>(x + head);
     auto loose_at = [&](int i) { return i < head ? i : tail + i - head; };
 
@@ -224,7 +226,7 @@ __global__ void __launch_bounds__(kThreads, kPerSM) token_logprobs_kernel(const 
         Vec<T> v[kAhead];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            if (i + u * kThreads < hi) v[u].v = __ldg(xv + i + u * kThreads);
+            if (i + u * kThreads < hi) v[u].v = xv[i + u * kThreads];
             else v[u] = none();
         }
 #pragma unroll
@@ -279,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, kPerSM) token_logprobs_kernel(const 
             const int q = j / turns, i = lo + asked[q] + (j - q * turns) * kThreads;
             if (i >= hi) continue;
             Vec<T> w;
-            w.v = __ldg(xv + i);
+            w.v = xv[i];
             if (w.largest() >= tau) {
                 float f[N];
                 w.unpack(f);
@@ -305,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, kPerSM) token_logprobs_kernel(const 
             if (tid < loose) look(own, loose_at(tid));
             for (int i = lo + tid; i < hi; i += kThreads) {
                 Vec<T> w;
-                w.v = __ldg(xv + i);
+                w.v = xv[i];
                 float f[N];
                 w.unpack(f);
 #pragma unroll

@@ -1082,3 +1082,16 @@ def test_plan_pages_refuses_more_tokens_than_its_indexes_hold():
     f = 4096                                     # aligned, never dereferenced
     for n in (2 ** 31 - 1 - 4096, 2 ** 31 - 150_000, 2 ** 31 - 2 ** 18, 2 ** 31, 2 ** 40):
         assert L.qvl_plan_pages(f, f, 4, f, 16, 4, f, f, 8, f + 4, f, f, f, f, f, n, None) == 1, n
+
+
+def test_no_read_only_loads_beside_the_launch_that_writes():
+    """The operators' launches begin before those ahead of them have ended (pdl_wait), so that what they
+    read is written in their lifetime: nothing for the read-only path."""
+    import os
+    import re
+    from conftest import PKG_DIR
+    for f in ("page_plan", "mrope_append", "tree_attention", "token_logprobs"):
+        with open(os.path.join(PKG_DIR, "csrc", f + ".cu")) as h:
+            src = h.read()
+        assert "pdl_wait();" in src
+        assert not re.search(r"__ldg|ld\.global\.nc|__restrict__|ld_stream", src), f
