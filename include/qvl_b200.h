@@ -492,11 +492,11 @@ int qvl_qknorm_mrope_kv_append(const void *q, const void *k, const void *v, int 
  * other value marks a root.  out [n_rows, NH, D] of q's type = softmax(scale
  * q k^T) v; masked keys and values have no influence whatever they hold, and
  * positions past the page table's width, or on pages outside [0, num_pages), do not
- * exist.  What is seen counts with its infinities: a score that is NaN or inf makes its row
- * NaN, a score of -inf has no weight, any other one a weight above 0, whatever
- * the value that it meets.  A row that sees nothing, or nothing with a weight, a row of q outside [starts[0], starts[n_seqs]) and a
- * node past max_nodes get zeros.  max_ctx, a bound of ctx_lens + nodes, only
- * shapes the launch.  Types (q, cache): fp32 or fp16 over fp16, bf16 over
+ * exist.  What is seen counts with its infinities: a score that is NaN or inf
+ * makes its row NaN, a score of -inf has no weight, any other one a weight above
+ * 0, whatever the value that it meets.  A row that sees nothing, or nothing with
+ * a weight, a row of q outside [starts[0], starts[n_seqs]) and a node past
+ * max_nodes get zeros.  max_ctx, a bound of ctx_lens + nodes, only shapes the launch.  Types (q, cache): fp32 or fp16 over fp16, bf16 over
  * bf16; out does not overlap q.  D 64 or 128, num_heads / num_kv_heads <= 128, max_nodes <= 256,
  * page_size a multiple of 16. */
 size_t qvl_tree_attention_workspace_bytes(size_t n_seqs, size_t n_rows, int max_ctx, int max_nodes,

@@ -10,13 +10,14 @@
 // Memory bound: one read of the logits, 16 bytes a load and four of them in flight a
 // thread.  A cluster of CTAs takes a row, each a slice of the vocabulary;
 // statistics and candidates meet in the first CTA's shared memory.  Measured: 512
-// rows of 151936 fp32 without alternatives 51 us (6.1 TB/s); 1024 rows of bf16 with 5 of
-// them 77 us (4.0 TB/s; 66 us without: one exponential a logit and its conversions take
-// the issue slots at two bytes a logit); 27 rows of fp32 with 20 of them 13.3 us.
+// rows of 151936 fp32 without alternatives 52 us (6.0 TB/s), with 5 of them 59; 1024 rows of
+// bf16 with 5 75.5 us (4.1 TB/s; 64 us without: one exponential a logit and its conversions take
+// the issue slots at two bytes a logit); 27 rows of fp32 with 20 13.3 us, without 6.7.
 //
 // Sums: a thread's exponentials are taken against a reference that moves only when a
 // logit passes it by 8, so that almost no load rescales anything; an exponent of up
-// to 8 is rounded by 8 u, u = 2^-24, which is what its exponential is then off by.
+// to 8 is rounded by 8 u, u = 2^-24, which is what its exponential is then off by (ex2.approx itself by
+// 4 u at most).
 //
 // Candidates: the pass leaves each thread with the largest of its logits.  A thread whose
 // maximum is passed by k others has nothing among the alternatives; the logits of the

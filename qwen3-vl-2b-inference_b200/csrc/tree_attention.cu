@@ -49,15 +49,17 @@
 // once more in plain fp32 (fix_row), after the products or in the joining launch.
 // 16-bit queries are exact as they are.
 //
-// Measured (16 query and 8 key heads of 128, fp16 cache, keys and values read once: 5 TB/s
-// and 4.3 TB/s of the 6.5 that a copy reaches): 16 requests of 64 nodes over up to 32768
-// positions, fp16, 247 us; 32 of 16 nodes over up to 4096, fp32, 73 us, of which
+// Exponentials are ex2.approx (relative error 2^-22) of arguments with one fp32 rounding.
+//
+// Measured (16 query and 8 key heads of 128, fp16 cache, keys and values read once: 4.6 TB/s
+// and 4.1 TB/s of the 6.5 that a copy reaches): 16 requests of 64 nodes over up to 32768
+// positions, fp16, 270 us; 32 of 16 nodes over up to 4096, fp32, 77 us, of which
 // tiles take what memory does, and a segment's beginning and end the rest.  In a long
-// row of such calls the board's power limit, not a pipe, sets the time (315 and 92 us, the
+// row of such calls the board's power limit, not a pipe, sets the time (320 to 350 and 92 us, the
 // SMs at 1.4 and 1.5 GHz of 1.97): the products of p's low halves are a tenth of it, and
 // at 32 rows a fifth goes to the scores' products, of which each block uses a quarter.  12 requests of
 // 132 rows over up to 6000, bf16, heads of 64: 38 us, the softmax's 3400 cycles for a
-// tile of 128 x 128.  One token over 452 positions 13.6 us, 27 nodes over 2011 20 us: latency,
+// tile of 128 x 128.  One token over 452 positions 13.9 us, 27 nodes over 2011 21 us: latency,
 // the kernel's beginning (5 us: finding the stretch, queries to tensor memory), one tile, and the
 // join (5 us).
 // Tried and not kept: 16 scores a step (4000 cycles a tile for 3000), 64 with the largest
