@@ -191,7 +191,7 @@ def _stream(stream=None):
 
 class Workspace:
     """Device scratch owned by the caller and reused across calls (the C ABI
-    never allocates).  Grows on demand outside any timed or captured region."""
+    never allocates), for one stream at a time.  Grows on demand outside any timed or captured region."""
 
     def __init__(self, device=None):
         self.device = torch.device(device or "cuda")
@@ -794,7 +794,8 @@ def tree_attention(q, kv: PagedKV, ctx_lens, starts, parents, max_ctx, max_nodes
     sees positions [0, ctx_lens[s]), itself and its ancestors: parents[row] is
     its parent's index in the request (-1: a root).  max_ctx bounds ctx_lens +
     nodes, max_nodes the nodes of a request (<= 256).  fp32 or fp16 queries
-    over an fp16 cache, bf16 over bf16; rows that see nothing get zeros."""
+    over an fp16 cache, bf16 over bf16; rows that see nothing get zeros.  workspace:
+    scratch of calls on one stream (this thread's for the stream if not given)."""
     d = kv.dims
     T, D, kp, vp, table = q.shape[0], d.head_dim, kv.k, kv.v, kv.page_table
     S, shape, pages = ctx_lens.numel(), table.shape, kp.shape
